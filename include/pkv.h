@@ -123,6 +123,40 @@ int pkv_rope_append_f32(void* q, const void* k, const void* v, const int* positi
                         const float* sin_table, const int* slots, void* k_cache, void* v_cache, int n_tokens,
                         int q_heads, int kv_heads, int head_dim, pkv_stream stream);
 
+/* ---------------------------------------------- QK norm + RoPE + append ----
+ * pkv_rope_append_* for models that norm the heads of q and k before the rotation: one
+ * pass over the projections' output instead of a norm launch for q, one for k, and the
+ * fused rotation and append.
+ *   y = x / sqrt(mean(x^2) + eps) * weight   per head of q (q_weight) and of k (k_weight)
+ *   q_out[t][h][:]          <- rope(y of q[t][h], positions[t])
+ *   k_cache[slots[t]][h][:] <- rope(y of k[t][h], positions[t])
+ *   v_cache[slots[t]][:]    <- v[t][:]
+ * with the rotation and the tables of pkv_rope_append_*.  fp32 arithmetic, one rounding
+ * to the element type at the end.  Weights are [head_dim], of the element type.
+ * q, k and v rows are q_stride, k_stride and v_stride ELEMENTS apart, so they may be
+ * column ranges of one projection's output; q_out is [n_tokens][q_heads*head_dim], and
+ * may be q itself if q's rows are contiguous (no other overlap is allowed).
+ * Padded steps: a row whose position is outside [0, max_positions) (rows of the tables)
+ * is neither read nor written; a row whose slot is outside [0, n_slots) (pool rows)
+ * gets its q_out, but no K/V.  Slots of a call are distinct.  head_dim must be even.
+ * No llm-engine counterpart (its models have no such norms); the rotation is
+ * include/engine/ops.h:56-68, the append src/kernels/store_kv.cu:20-36. */
+int pkv_qk_norm_rope_append_f16(const void* q, const void* k, const void* v, long long q_stride, long long k_stride,
+                                long long v_stride, const void* q_weight, const void* k_weight, float eps,
+                                const int* positions, const float* cos_table, const float* sin_table, int max_positions,
+                                const int* slots, void* q_out, void* k_cache, void* v_cache, long long n_slots,
+                                int n_tokens, int q_heads, int kv_heads, int head_dim, pkv_stream stream);
+int pkv_qk_norm_rope_append_bf16(const void* q, const void* k, const void* v, long long q_stride, long long k_stride,
+                                 long long v_stride, const void* q_weight, const void* k_weight, float eps,
+                                 const int* positions, const float* cos_table, const float* sin_table, int max_positions,
+                                 const int* slots, void* q_out, void* k_cache, void* v_cache, long long n_slots,
+                                 int n_tokens, int q_heads, int kv_heads, int head_dim, pkv_stream stream);
+int pkv_qk_norm_rope_append_f32(const void* q, const void* k, const void* v, long long q_stride, long long k_stride,
+                                long long v_stride, const void* q_weight, const void* k_weight, float eps,
+                                const int* positions, const float* cos_table, const float* sin_table, int max_positions,
+                                const int* slots, void* q_out, void* k_cache, void* v_cache, long long n_slots,
+                                int n_tokens, int q_heads, int kv_heads, int head_dim, pkv_stream stream);
+
 /* ----------------------------------------------------- decode attention ----
  * Paged decode attention.  Replaces engine::launch_attention_decode and
  * engine::launch_attention_decode_gqa (include/engine/cuda_kernels.h:48-62,

@@ -28,7 +28,7 @@ class DecodePlan(C.Structure):
                 ("num_blocks", C.c_int), ("cluster", C.c_int), ("cluster_wide", C.c_int), ("cluster_least", C.c_int)]
 
 
-_vp, _i, _f, _sz, _u64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64
+_vp, _i, _f, _sz, _u64, _ll = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64, C.c_longlong
 
 # name -> (restype, argtypes); every symbol include/pkv.h declares.
 SIGNATURES = {
@@ -42,6 +42,8 @@ SIGNATURES = {
     **{f"pkv_mixed_attn_{s}": (_i, [_vp] * 8 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]) for s in ("f16", "bf16")},
     **{f"pkv_append_{s}": (_i, [_vp] * 5 + [_i, _i, _vp]) for s in ("f16", "bf16", "f32")},
     **{f"pkv_rope_append_{s}": (_i, [_vp] * 9 + [_i] * 4 + [_vp]) for s in ("f16", "bf16", "f32")},
+    **{f"pkv_qk_norm_rope_append_{s}": (_i, [_vp] * 3 + [_ll] * 3 + [_vp] * 2 + [_f] + [_vp] * 3 + [_i] + [_vp] * 4 + [_ll] + [_i] * 4 + [_vp])
+       for s in ("f16", "bf16", "f32")},
     "pkv_decode_workspace_bytes": (_sz, [_i] * 4),
     **{f"pkv_decode_attn_{s}": (_i, [_vp] * 8 + [_i] * 5 + [_f, _vp, _sz, _vp]) for s in ("f16", "bf16", "f32")},
     "pkv_decode_attn_bf16_builtin_scratch": (_i, [_vp] * 8 + [_i] * 5 + [_f, _vp]),

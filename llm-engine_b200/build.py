@@ -22,6 +22,7 @@ SOURCES = [
     "append.cu",
     "copy_blocks.cu",
     "rope_append.cu",
+    "qk_norm_rope.cu",
     "step_pack.cu",
     "peer_memory.cu",
     "error_mirror.cu",

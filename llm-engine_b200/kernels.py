@@ -8,6 +8,7 @@ is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 from . import _lib
@@ -81,6 +82,72 @@ def launch_rope_store_kv(q, k, v, positions, cos_table, sin_table, slots, k_cach
     st = call(_ptr(q), _ptr(k), _ptr(v), _ptr(positions), _ptr(cos_table), _ptr(sin_table),
               _ptr(slots), _ptr(k_cache), _ptr(v_cache), n_tokens, q_heads, kv_heads, head_dim,
               _stream(stream))
+    _lib.check(fn, st)
+
+
+def _rows(t, cols: int, what: str):
+    """(pointer, elements from one row to the next) of a [rows][cols] tensor whose rows may lie apart."""
+    if not t.is_cuda:
+        raise ValueError("paged-KV operators take CUDA tensors; there is no CPU path")
+    if t.dim() != 2 or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what} must be [rows][{cols}] with contiguous rows, not {tuple(t.shape)} with strides {tuple(t.stride())}")
+    return t.data_ptr(), t.stride(0)
+
+
+def _same(ref, *tensors):
+    """Every tensor has the element type of `ref` and lies on its device."""
+    for t in tensors:
+        if t.dtype != ref.dtype:
+            raise TypeError(f"element types differ: {t.dtype} and {ref.dtype}")
+    _on_device(ref, *tensors)
+
+
+def _on_device(ref, *tensors):
+    for t in tensors:
+        if t.device != ref.device:
+            raise ValueError(f"tensors on different devices: {t.device} and {ref.device}")
+
+
+def _ints(*tensors):
+    import torch
+    for t in tensors:
+        if t.dtype != torch.int32:
+            raise TypeError(f"index arrays are int32, not {t.dtype}")
+
+
+def _device_of(t):
+    """A context in which t's device is the current one (launches and their streams follow it)."""
+    import torch
+    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def launch_qk_norm_rope_store_kv(q, k, v, q_weight, k_weight, eps: float, positions, cos_table, sin_table, slots, q_out, k_cache,
+                                 v_cache, n_tokens: int, q_heads: int, kv_heads: int, head_dim: int, stream=None) -> None:
+    """launch_rope_store_kv for models that norm the heads of q and k first: RMS norm per head with its weight,
+    rotation, append, in one pass.  q, k and v are [rows][heads*head_dim] and may be column ranges of one
+    projection's output; q_out (contiguous) receives the rotated q.  Rows whose position is outside the tables are
+    left alone, rows whose slot is outside the pools bring no K/V (padded steps)."""
+    fn, call = _fn("pkv_qk_norm_rope_append_", k_cache)
+    q_dim, kv_dim = q_heads * head_dim, kv_heads * head_dim
+    _same(k_cache, q, k, v, q_weight, k_weight, q_out, v_cache)
+    _on_device(k_cache, positions, cos_table, sin_table, slots)
+    _ints(positions, slots)
+    if cos_table.dtype != sin_table.dtype or "float32" not in str(cos_table.dtype):
+        raise TypeError("cos and sin tables are float32")
+    if cos_table.shape != sin_table.shape or cos_table.dim() != 2 or cos_table.shape[1] != head_dim // 2:
+        raise ValueError(f"cos and sin tables must both be [positions][{head_dim // 2}]")
+    if q_weight.numel() != head_dim or k_weight.numel() != head_dim:
+        raise ValueError(f"norm weights must have head_dim = {head_dim} elements")
+    if min(q.shape[0], k.shape[0], v.shape[0], positions.numel(), slots.numel()) < n_tokens or q_out.numel() < n_tokens * q_dim:
+        raise ValueError(f"fewer rows than n_tokens = {n_tokens}")
+    n_slots = k_cache.numel() // max(kv_dim, 1)
+    if v_cache.numel() != k_cache.numel():
+        raise ValueError("K and V pools differ in size")
+    (qp, qs), (kp, ks), (vp, vs) = _rows(q, q_dim, "q"), _rows(k, kv_dim, "k"), _rows(v, kv_dim, "v")
+    with _device_of(k_cache):
+        st = call(qp, kp, vp, qs, ks, vs, _ptr(q_weight), _ptr(k_weight), C.c_float(eps), _ptr(positions), _ptr(cos_table),
+                  _ptr(sin_table), cos_table.shape[0], _ptr(slots), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), n_slots, n_tokens,
+                  q_heads, kv_heads, head_dim, _stream(stream))
     _lib.check(fn, st)
 
 

@@ -62,7 +62,8 @@ const char* pkv_last_error(void);
  * makes its warp or block wind down (tensor memory released, no trap) and leaves the
  * launch's output incomplete.  The record of it is a bit -- 1: a TMA producer never saw
  * its ring slot released; 2: a consumer never saw its tile arrive; 4: a prefill
- * pipeline wait; 8: a peer GPU's flag in the head-sharded exchange; 16: a block copy -- kept in two
+ * pipeline wait; 8: a peer GPU's flag in the head-sharded exchange; 16: a block copy; 32: a wait of
+ * the tile kernel (pkv_cross_attn_*, pkv_prefix_attn_*) -- kept in two
  * places: a device word, and a pinned host word the kernels store to.  The attention
  * entry points (pkv_decode_attn_*, the planned, fused, peer and mixed forms,
  * pkv_prefill_attn_*) look at the host word before they enqueue anything, and so do
@@ -440,6 +441,82 @@ int pkv_prefill_attn_f16(const void* q, const void* k_cache, const void* v_cache
                          const int* q_len, const int* ctx_len, void* out, int n_tokens, int n_seqs,
                          int max_q_len, int q_heads, int kv_heads, int head_dim, int block_size,
                          int num_blocks, float scale, pkv_stream stream);
+
+/* ------------------------------------ attention to an encoder's states, shared prefix ----
+ * Two forms of attention in which many rows see exactly the same keys, on one tensor-core
+ * kernel (16-bit K/V, head_dim 64 or 128, block_size a power of two >= 16; all other
+ * geometries of pkv_decode_attn_*, fp32 included, run on its kernels instead).  As with
+ * pkv_decode_plan_host, a step's work list is built once on the host and serves every
+ * layer's call.  No llm-engine counterparts; each (token, head) agrees with
+ * ref::paged_attention_head (include/engine/ops.h:87-111) over the keys named here.
+ *
+ * pkv_cross_*: attention to states of another sequence, of another length (an encoder's
+ * output), whose K and V rows lie in blocks of the pools like any others.  Sequence s has
+ * rows q_start[s] .. q_start[s] + q_len[s] - 1 of q / out (NULL q_start: one sequence
+ * behind the other) and kv_len[s] keys, at positions 0 .. kv_len[s] - 1 of the table at
+ * block_tables + table_offset[s]; every row sees all of them.  Without keys a row's output
+ * is zero; rows that belong to no sequence are left as they were; no row may belong to two.
+ *
+ * pkv_prefix_*: pkv_decode_attn_* for tokens whose sequences all begin with the same
+ * prefix_len positions in the same blocks (as KVCacheManager::allocate_prompt shares them,
+ * src/kv_cache/block_allocator.cpp:28-78).  The prefix is worked through once for all tokens
+ * together, through the table of one of them, each token's other keys as ever.  The index
+ * arrays are those of pkv_decode_attn_*, with the whole tables; that they agree on the
+ * prefix is the caller's word.  A token whose position lies inside the prefix sees the keys up
+ * to its own position only.  (pkv_decode_plan_host_shared finds common prefixes by itself and
+ * reads them once per four tokens.)
+ *
+ * A plan belongs to the host lengths it was made from and to the workspace it was uploaded
+ * to (256-byte aligned; pkv_cross_workspace_bytes / pkv_prefix_workspace_bytes are enough for
+ * any lengths); it serves any number of calls on one stream, captured ones included.  Calls
+ * that may overlap need a workspace each.  h_staging (at least pkv_segment_staging_bytes, pinned
+ * for a truly asynchronous copy) must stay untouched until the upload has run; the _image forms
+ * write it and leave the copy of plan->image_bytes to the start of the workspace to the caller.
+ * elem_bytes: 2 for f16 and bf16, 4 for f32.  A caller that knows the pool size sets
+ * plan->num_blocks, and a wrong block id then reads zeros in the TMA kernels.  The fields behind
+ * num_blocks are the library's. */
+typedef struct pkv_segment_plan {
+  int kind, n_tokens, q_heads, kv_heads, head_dim, block_size, elem_bytes;
+  int num_blocks;
+  int n_tiles, n_items, n_merged, n_parts;   /* tensor-core items, decode items, tokens that the merge writes, partials */
+  int cluster, cluster_least;
+  size_t image_bytes, workspace_bytes;
+  size_t off_seq, off_pos, off_rows, off_items, off_tiles, off_merge, off_ml, off_acc;
+} pkv_segment_plan;
+
+size_t pkv_cross_workspace_bytes(int n_tokens, int q_heads, int kv_heads, int head_dim);
+size_t pkv_prefix_workspace_bytes(int n_tokens, int q_heads, int kv_heads, int head_dim);
+size_t pkv_segment_staging_bytes(int n_tokens, int q_heads, int kv_heads);
+int pkv_cross_plan_host(const int* h_q_start, const int* h_q_len, const int* h_kv_len, int n_seqs, int n_tokens, int q_heads,
+                        int kv_heads, int head_dim, int block_size, int elem_bytes, void* h_staging, size_t staging_bytes,
+                        void* workspace, size_t workspace_bytes, pkv_stream stream, pkv_segment_plan* plan);
+int pkv_cross_plan_host_image(const int* h_q_start, const int* h_q_len, const int* h_kv_len, int n_seqs, int n_tokens, int q_heads,
+                              int kv_heads, int head_dim, int block_size, int elem_bytes, void* h_staging, size_t staging_bytes,
+                              size_t workspace_bytes, pkv_segment_plan* plan);
+int pkv_prefix_plan_host(const int* h_token_pos, int n_tokens, int prefix_len, int q_heads, int kv_heads, int head_dim,
+                         int block_size, int elem_bytes, void* h_staging, size_t staging_bytes, void* workspace,
+                         size_t workspace_bytes, pkv_stream stream, pkv_segment_plan* plan);
+int pkv_prefix_plan_host_image(const int* h_token_pos, int n_tokens, int prefix_len, int q_heads, int kv_heads, int head_dim,
+                               int block_size, int elem_bytes, void* h_staging, size_t staging_bytes, size_t workspace_bytes,
+                               pkv_segment_plan* plan);
+int pkv_cross_attn_f16(const pkv_segment_plan* plan, const void* q, const void* k_cache, const void* v_cache,
+                       const int* block_tables, const int* table_offset, void* out, float scale, void* workspace,
+                       size_t workspace_bytes, pkv_stream stream);
+int pkv_cross_attn_bf16(const pkv_segment_plan* plan, const void* q, const void* k_cache, const void* v_cache,
+                        const int* block_tables, const int* table_offset, void* out, float scale, void* workspace,
+                        size_t workspace_bytes, pkv_stream stream);
+int pkv_cross_attn_f32(const pkv_segment_plan* plan, const void* q, const void* k_cache, const void* v_cache,
+                       const int* block_tables, const int* table_offset, void* out, float scale, void* workspace,
+                       size_t workspace_bytes, pkv_stream stream);
+int pkv_prefix_attn_f16(const pkv_segment_plan* plan, const void* q, const void* k_cache, const void* v_cache,
+                        const int* block_tables, const int* table_offset, const int* token_seq, void* out, float scale,
+                        void* workspace, size_t workspace_bytes, pkv_stream stream);
+int pkv_prefix_attn_bf16(const pkv_segment_plan* plan, const void* q, const void* k_cache, const void* v_cache,
+                         const int* block_tables, const int* table_offset, const int* token_seq, void* out, float scale,
+                         void* workspace, size_t workspace_bytes, pkv_stream stream);
+int pkv_prefix_attn_f32(const pkv_segment_plan* plan, const void* q, const void* k_cache, const void* v_cache,
+                        const int* block_tables, const int* table_offset, const int* token_seq, void* out, float scale,
+                        void* workspace, size_t workspace_bytes, pkv_stream stream);
 
 /* ----------------------------------------------------------- block copy ----
  * Prefix-cache copy-on-write block copy.  No llm-engine counterpart (it shares

@@ -28,6 +28,14 @@ class DecodePlan(C.Structure):
                 ("num_blocks", C.c_int), ("cluster", C.c_int), ("cluster_wide", C.c_int), ("cluster_least", C.c_int)]
 
 
+class SegmentPlan(C.Structure):
+    """Mirror of struct pkv_segment_plan."""
+    _fields_ = [(n, C.c_int) for n in ("kind", "n_tokens", "q_heads", "kv_heads", "head_dim", "block_size", "elem_bytes", "num_blocks",
+                                       "n_tiles", "n_items", "n_merged", "n_parts", "cluster", "cluster_least")] + \
+               [(n, C.c_size_t) for n in ("image_bytes", "workspace_bytes", "off_seq", "off_pos", "off_rows", "off_items", "off_tiles",
+                                          "off_merge", "off_ml", "off_acc")]
+
+
 _vp, _i, _f, _sz, _u64, _ll = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64, C.c_longlong
 
 # name -> (restype, argtypes); every symbol include/pkv.h declares.
@@ -64,6 +72,15 @@ SIGNATURES = {
     **{f"pkv_decode_attn_planned_{s}": (_i, [C.POINTER(DecodePlan)] + [_vp] * 8 + [_i, _f, _vp, _sz, _vp])
        for s in ("f16", "bf16", "f32")},
     **{f"pkv_prefill_attn_{s}": (_i, [_vp] * 9 + [_i] * 8 + [_f, _vp]) for s in ("f16", "bf16")},
+    "pkv_cross_workspace_bytes": (_sz, [_i] * 4),
+    "pkv_prefix_workspace_bytes": (_sz, [_i] * 4),
+    "pkv_segment_staging_bytes": (_sz, [_i] * 3),
+    "pkv_cross_plan_host": (_i, [_vp] * 3 + [_i] * 7 + [_vp, _sz, _vp, _sz, _vp, C.POINTER(SegmentPlan)]),
+    "pkv_cross_plan_host_image": (_i, [_vp] * 3 + [_i] * 7 + [_vp, _sz, _sz, C.POINTER(SegmentPlan)]),
+    "pkv_prefix_plan_host": (_i, [_vp] + [_i] * 7 + [_vp, _sz, _vp, _sz, _vp, C.POINTER(SegmentPlan)]),
+    "pkv_prefix_plan_host_image": (_i, [_vp] + [_i] * 7 + [_vp, _sz, _sz, C.POINTER(SegmentPlan)]),
+    **{f"pkv_cross_attn_{s}": (_i, [C.POINTER(SegmentPlan)] + [_vp] * 6 + [_f, _vp, _sz, _vp]) for s in ("f16", "bf16", "f32")},
+    **{f"pkv_prefix_attn_{s}": (_i, [C.POINTER(SegmentPlan)] + [_vp] * 7 + [_f, _vp, _sz, _vp]) for s in ("f16", "bf16", "f32")},
     **{f"pkv_copy_blocks_{s}": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]) for s in ("f16", "bf16", "f32")},
     "pkv_copy_blocks_layers": (_i, [_vp, _i, _vp, _i, _sz, _vp]),
     "pkv_step_pack_device": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp]),

@@ -28,6 +28,7 @@ SOURCES = [
     "error_mirror.cu",
     "decode_attn.cu",
     "prefill_attn.cu",
+    "segment_attn.cu",
     "engine_shim.cu",
 ]
 

@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "decode_attn.cuh"
+#include "decode_list.hpp"
 #include "decode_tma.cuh"
 #include "launch_util.hpp"
 #include "status.hpp"
@@ -22,6 +23,7 @@ static __device__ __align__(256) unsigned char g_builtin_scratch[kBuiltinScratch
 namespace pkv {
 int prefill_read_flags(unsigned int* flags);  // prefill_attn.cu
 int copy_read_flags(unsigned int* flags);     // copy_blocks.cu
+int tile_read_flags(unsigned int* flags);     // segment_attn.cu
 template <typename T>
 int prefill_launch(const void* q, const void* k_cache, const void* v_cache, const int* block_tables,
                    const int* table_offset, const int* q_start, const int* q_len, const int* ctx_len, void* out,
@@ -970,6 +972,64 @@ int mixed_attn(const void* q, const void* kc, const void* vc, const int* bt, con
 }
 
 }  // namespace
+
+// ---- for lists of work items made elsewhere (decode_list.hpp) ----
+int decode_sms() { return persistent_sms(); }
+int decode_max_extra(int kv_heads) { return (tuning().target_ctas + kv_heads - 1) / kv_heads; }
+PlanLimits decode_plan_limits(int extra, int q_heads, int kv_heads, int head_dim) {
+  return plan_limits(extra, q_heads, kv_heads, head_dim, true, true);
+}
+int decode_cluster_size(int n_tokens, int longest, int q_heads, int kv_heads, int head_dim, int* least) {
+  if (!cluster_form_enabled() || (head_dim != 64 && head_dim != 128) || q_heads / kv_heads > 8) return 0;
+  const long long pairs = static_cast<long long>(n_tokens) * kv_heads;
+  const long long resident = static_cast<long long>(persistent_sms()) * (head_dim == 64 ? 3 : 2);
+  const int max_keys = tuning().cluster_max_keys * 64 / head_dim;    // as many bytes per warp
+  if (pairs * 2 > resident) return 0;
+  int cs = static_cast<int>(std::min<long long>(8, resident / pairs));
+  if (tuning().cluster_size >= 2 && tuning().cluster_size < cs) cs = tuning().cluster_size;
+  while (cs > 2 && !cluster_size_ok(cs)) --cs;                       // 8, 4, 3 or 2 blocks: what the landing areas are sized for
+  if ((longest + 4 * cs - 1) / (4 * cs) > max_keys) return 0;
+  *least = (longest + 4 * max_keys - 1) / (4 * max_keys);
+  return cs;
+}
+
+template <typename T>
+bool decode_log2_domain(int q_heads, int kv_heads, int head_dim, int block_size, float scale) {
+  DecodeArgs a;
+  fill_args(a, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 1, q_heads, kv_heads, head_dim, block_size, scale);
+  if (IsF32<T>::value) return false;
+  return (head_dim == 64 || head_dim == 128) && a.group <= 16 && a.bs_log2 >= 0;
+}
+
+template <typename T>
+int decode_listed(const DecodeList& l, cudaStream_t stream, bool* merged) {
+  *merged = false;
+  DecodeArgs a;
+  fill_args(a, l.q, l.k_cache, l.v_cache, l.block_tables, l.table_offset, l.token_seq, l.token_pos, l.out, l.n_tokens, l.q_heads,
+            l.kv_heads, l.head_dim, l.block_size, l.scale);
+  a.host_err = l.host_err;
+  if (l.pool_rows > 0) a.pool_rows = l.pool_rows;
+  if (l.cluster >= 2 && a.group <= 8 && tma_path<T>(a)) {
+    const int st = launch_tma_cluster<T>(a, l.cluster, l.cluster_least, stream, merged);
+    if (st != PKV_OK || *merged) return st;
+  }
+  a.header = l.header;
+  a.items = l.items;
+  a.part_ml = l.part_ml;
+  a.part_acc = l.part_acc;
+  a.direct = 0;
+  a.wait_last = l.behind_tiles ? 1 : 0;
+  const long long units = std::min<long long>(static_cast<long long>(l.n_items) * l.kv_heads, 0x7fffffffll);
+  bool log2_domain;
+  return launch_decode_main<T>(a, static_cast<int>(units), stream, &log2_domain);
+}
+#define PKV_DECODE_LISTED(T)                                              \
+  template int decode_listed<T>(const DecodeList&, cudaStream_t, bool*);  \
+  template bool decode_log2_domain<T>(int, int, int, int, float);
+PKV_DECODE_LISTED(__half)
+PKV_DECODE_LISTED(__nv_bfloat16)
+PKV_DECODE_LISTED(float)
+
 }  // namespace pkv
 
 using namespace pkv;
@@ -982,11 +1042,12 @@ int pkv_debug_device_flags(unsigned int* flags) {
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_pkv_device_error, sizeof(v));
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_pkv_device_error, &zero, sizeof(zero));
   if (e != cudaSuccess) return fail(PKV_E_CUDA, "pkv_debug_device_flags: %s", cudaGetErrorString(e));
-  unsigned int pf = 0, cf = 0;
+  unsigned int pf = 0, cf = 0, tf = 0;
   int st = pkv::prefill_read_flags(&pf);
   if (st == PKV_OK) st = pkv::copy_read_flags(&cf);
+  if (st == PKV_OK) st = pkv::tile_read_flags(&tf);
   if (st != PKV_OK) return st;
-  *flags = v | pf | cf | pkv::take_error_mirror();
+  *flags = v | pf | cf | tf | pkv::take_error_mirror();
   return PKV_OK;
 }
 
@@ -1109,19 +1170,9 @@ static int plan_host_image(const char* fn, const int* h_token_pos, int n_tokens,
   // once, and no warp of a cluster would get more than a few slabs, the attention call runs as clusters
   // and merges inside the launch (the image above stays valid: the call falls back to it if the device
   // turns the cluster launch down).
-  if (cluster_form_enabled() && np > 0 && (head_dim == 64 || head_dim == 128) && q_heads / kv_heads <= 8) {
-    const long long pairs = static_cast<long long>(n_tokens) * kv_heads;
-    const long long resident = static_cast<long long>(persistent_sms()) * (head_dim == 64 ? 3 : 2);
-    const int max_keys = tuning().cluster_max_keys * 64 / head_dim;    // as many bytes per warp
-    if (pairs * 2 <= resident) {
-      int cs = static_cast<int>(std::min<long long>(8, resident / pairs));
-      if (tuning().cluster_size >= 2 && tuning().cluster_size < cs) cs = tuning().cluster_size;
-      while (cs > 2 && !cluster_size_ok(cs)) --cs;       // 8, 4, 3 or 2 blocks: what the landing areas are sized for
-      if ((max_len + 4 * cs - 1) / (4 * cs) <= max_keys) {
-        (head_dim == 64 ? plan->cluster : plan->cluster_wide) = cs;
-        plan->cluster_least = (max_len + 4 * max_keys - 1) / (4 * max_keys);
-      }
-    }
+  if (np > 0) {
+    const int cs = decode_cluster_size(n_tokens, max_len, q_heads, kv_heads, head_dim, &plan->cluster_least);
+    if (cs > 0) (head_dim == 64 ? plan->cluster : plan->cluster_wide) = cs;
   }
   return PKV_OK;
 }

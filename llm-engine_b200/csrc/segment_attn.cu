@@ -1,0 +1,915 @@
+// Attention without a causal mask over paged K/V (include/pkv.h, "attention to an encoder's states" and "shared
+// prefix"): the tile kernel on the 5th-generation tensor cores, the merge kernel, and the entry points.  How a step is
+// cut into work for them and for the decode kernels is in segment_plan.hpp.
+//
+//   out[t][h] = sum_j p_j V[j] / sum_j p_j,   p_j = exp(scale q[t][h] . K[j] - m),   m = the row's maximum
+//
+// A tile item is up to 256 rows (token, query head of one kv head's group) that all see the same keys, walked in tiles of
+// 128.  The rows are two groups of 128, each with its own scores S (128 columns of tensor memory) and output O (head_dim
+// columns); a K or V tile is fetched once for both.  While one group's scores are turned into probabilities by its
+// four warps, the tensor cores work on the other group: a 128 x 128 x 128 product takes 512 cycles, the 16,384
+// exponentials of a group's tile 1,024, so at head_dim 128 (two products) both pipes can be busy all the time, and at
+// head_dim 64 the exponentials decide.
+//
+//   warps 0-3, 4-7  softmax of group 0, 1: thread = row.  128 scores to registers, maximum, exponentials, sum; P goes
+//                   back as 16-bit pairs over the first 64 columns of S, where the second product reads its A operand.
+//                   O stays in tensor memory and is rescaled only when a row's maximum has grown by more than 2^8.
+//   warp 8          TMA: K and V tiles through the block table into a ring (boxes of up to 128 slots x 128 bytes).
+//   warp 9          issues the products, one thread: S = Q K^T for either group, then O += P V and the next S in turns.
+//   warp 10         gathers the next item's rows of Q, whatever tokens and heads they are.
+//
+// An item of at most 128 rows whose keys are many runs both groups over the same rows, every other key tile each (`halves`).
+// P is rounded to 16 bits for the second product (the sums are of the unrounded ones), as the operands of the
+// tensor cores are; scores, sums and accumulators are fp32.
+//
+// Blocks are persistent, one on an SM, and take the list of items in a serpentine, longest first.  Every wait is
+// bounded: one that runs out sets bit 32 of the error word and the block winds down.
+#include <algorithm>
+#include <new>
+#include <type_traits>
+#include <vector>
+
+#include "common.cuh"
+#include "decode_list.hpp"
+#include "launch_util.hpp"
+#include "segment_plan.hpp"
+#include "status.hpp"
+#include "tcgen05.cuh"
+#include "tma_util.hpp"
+
+namespace pkv {
+
+__device__ unsigned int g_pkv_tile_error = 0;
+constexpr unsigned kErrTileWait = 32u;
+
+unsigned int* error_mirror(bool create);                 // error_mirror.cu
+int check_error_mirror(const char* fn, unsigned int bits = ~0u);
+
+namespace {
+
+constexpr int kTileThreads = 384;                        // 12 warps, the last one idle: registers are split by fours
+// Registers a thread of the softmax warps and of the others; launched with 168 each (2 x 208 + 80 <= 3 x 168).
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
+constexpr int kProducer = 8, kIssuer = 9, kGatherer = 10;
+constexpr int kBlockBytes = 128 * 128;                   // 128 rows x 64 16-bit elements: one operand block
+constexpr uint32_t kGroupCols = 256, kColO = 128;        // tensor memory of a group: S, then O
+constexpr float kRescale = 8.f;                          // in log2 units: P stays below 2^8
+constexpr int kMinTileTokens = 4;                        // sequences with fewer tokens go to the decode kernels
+constexpr int kMinPrefixTokens = 2;                      // batches of fewer tokens behind the prefix, too
+
+template <int D> struct TileSmem {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTile = kHalves * kBlockBytes;    // a K or V tile, or one group's Q
+  static constexpr int kStages = D == 64 ? 8 : 5;
+  static constexpr int kRing = 2 * kTile;
+  static constexpr int kBytes = kRing + kStages * kTile + 1024;
+};
+
+struct TileArgs {
+  const void* q;
+  const int *block_tables, *table_offset, *token_seq;
+  const RowToken* rows;
+  const TileItem* tiles;
+  void* out;
+  float *part_ml, *part_acc;
+  int n_work;                        // items x kv heads
+  int q_heads, kv_heads, group;
+  int block_size, bs_log2, box_log2; // a TMA box is 1 << box_log2 slots
+  float scale;
+  float ml_scale;                    // what partial maxima are multiplied with: scale, or scale log2 e
+  unsigned int* host_err;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// (a0, a1) * (s, s) + (n, n) and (a0, a1) + (b0, b1), two at a time
+__device__ __forceinline__ void fma2(float a0, float a1, float s, float n, float& r0, float& r1) {
+  asm("{\n .reg .b64 ra, rs, rn, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rs, {%4, %4};\n mov.b64 rn, {%5, %5};\n"
+      " fma.rn.f32x2 rd, ra, rs, rn;\n mov.b64 {%0, %1}, rd;\n}\n"
+      : "=f"(r0), "=f"(r1)
+      : "f"(a0), "f"(a1), "f"(s), "f"(n));
+}
+__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
+  asm("{\n .reg .b64 ra, rb;\n mov.b64 ra, {%0, %1};\n mov.b64 rb, {%2, %3};\n add.rn.f32x2 ra, ra, rb;\n mov.b64 {%0, %1}, ra;\n}\n"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1));
+}
+
+// The r-th item of a block, or -1.
+__device__ __forceinline__ int work_at(int r, int n_work) {
+  const int G = static_cast<int>(gridDim.x), b = static_cast<int>(blockIdx.x);
+  const long long w = static_cast<long long>(r) * G + ((r & 1) ? G - 1 - b : b);
+  return w < n_work ? static_cast<int>(w) : -1;
+}
+__device__ __forceinline__ TileItem load_tile(const TileItem* p) {
+  const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
+  return TileItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    tile_attn_kernel(const TileArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using S = TileSmem<D>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t kInstrQK = tc::instruction(kBf16, kTileKeys, false), kInstrPV = tc::instruction(kBf16, D, true);
+  constexpr float kLog2e = 1.4426950408889634f;
+  constexpr int NS = S::kStages;
+
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  __shared__ __align__(8) unsigned long long bars[2 + 2 * NS + 6];
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t ring = base + S::kRing, bar0 = smem_u32(&bars[0]);
+  enum { Q_FULL = 0, Q_EMPTY = 1, KV_FULL = 2, KV_EMPTY = KV_FULL + NS, S_FULL = KV_EMPTY + NS, P_FULL = S_FULL + 2, O_FULL = P_FULL + 2 };
+  auto BAR = [&](int i) { return bar0 + 8u * i; };
+
+  if (threadIdx.x == 0) {
+    mbar_init(BAR(Q_FULL), 1);          // the gatherer, its copies done
+    mbar_init(BAR(Q_EMPTY), 1);         // commit after the item's last Q K^T
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(BAR(KV_FULL + i), 1);
+      mbar_init(BAR(KV_EMPTY + i), 1);  // commit after the last product that reads the stage
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(BAR(S_FULL + g), 1);    // commit after the group's Q K^T
+      mbar_init(BAR(P_FULL + g), 128);  // the group's softmax threads (32 at a time)
+      mbar_init(BAR(O_FULL + g), 1);    // commit after the group's last P V of an item
+    }
+    mbar_fence_init();
+  }
+  if (warp == kIssuer) tc::alloc<512>(smem_u32(&tmem_slot));
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  // The launch behind this one may be the decode kernel of the same call, which does not wait for this one before
+  // it reads (decode_list.hpp): it may start once everything before this launch is complete.
+  pdl_wait();
+  pdl_launch_dependents();
+
+  bool dead = false;
+  auto WAIT = [&](uint32_t bar, uint32_t parity) {
+    if (dead) return;
+    if (!mbar_wait(bar, parity)) {
+      dead = true;
+      atomicOr(&g_pkv_tile_error, kErrTileWait);
+      if (a.host_err) {
+        *reinterpret_cast<volatile unsigned int*>(a.host_err) = kErrTileWait;
+        __threadfence_system();
+      }
+    }
+  };
+
+  if (warp >= kProducer) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
+    if (warp == kProducer) {
+      // The entries of the ring for an item of n key tiles, in the order the products use them:
+      //   both groups on every tile   K0 V0 K1 V1 ...
+      //   every other tile each       K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1)
+      uint32_t e = 0;
+      const int box_rows = 1 << a.box_log2, boxes = kTileKeys >> a.box_log2;
+      for (int r = 0; !dead; ++r) {
+        const int w = work_at(r, a.n_work);
+        if (w < 0) break;
+        const TileItem it = load_tile(a.tiles + w / a.kv_heads);
+        const int kvh = w % a.kv_heads, n = (it.kv_len + kTileKeys - 1) / kTileKeys, end = it.kv_begin + it.kv_len;
+        const int* tbl = a.block_tables + __ldg(a.table_offset + __ldg(a.token_seq + __ldg(&a.rows[it.tok0].token)));
+        auto tile_of = [&](int i) { return !it.halves ? i >> 1 : i < 2 ? i : i == 2 * n - 1 ? n - 1 : (i & 1) ? (i + 1) >> 1 : (i - 2) >> 1; };
+        auto is_v = [&](int i) { return !it.halves ? (i & 1) != 0 : i >= 2 && (i == 2 * n - 1 || (i & 1) == 0); };
+        auto row_of = [&](int i) {           // pool row of this lane's box
+          const int pos = it.kv_begin + tile_of(i) * kTileKeys + (lane << a.box_log2);
+          if (lane >= boxes || pos >= end) return 0;
+          return (__ldg(tbl + (pos >> a.bs_log2)) << a.bs_log2) + (pos & (a.block_size - 1));
+        };
+        int y = row_of(0);
+        for (int i = 0; i < 2 * n; ++i, ++e) {
+          const int y_next = i + 1 < 2 * n ? row_of(i + 1) : 0;
+          const int st = static_cast<int>(e % NS), left = it.kv_len - tile_of(i) * kTileKeys;
+          const int valid = min(boxes, (left + box_rows - 1) >> a.box_log2);
+          if (lane == 0) {
+            WAIT(BAR(KV_EMPTY + st), ((e / NS) & 1) ^ 1);
+            if (!dead) mbar_arrive_expect_tx(BAR(KV_FULL + st), static_cast<uint32_t>(valid * box_rows) * 128u * S::kHalves);
+          }
+          dead = __shfl_sync(0xffffffffu, dead ? 1 : 0, 0) != 0;
+          if (dead) break;
+          if (lane < valid) {
+            const uint32_t dst = ring + st * S::kTile + (lane << a.box_log2) * 128;
+            const CUtensorMap* map = is_v(i) ? &vmap : &kmap;
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h) tma_load_2d(dst + h * kBlockBytes, map, kvh * D + h * 64, y, BAR(KV_FULL + st));
+          }
+          __syncwarp();
+          y = y_next;
+        }
+      }
+      // whatever this warp has sent for has arrived before the block leaves
+      if (lane == 0) {
+        for (uint32_t i = e > NS ? e - NS : 0; i < e; ++i) mbar_wait(BAR(KV_FULL + i % NS), (i / NS) & 1);
+      }
+      __syncwarp();
+    } else if (warp == kGatherer) {
+      constexpr int kRowBytes = D * 2;
+      const int half = lane & 7;                                   // 16-byte piece of a 128-byte operand row
+      for (int r = 0; !dead; ++r) {
+        const int w = work_at(r, a.n_work);
+        if (w < 0) break;
+        const TileItem it = load_tile(a.tiles + w / a.kv_heads);
+        const int kvh = w % a.kv_heads;
+        if (lane == 0) WAIT(BAR(Q_EMPTY), (r & 1) ^ 1);
+        dead = __shfl_sync(0xffffffffu, dead ? 1 : 0, 0) != 0;
+        if (dead) break;
+        const unsigned char* q = static_cast<const unsigned char*>(a.q);
+        for (int row0 = 0; row0 < (it.rows > 128 ? 256 : 128); row0 += 32) {
+          unsigned long long src = 0;
+          if (row0 + lane < it.rows) {
+            const int f = it.f0 + row0 + lane, t = f / a.group;
+            const int token = __ldg(&a.rows[it.tok0 + t].token);
+            src = reinterpret_cast<unsigned long long>(q + (static_cast<size_t>(token) * a.q_heads + kvh * a.group + (f - t * a.group)) * kRowBytes);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row = row0 + 4 * i + (lane >> 3);
+            const unsigned long long from = __shfl_sync(0xffffffffu, src, 4 * i + (lane >> 3));
+            const uint32_t dst = base + (row >> 7) * S::kTile + (row & 127) * 128 + ((half ^ (row & 7)) << 4);
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)
+              cp_async16(dst + h * kBlockBytes, from ? reinterpret_cast<const unsigned char*>(from) + h * 128 + half * 16 : q, from ? 16 : 0);
+          }
+        }
+        cp_async_commit();
+        cp_async_wait_all();
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(Q_FULL));
+      }
+    } else if (warp == kIssuer) {
+      if (lane == 0) {
+        uint32_t e = 0, done[2] = {0, 0};                          // ring entries; key tiles of either group, over all items
+        for (int r = 0; !dead; ++r) {
+          const int w = work_at(r, a.n_work);
+          if (w < 0) break;
+          const TileItem it = load_tile(a.tiles + w / a.kv_heads);
+          const int n = (it.kv_len + kTileKeys - 1) / kTileKeys;
+          WAIT(BAR(Q_FULL), r & 1);
+          // waits for the ring entry and returns where it lies
+          auto full = [&](uint32_t entry) {
+            WAIT(BAR(KV_FULL + entry % NS), (entry / NS) & 1);
+            tc::fence_after();
+            return ring + (entry % NS) * S::kTile;
+          };
+          auto scores = [&](int g, uint32_t k_addr) {
+            const uint64_t qd = tc::operand(base + (it.halves ? 0 : g) * S::kTile), kd = tc::operand(k_addr);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+              const uint64_t step = static_cast<uint64_t>((ks >> 2) * (kBlockBytes >> 4) + (ks & 3) * 2);
+              tc::mma_ss(tmem + g * kGroupCols, qd + step, kd + step, kInstrQK, ks > 0);
+            }
+            tc::commit(BAR(S_FULL + g));
+          };
+          // The group's S is overwritten by its next scores only behind these products: those of one thread run in order.
+          auto values = [&](int g, uint32_t v_addr, bool first) {
+            WAIT(BAR(P_FULL + g), done[g] & 1);
+            ++done[g];
+            tc::fence_after();
+            const uint64_t vd = tc::operand(v_addr, kBlockBytes);
+#pragma unroll
+            for (int kk = 0; kk < kTileKeys / 16; ++kk)
+              tc::mma_ts(tmem + g * kGroupCols + kColO, tmem + g * kGroupCols + kk * 8, vd + kk * (2048 >> 4), kInstrPV, !(first && kk == 0));
+          };
+          if (!it.halves) {
+            const int last = it.rows > 128 ? 1 : 0;                // last group
+            uint32_t k_addr = full(e);
+            for (int g = 0; g <= last; ++g) scores(g, k_addr);
+            tc::commit(BAR(KV_EMPTY + e % NS));
+            if (n == 1) tc::commit(BAR(Q_EMPTY));
+            ++e;
+            for (int j = 0; j < n && !dead; ++j) {
+              const bool more = j + 1 < n;
+              const uint32_t v_addr = full(e);
+              for (int g = 0; g <= last; ++g) {
+                values(g, v_addr, j == 0);
+                if (g == last) tc::commit(BAR(KV_EMPTY + e % NS));
+                if (!more) { tc::commit(BAR(O_FULL + g)); continue; }
+                if (g == 0) k_addr = full(e + 1);
+                scores(g, k_addr);
+                if (g == last) tc::commit(BAR(KV_EMPTY + (e + 1) % NS));
+              }
+              if (j + 2 == n) tc::commit(BAR(Q_EMPTY));
+              e += more ? 2 : 1;
+            }
+          } else {
+            for (int g = 0; g < 2; ++g, ++e) {
+              scores(g, full(e));
+              tc::commit(BAR(KV_EMPTY + e % NS));
+            }
+            if (n == 2) tc::commit(BAR(Q_EMPTY));
+            for (int t = 0; t < n && !dead; ++t) {
+              const int g = t & 1;
+              const uint32_t v_addr = full(e);
+              values(g, v_addr, t < 2);
+              tc::commit(BAR(KV_EMPTY + e % NS));
+              ++e;
+              if (t + 2 < n) {
+                scores(g, full(e));
+                tc::commit(BAR(KV_EMPTY + e % NS));
+                ++e;
+                if (t + 3 == n) tc::commit(BAR(Q_EMPTY));
+              } else {
+                tc::commit(BAR(O_FULL + g));
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
+    // ---- softmax: thread = row of its group = lane of tensor memory ----
+    const int g = warp >> 2, r_in = threadIdx.x & 127;
+    const uint32_t t_s = tmem + g * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16), t_o = t_s + kColO;
+    const float sl2 = a.scale * kLog2e;
+    uint32_t e0 = 0, done = 0, finished = 0;                     // ring entries before this item; the group's key tiles and items
+    for (int r = 0; !dead; ++r) {
+      const int w = work_at(r, a.n_work);
+      if (w < 0) break;
+      const TileItem it = load_tile(a.tiles + w / a.kv_heads);
+      const int kvh = w % a.kv_heads, n = (it.kv_len + kTileKeys - 1) / kTileKeys;
+      const uint32_t last_v = e0 + 2 * n - 1;                    // ring entry of the last V tile
+      e0 += 2 * n;
+      const int row = it.halves ? r_in : g * 128 + r_in;         // row of the item
+      const bool mine = row < it.rows;
+      RowToken rt{0, 0};
+      int head = 0;
+      if (mine) {
+        const int f = it.f0 + row, t = f / a.group;
+        const int2 x = __ldg(reinterpret_cast<const int2*>(a.rows + it.tok0 + t));
+        rt = RowToken{x.x, x.y};
+        head = kvh * a.group + (f - t * a.group);
+      }
+      if (g == 1 && !it.halves && it.rows <= 128) {
+        if (it.pad && r_in < it.rows) {                          // the others of the segment leave two partials
+          const int f = it.f0 + r_in, t = f / a.group;
+          const size_t p = static_cast<size_t>(__ldg(&a.rows[it.tok0 + t].part_base) + it.part + 1) * a.q_heads + kvh * a.group + (f - t * a.group);
+          *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(-INFINITY, 0.f);
+        }
+        continue;
+      }
+      const bool working = (row & ~31) < it.rows;                // some row of this warp is the item's
+      float m_used = -INFINITY, l0 = 0.f, l1 = 0.f;
+      const int step = it.halves ? 2 : 1;
+      for (int t = it.halves ? g : 0; t < n; t += step, ++done) {
+        WAIT(BAR(S_FULL + g), done & 1);
+        tc::fence_after();
+        const int valid = it.kv_len - t * kTileKeys;             // keys of this tile, if fewer than kTileKeys
+        if (working) {
+          float sc[kTileKeys];
+#pragma unroll
+          for (int c = 0; c < kTileKeys; c += 32) tc::ld32(t_s + c, reinterpret_cast<uint32_t*>(sc) + c);
+          tc::wait_ld();
+          if (valid < kTileKeys) {
+#pragma unroll
+            for (int i = 0; i < kTileKeys; ++i)
+              if (i >= valid) sc[i] = -INFINITY;
+          }
+          float mx8[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) mx8[u] = fmaxf(sc[u], sc[8 + u]);
+#pragma unroll
+          for (int i = 16; i < kTileKeys; i += 16)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) mx8[u] = max3(mx8[u], sc[i + u], sc[i + 8 + u]);
+          const float mx = fmaxf(max3(mx8[0], mx8[1], mx8[2]), fmaxf(max3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+          if (t < step) {
+            m_used = mx;
+          } else if (__any_sync(0xffffffffu, (mx - m_used) * sl2 > kRescale)) {
+            // The group's product before this one is complete: its next scores, which have arrived, were issued behind it.
+            const float m_new = (mx - m_used) * sl2 > kRescale ? mx : m_used;
+            const float f = ex2((m_used - m_new) * sl2);
+            m_used = m_new;
+            l0 *= f;
+            l1 *= f;
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t v[32];
+              tc::ld32(t_o + c, v);
+              tc::wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+              tc::st32(t_o + c, v);
+            }
+          }
+          const float neg = -m_used * sl2;
+#pragma unroll
+          for (int c = 0; c < kTileKeys; c += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float x0, x1;
+              fma2(sc[c + 2 * i], sc[c + 2 * i + 1], sl2, neg, x0, x1);
+              x0 = ex2(x0);
+              x1 = ex2(x1);
+              add2(l0, l1, x0, x1);
+              pk[i] = pack2<T>(x0, x1);
+            }
+            tc::st16(t_s + c / 2, pk);
+          }
+        }
+        if (t == n - 1 && valid < kTileKeys && (g == 0 || it.halves)) {
+          // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring
+          // held.  Cleared, so that 0 * x stays 0.
+          WAIT(BAR(KV_FULL + last_v % NS), (last_v / NS) & 1);
+          if (r_in >= valid) {
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h) {
+              unsigned char* v = base_ptr + S::kRing + (last_v % NS) * S::kTile + h * kBlockBytes + r_in * 128;
+#pragma unroll
+              for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        }
+        if (working) tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_warp(BAR(P_FULL + g));
+      }
+      // ---- epilogue: the next item's first product cannot touch O before this thread has arrived with its P ----
+      WAIT(BAR(O_FULL + g), finished & 1);
+      ++finished;
+      tc::fence_after();
+      if (!working) continue;
+      const float l = l0 + l1;
+      if (it.part < 0) {
+        const float inv = 1.f / l;
+        T* o = static_cast<T*>(a.out) + (static_cast<size_t>(rt.token) * a.q_heads + head) * D;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          tc::ld32(t_o + c, v);
+          tc::wait_ld();
+          if (mine) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 x;
+              x.x = pack2<T>(__uint_as_float(v[i]) * inv, __uint_as_float(v[i + 1]) * inv);
+              x.y = pack2<T>(__uint_as_float(v[i + 2]) * inv, __uint_as_float(v[i + 3]) * inv);
+              x.z = pack2<T>(__uint_as_float(v[i + 4]) * inv, __uint_as_float(v[i + 5]) * inv);
+              x.w = pack2<T>(__uint_as_float(v[i + 6]) * inv, __uint_as_float(v[i + 7]) * inv);
+              *reinterpret_cast<uint4*>(o + c + i) = x;
+            }
+          }
+        }
+      } else {
+        const size_t p = static_cast<size_t>(rt.part_base + it.part + (it.halves ? g : 0)) * a.q_heads + head;
+        float* o = a.part_acc + p * D;
+        if (mine) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_used * a.ml_scale, l);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          tc::ld32(t_o + c, v);
+          tc::wait_ld();
+          if (mine) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(o + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+        }
+      }
+      tc::fence_before();
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == kIssuer) {
+    tc::fence_after();
+    tc::dealloc<512>(tmem);
+  }
+}
+
+// Folds each listed token's partials: thread = (row of the list, head, VEC dims).  Partials sit in L2; a batch of loads is in
+// flight before the first is used.
+constexpr int kMergeThreads = 256, kMergeBatch = 8;
+struct MergeArgs {
+  const MergeRow* rows;
+  int n_rows, q_heads, head_dim;
+  const float *part_ml, *part_acc;
+  void* out;
+};
+template <typename T, bool LOG2, int VEC>
+__global__ void __launch_bounds__(kMergeThreads) segment_merge_kernel(const MergeArgs a) {
+  pdl_launch_dependents();
+  const int per_head = a.head_dim / VEC;
+  const long long per_row = static_cast<long long>(a.q_heads) * per_head, i = blockIdx.x * static_cast<long long>(kMergeThreads) + threadIdx.x;
+  const long long row = i / per_row;
+  const bool live = row < a.n_rows;
+  int4 m = make_int4(0, 0, 0, 0);
+  if (live) m = __ldg(reinterpret_cast<const int4*>(a.rows) + row);      // part of the plan, complete before the kernels that wrote the partials began
+  pdl_wait();
+  if (!live) return;
+  const int at = static_cast<int>(i - row * per_row), head = at / per_head, d = (at - head * per_head) * VEC;
+  const MergeRow mr{m.x, m.y, m.z, m.w};
+  float run = -INFINITY, sum = 0.f, acc[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
+  for (int p0 = 0; p0 < mr.n_parts; p0 += kMergeBatch) {
+    float2 ml[kMergeBatch];
+    float x[kMergeBatch][VEC];
+#pragma unroll
+    for (int u = 0; u < kMergeBatch; ++u) {
+      ml[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[u][v] = 0.f;
+      if (p0 + u < mr.n_parts) {
+        const size_t p = static_cast<size_t>(mr.part_base + p0 + u) * a.q_heads + head;
+        ml[u] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + p);
+        if constexpr (VEC == 4) {
+          const float4 f = __ldcg(reinterpret_cast<const float4*>(a.part_acc + p * a.head_dim + d));
+          x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
+        } else {
+          x[u][0] = __ldcg(a.part_acc + p * a.head_dim + d);
+        }
+      }
+    }
+    float top = run;
+#pragma unroll
+    for (int u = 0; u < kMergeBatch; ++u) top = fmaxf(top, ml[u].x);
+    auto weight = [&](float m0) { return m0 == -INFINITY ? 0.f : LOG2 ? exp2f(m0 - top) : expf(m0 - top); };
+    const float keep = weight(run);
+    sum *= keep;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) acc[v] *= keep;
+#pragma unroll
+    for (int u = 0; u < kMergeBatch; ++u) {
+      const float f = weight(ml[u].x);
+      sum += f * ml[u].y;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) acc[v] += ml[u].x == -INFINITY ? 0.f : f * x[u][v];   // an empty partial's accumulator is not written
+    }
+    run = top;
+  }
+  const float inv = mr.n_parts > 0 ? 1.f / sum : 0.f;
+  T* o = static_cast<T*>(a.out) + (static_cast<size_t>(mr.token) * a.q_heads + head) * a.head_dim + d;
+  if constexpr (VEC == 4 && sizeof(T) == 2) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
+  } else if constexpr (VEC == 4) {
+    *reinterpret_cast<float4*>(o) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+  } else {
+    o[0] = Elem<T>::from_f32(acc[0] * inv);
+  }
+}
+
+// ---------------------------------------------------------------- launches ----
+template <typename T, int D>
+int launch_tiles(const TileArgs& a, const void* k_cache, const void* v_cache, uint64_t pool_rows, cudaStream_t stream) {
+  using S = TileSmem<D>;
+  auto kern = tile_attn_kernel<T, D>;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_device != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (e != cudaSuccess) return fail(PKV_E_CUDA, "tile_attn_kernel: cannot reserve %d bytes of shared memory: %s", S::kBytes, cudaGetErrorString(e));
+    configured_device = dev;
+  }
+  constexpr PoolElem elem = std::is_same<T, __half>::value ? PoolElem::kF16 : PoolElem::kBF16;
+  alignas(64) CUtensorMap kmap, vmap;
+  int st = make_pool_tensor_map(&kmap, k_cache, elem, a.kv_heads * D, 1u << a.box_log2, pool_rows);
+  if (st == PKV_OK) st = make_pool_tensor_map(&vmap, v_cache, elem, a.kv_heads * D, 1u << a.box_log2, pool_rows);
+  if (st != PKV_OK) return st;
+  launch_pdl(kern, dim3(static_cast<unsigned>(std::min(a.n_work, decode_sms()))), dim3(kTileThreads), S::kBytes, stream, a, kmap, vmap);
+  return check_launch("tile_attn_kernel");
+}
+
+int log2_floor(int x) {
+  int l = 0;
+  while ((2 << l) <= x) ++l;
+  return l;
+}
+
+struct SegmentOffsets { size_t seq, pos, rows, items, tiles, merge, image, ml, acc, total; };
+SegmentOffsets segment_offsets(const SegmentGeometry& g, size_t rows, size_t items, size_t first, size_t tiles, size_t merge, size_t parts) {
+  SegmentOffsets o;
+  size_t at = align256(sizeof(PlanHeader));
+  o.seq = at;   at = align256(at + sizeof(int) * static_cast<size_t>(g.n_tokens));
+  o.pos = at;   at = align256(at + sizeof(int) * static_cast<size_t>(g.n_tokens));
+  o.rows = at;  at = align256(at + sizeof(RowToken) * rows);
+  o.items = at; at = align256(at + sizeof(WorkItem) * items + sizeof(int) * first);
+  o.tiles = at; at = align256(at + sizeof(TileItem) * tiles);
+  o.merge = at; at = align256(at + sizeof(MergeRow) * merge);
+  o.image = at;
+  o.ml = at;    at = align256(at + sizeof(float) * 2 * parts * g.q_heads);
+  o.acc = at;   at = align256(at + sizeof(float) * parts * g.q_heads * g.head_dim);
+  o.total = at;
+  return o;
+}
+// For any step of these sizes: tiles of uncut segments, and one more item at most for every partial.
+SegmentOffsets segment_bounds(const SegmentGeometry& g, bool prefix) {
+  const size_t n = static_cast<size_t>(g.n_tokens), slots = static_cast<size_t>(tile_slots(g, decode_sms())) + (prefix ? n : 0);
+  const size_t tiles = n * g.group() / kTileRows + n + slots;
+  const size_t items = n + own_extra(g) + 2;
+  return segment_offsets(g, n, items, items + 1, tiles, n, static_cast<size_t>(most_parts(g, decode_sms(), prefix)));
+}
+
+int check_geometry(const char* fn, const SegmentGeometry& g) {
+  if (g.q_heads <= 0 || g.kv_heads <= 0 || g.head_dim <= 0 || g.block_size <= 0)
+    return fail(PKV_E_ARG, "%s: q_heads %d, kv_heads %d, head_dim %d, block_size %d must all be > 0", fn, g.q_heads, g.kv_heads, g.head_dim, g.block_size);
+  if (g.elem_bytes != 2 && g.elem_bytes != 4) return fail(PKV_E_ARG, "%s: elements of %d bytes; 2 (f16, bf16) or 4 (f32)", fn, g.elem_bytes);
+  if (g.q_heads % g.kv_heads) return fail(PKV_E_UNSUPPORTED, "%s: q_heads %d is not a multiple of kv_heads %d", fn, g.q_heads, g.kv_heads);
+  if (g.head_dim > 256) return fail(PKV_E_UNSUPPORTED, "%s: head_dim %d exceeds 256", fn, g.head_dim);
+  if (static_cast<long long>(g.n_tokens) * g.q_heads > 0x7fffffffll) return fail(PKV_E_UNSUPPORTED, "%s: %d tokens of %d heads; at most 2^31 - 1 rows", fn, g.n_tokens, g.q_heads);
+  return PKV_OK;
+}
+
+enum Kind { kCross = 1, kPrefix = 2 };
+
+int write_image(const char* fn, Kind kind, const SegmentGeometry& g, const SegmentLists& l, const std::vector<int>& seq, const std::vector<int>& pos,
+                bool cluster, void* h_staging, size_t staging_bytes, size_t workspace_bytes, pkv_segment_plan* plan) {
+  const SegmentOffsets o = segment_offsets(g, l.rows.size(), l.items.size(), l.first.size(), l.tiles.size(), l.merge.size(), static_cast<size_t>(l.n_parts));
+  if (o.total > workspace_bytes) return fail(PKV_E_WORKSPACE, "%s: workspace of %zu bytes; this step takes %zu", fn, workspace_bytes, o.total);
+  if (o.image > staging_bytes) return fail(PKV_E_WORKSPACE, "%s: staging buffer of %zu bytes; this step's plan takes %zu", fn, staging_bytes, o.image);
+  if (static_cast<long long>(l.tiles.size()) * g.kv_heads > 0x7fffffffll || static_cast<long long>(l.items.size()) * g.kv_heads > 0x7fffffffll)
+    return fail(PKV_E_UNSUPPORTED, "%s: more than 2^31 - 1 work items", fn);
+  char* img = static_cast<char*>(h_staging);
+  std::memset(img, 0, o.seq);
+  PlanHeader* hd = reinterpret_cast<PlanHeader*>(img);
+  hd->magic = kPlanMagic;
+  hd->n_items = static_cast<int>(l.items.size());
+  hd->chunk = l.chunk;
+  hd->n_tokens = g.n_tokens;
+  hd->n_parts = l.n_parts;
+  hd->kv_heads = g.kv_heads;
+  hd->n_shares = l.first.empty() ? 0 : static_cast<int>(l.first.size()) - 1;
+  auto put = [&](size_t at, const void* p, size_t bytes) { if (bytes) std::memcpy(img + at, p, bytes); };
+  put(o.seq, seq.data(), seq.size() * sizeof(int));
+  put(o.pos, pos.data(), pos.size() * sizeof(int));
+  put(o.rows, l.rows.data(), l.rows.size() * sizeof(RowToken));
+  put(o.items, l.items.data(), l.items.size() * sizeof(WorkItem));
+  put(o.items + l.items.size() * sizeof(WorkItem), l.first.data(), l.first.size() * sizeof(int));
+  put(o.tiles, l.tiles.data(), l.tiles.size() * sizeof(TileItem));
+  put(o.merge, l.merge.data(), l.merge.size() * sizeof(MergeRow));
+  std::memset(plan, 0, sizeof(*plan));
+  plan->kind = kind;
+  plan->n_tokens = g.n_tokens; plan->q_heads = g.q_heads; plan->kv_heads = g.kv_heads; plan->head_dim = g.head_dim;
+  plan->block_size = g.block_size; plan->elem_bytes = g.elem_bytes;
+  plan->n_tiles = static_cast<int>(l.tiles.size());
+  plan->n_items = static_cast<int>(l.items.size());
+  plan->n_merged = static_cast<int>(l.merge.size());
+  plan->n_parts = l.n_parts;
+  plan->image_bytes = o.image;
+  plan->workspace_bytes = o.total;
+  plan->off_seq = o.seq; plan->off_pos = o.pos; plan->off_rows = o.rows; plan->off_items = o.items;
+  plan->off_tiles = o.tiles; plan->off_merge = o.merge; plan->off_ml = o.ml; plan->off_acc = o.acc;
+  if (cluster && l.n_parts > 0) plan->cluster = decode_cluster_size(g.n_tokens, l.longest, g.q_heads, g.kv_heads, g.head_dim, &plan->cluster_least);
+  return PKV_OK;
+}
+
+int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* kv_len, int n_seqs, const SegmentGeometry& g, void* h_staging,
+               size_t staging_bytes, size_t workspace_bytes, pkv_segment_plan* plan) {
+  if (!plan) return fail(PKV_E_ARG, "%s: null plan", fn);
+  std::memset(plan, 0, sizeof(*plan));
+  if (g.n_tokens <= 0 || n_seqs <= 0) return PKV_OK;
+  if (!q_len || !kv_len || !h_staging) return fail(PKV_E_ARG, "%s: null pointer", fn);
+  int st = check_geometry(fn, g);
+  if (st != PKV_OK) return st;
+  std::vector<int> seq(g.n_tokens, -1), pos(g.n_tokens, -1), empty;
+  std::vector<Segment> segs;
+  std::vector<OwnRange> own;
+  SegmentLists l;
+  long long next = 0;
+  int listed = 0;
+  for (int s = 0; s < n_seqs; ++s) {
+    const long long start = q_start ? q_start[s] : next;
+    if (q_len[s] < 0 || kv_len[s] < 0 || start < 0 || start + q_len[s] > g.n_tokens)
+      return fail(PKV_E_ARG, "%s: sequence %d has rows %lld .. + %d of %d and %d keys", fn, s, start, q_len[s], g.n_tokens, kv_len[s]);
+    next = start + q_len[s];
+    listed += q_len[s];
+    const bool tiled = kv_len[s] > 0 && g.tiles() && q_len[s] >= kMinTileTokens;
+    if (tiled) segs.push_back(Segment{static_cast<int>(l.rows.size()), q_len[s], kv_len[s], 1, 0});
+    for (int i = 0; i < q_len[s]; ++i) {
+      const int t = static_cast<int>(start) + i;
+      if (seq[t] >= 0) return fail(PKV_E_ARG, "%s: row %d belongs to sequences %d and %d", fn, t, seq[t], s);
+      seq[t] = s;
+      pos[t] = kv_len[s] - 1;
+      if (kv_len[s] == 0) empty.push_back(t);
+      else if (tiled) l.rows.push_back(RowToken{t, 0});
+      else own.push_back(OwnRange{t, 0, kv_len[s]});
+    }
+  }
+  list_segments(segs, own, empty, g, decode_sms(), false, l);
+  return write_image(fn, kCross, g, l, seq, pos, segs.empty() && empty.empty() && listed == g.n_tokens, h_staging, staging_bytes, workspace_bytes, plan);
+}
+
+int plan_prefix(const char* fn, const int* token_pos, int prefix_len, const SegmentGeometry& g, void* h_staging, size_t staging_bytes,
+                size_t workspace_bytes, pkv_segment_plan* plan) {
+  if (!plan) return fail(PKV_E_ARG, "%s: null plan", fn);
+  std::memset(plan, 0, sizeof(*plan));
+  if (g.n_tokens <= 0) return PKV_OK;
+  if (!token_pos || !h_staging) return fail(PKV_E_ARG, "%s: null pointer", fn);
+  if (prefix_len < 0) return fail(PKV_E_ARG, "%s: prefix_len %d must not be negative", fn, prefix_len);
+  int st = check_geometry(fn, g);
+  if (st != PKV_OK) return st;
+  // the decode kernels fetch boxes of 16 slots: a token's own keys begin on a multiple of 16
+  const int shared = g.tiles() ? prefix_len & ~15 : 0;
+  std::vector<int> none, pos(token_pos, token_pos + g.n_tokens), empty;
+  std::vector<Segment> segs;
+  std::vector<OwnRange> own;
+  SegmentLists l;
+  for (int t = 0; t < g.n_tokens; ++t) {
+    if (token_pos[t] < 0 || token_pos[t] == 0x7fffffff) return fail(PKV_E_ARG, "%s: token %d has position %d", fn, t, token_pos[t]);
+    if (shared > 0 && token_pos[t] >= shared - 1) l.rows.push_back(RowToken{t, 0});
+  }
+  const bool together = static_cast<int>(l.rows.size()) >= kMinPrefixTokens;
+  if (!together) l.rows.clear();
+  for (int t = 0; t < g.n_tokens; ++t) {
+    const int begin = together && token_pos[t] >= shared - 1 ? shared : 0, len = token_pos[t] + 1 - begin;
+    if (len > 0) own.push_back(OwnRange{t, begin, len});
+  }
+  if (together) segs.push_back(Segment{0, static_cast<int>(l.rows.size()), shared, 1, 0});
+  list_segments(segs, own, empty, g, decode_sms(), true, l);
+  return write_image(fn, kPrefix, g, l, none, pos, segs.empty(), h_staging, staging_bytes, workspace_bytes, plan);
+}
+
+int upload(const char* fn, pkv_segment_plan* plan, const void* h_staging, void* workspace, pkv_stream stream) {
+  if (plan->n_tokens <= 0) return PKV_OK;
+  const cudaError_t e = cudaMemcpyAsync(workspace, h_staging, plan->image_bytes, cudaMemcpyHostToDevice, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(PKV_E_CUDA, "%s: plan upload failed: %s", fn, cudaGetErrorString(e));
+  return PKV_OK;
+}
+
+template <typename T>
+int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const void* k_cache, const void* v_cache, const int* block_tables,
+                 const int* table_offset, const int* token_seq, void* out, float scale, void* workspace, size_t workspace_bytes, pkv_stream stream) {
+  const char* fn = kind == kCross ? "pkv_cross_attn" : "pkv_prefix_attn";
+  if (!plan) return fail(PKV_E_ARG, "%s: null plan", fn);
+  if (plan->n_tokens <= 0 || (plan->n_tiles == 0 && plan->n_items == 0 && plan->n_merged == 0)) return PKV_OK;
+  int st = check_error_mirror(fn);
+  if (st != PKV_OK) return st;
+  if (plan->kind != kind) return fail(PKV_E_ARG, "%s: a plan of the other kind", fn);
+  if (plan->elem_bytes != static_cast<int>(sizeof(T))) return fail(PKV_E_ARG, "%s: the plan is for elements of %d bytes", fn, plan->elem_bytes);
+  if (!q || !k_cache || !v_cache || !block_tables || !table_offset || !out || (kind == kPrefix && !token_seq)) return fail(PKV_E_ARG, "%s: null device pointer", fn);
+  if (!(scale > 0.f)) return fail(PKV_E_ARG, "%s: scale must be positive", fn);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255)) return fail(PKV_E_ARG, "%s: workspace null or not 256-byte aligned", fn);
+  if (workspace_bytes < plan->workspace_bytes) return fail(PKV_E_WORKSPACE, "%s: workspace of %zu bytes; the plan takes %zu", fn, workspace_bytes, plan->workspace_bytes);
+  const int D = plan->head_dim, group = plan->q_heads / plan->kv_heads;
+  if (static_cast<size_t>(D) * sizeof(T) % 16 == 0 && (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)))
+    return fail(PKV_E_ARG, "%s: q, out and the K/V pools must be 16-byte aligned", fn);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  const uint64_t pool_rows = plan->num_blocks > 0 ? static_cast<uint64_t>(plan->num_blocks) * plan->block_size : 0;
+  const bool log2_domain = decode_log2_domain<T>(plan->q_heads, plan->kv_heads, D, plan->block_size, scale);
+  const int* seq = kind == kCross ? reinterpret_cast<const int*>(ws + plan->off_seq) : token_seq;
+  float *ml = reinterpret_cast<float*>(ws + plan->off_ml), *acc = reinterpret_cast<float*>(ws + plan->off_acc);
+  unsigned int* host_err = error_mirror(true);
+  if (plan->n_tiles > 0) {
+    if constexpr (sizeof(T) == 2) {
+      if (!tensor_map_encoder()) return fail(PKV_E_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", fn);
+      TileArgs a;
+      a.q = q; a.block_tables = block_tables; a.table_offset = table_offset; a.token_seq = seq;
+      a.rows = reinterpret_cast<const RowToken*>(ws + plan->off_rows);
+      a.tiles = reinterpret_cast<const TileItem*>(ws + plan->off_tiles);
+      a.out = out; a.part_ml = ml; a.part_acc = acc;
+      a.n_work = plan->n_tiles * plan->kv_heads;
+      a.q_heads = plan->q_heads; a.kv_heads = plan->kv_heads; a.group = group;
+      a.block_size = plan->block_size; a.bs_log2 = log2_floor(plan->block_size); a.box_log2 = std::min(a.bs_log2, 7);
+      a.scale = scale;
+      a.ml_scale = log2_domain ? scale * 1.4426950408889634f : scale;
+      a.host_err = host_err;
+      const uint64_t rows = pool_rows ? pool_rows : 1ull << 30;
+      st = D == 64 ? launch_tiles<T, 64>(a, k_cache, v_cache, rows, s) : launch_tiles<T, 128>(a, k_cache, v_cache, rows, s);
+      if (st != PKV_OK) return st;
+    }
+  }
+  if (plan->n_items > 0) {
+    DecodeList l;
+    l.q = q; l.k_cache = k_cache; l.v_cache = v_cache; l.block_tables = block_tables; l.table_offset = table_offset; l.token_seq = seq;
+    l.token_pos = reinterpret_cast<const int*>(ws + plan->off_pos);
+    l.out = out;
+    l.n_tokens = plan->n_tokens; l.q_heads = plan->q_heads; l.kv_heads = plan->kv_heads; l.head_dim = D; l.block_size = plan->block_size;
+    l.scale = scale;
+    l.header = reinterpret_cast<const PlanHeader*>(ws);
+    l.items = reinterpret_cast<const WorkItem*>(ws + plan->off_items);
+    l.n_items = plan->n_items;
+    l.part_ml = ml; l.part_acc = acc;
+    l.pool_rows = pool_rows;
+    l.host_err = host_err;
+    l.behind_tiles = plan->n_tiles > 0;
+    l.cluster = plan->cluster; l.cluster_least = plan->cluster_least;
+    bool merged = false;
+    st = decode_listed<T>(l, s, &merged);
+    if (st != PKV_OK || merged) return st;
+  }
+  if (plan->n_merged > 0) {
+    MergeArgs m{reinterpret_cast<const MergeRow*>(ws + plan->off_merge), plan->n_merged, plan->q_heads, D, ml, acc, out};
+    const int vec = D % 4 == 0 ? 4 : 1;
+    const long long blocks = (static_cast<long long>(plan->n_merged) * plan->q_heads * (D / vec) + kMergeThreads - 1) / kMergeThreads;
+    if (blocks > 0x7fffffffll) return fail(PKV_E_UNSUPPORTED, "%s: %lld blocks to merge", fn, blocks);
+    auto kern = vec == 4 ? (log2_domain ? segment_merge_kernel<T, true, 4> : segment_merge_kernel<T, false, 4>)
+                         : (log2_domain ? segment_merge_kernel<T, true, 1> : segment_merge_kernel<T, false, 1>);
+    launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(kMergeThreads), 0, s, m);
+    return check_launch("segment_merge_kernel");
+  }
+  return PKV_OK;
+}
+
+// No exception leaves the C entry points.
+template <typename F> int guarded(const char* fn, F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return fail(PKV_E_NOMEM, "%s: out of host memory", fn);
+  } catch (...) {
+    return fail(PKV_E_STATE, "%s: internal error", fn);
+  }
+}
+
+}  // namespace
+
+int tile_read_flags(unsigned int* flags) {
+  unsigned int v = 0, zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_pkv_tile_error, sizeof(v));
+  if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_pkv_tile_error, &zero, sizeof(zero));
+  if (e != cudaSuccess) return fail(PKV_E_CUDA, "pkv_debug_device_flags: %s", cudaGetErrorString(e));
+  *flags = v;
+  return PKV_OK;
+}
+
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" {
+
+static size_t segment_workspace(int n_tokens, int q_heads, int kv_heads, int head_dim, bool prefix) {
+  if (n_tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads) return 0;
+  return segment_bounds(SegmentGeometry{n_tokens, q_heads, kv_heads, head_dim, 16, 2}, prefix).total;
+}
+size_t pkv_cross_workspace_bytes(int n_tokens, int q_heads, int kv_heads, int head_dim) { return segment_workspace(n_tokens, q_heads, kv_heads, head_dim, false); }
+size_t pkv_prefix_workspace_bytes(int n_tokens, int q_heads, int kv_heads, int head_dim) { return segment_workspace(n_tokens, q_heads, kv_heads, head_dim, true); }
+size_t pkv_segment_staging_bytes(int n_tokens, int q_heads, int kv_heads) {
+  if (n_tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads) return 0;
+  return segment_bounds(SegmentGeometry{n_tokens, q_heads, kv_heads, 64, 16, 2}, true).image;
+}
+
+int pkv_cross_plan_host_image(const int* h_q_start, const int* h_q_len, const int* h_kv_len, int n_seqs, int n_tokens, int q_heads, int kv_heads,
+                              int head_dim, int block_size, int elem_bytes, void* h_staging, size_t staging_bytes, size_t workspace_bytes,
+                              pkv_segment_plan* plan) {
+  const char* fn = "pkv_cross_plan_host_image";
+  return guarded(fn, [&] {
+    return plan_cross(fn, h_q_start, h_q_len, h_kv_len, n_seqs, SegmentGeometry{n_tokens, q_heads, kv_heads, head_dim, block_size, elem_bytes}, h_staging,
+                      staging_bytes, workspace_bytes, plan);
+  });
+}
+int pkv_cross_plan_host(const int* h_q_start, const int* h_q_len, const int* h_kv_len, int n_seqs, int n_tokens, int q_heads, int kv_heads,
+                        int head_dim, int block_size, int elem_bytes, void* h_staging, size_t staging_bytes, void* workspace, size_t workspace_bytes,
+                        pkv_stream stream, pkv_segment_plan* plan) {
+  const char* fn = "pkv_cross_plan_host";
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255)) return fail(PKV_E_ARG, "%s: workspace null or not 256-byte aligned", fn);
+  const int st = pkv_cross_plan_host_image(h_q_start, h_q_len, h_kv_len, n_seqs, n_tokens, q_heads, kv_heads, head_dim, block_size, elem_bytes,
+                                           h_staging, staging_bytes, workspace_bytes, plan);
+  return st != PKV_OK ? st : upload(fn, plan, h_staging, workspace, stream);
+}
+int pkv_prefix_plan_host_image(const int* h_token_pos, int n_tokens, int prefix_len, int q_heads, int kv_heads, int head_dim, int block_size,
+                               int elem_bytes, void* h_staging, size_t staging_bytes, size_t workspace_bytes, pkv_segment_plan* plan) {
+  const char* fn = "pkv_prefix_plan_host_image";
+  return guarded(fn, [&] {
+    return plan_prefix(fn, h_token_pos, prefix_len, SegmentGeometry{n_tokens, q_heads, kv_heads, head_dim, block_size, elem_bytes}, h_staging,
+                       staging_bytes, workspace_bytes, plan);
+  });
+}
+int pkv_prefix_plan_host(const int* h_token_pos, int n_tokens, int prefix_len, int q_heads, int kv_heads, int head_dim, int block_size,
+                         int elem_bytes, void* h_staging, size_t staging_bytes, void* workspace, size_t workspace_bytes, pkv_stream stream,
+                         pkv_segment_plan* plan) {
+  const char* fn = "pkv_prefix_plan_host";
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255)) return fail(PKV_E_ARG, "%s: workspace null or not 256-byte aligned", fn);
+  const int st = pkv_prefix_plan_host_image(h_token_pos, n_tokens, prefix_len, q_heads, kv_heads, head_dim, block_size, elem_bytes, h_staging,
+                                            staging_bytes, workspace_bytes, plan);
+  return st != PKV_OK ? st : upload(fn, plan, h_staging, workspace, stream);
+}
+
+#define PKV_SEGMENT_ATTN(SUFFIX, TYPE)                                                                                                            \
+  int pkv_cross_attn_##SUFFIX(const pkv_segment_plan* plan, const void* q, const void* k_cache, const void* v_cache, const int* block_tables,      \
+                              const int* table_offset, void* out, float scale, void* workspace, size_t workspace_bytes, pkv_stream stream) {       \
+    return segment_attn<TYPE>(kCross, plan, q, k_cache, v_cache, block_tables, table_offset, nullptr, out, scale, workspace, workspace_bytes,      \
+                              stream);                                                                                                            \
+  }                                                                                                                                               \
+  int pkv_prefix_attn_##SUFFIX(const pkv_segment_plan* plan, const void* q, const void* k_cache, const void* v_cache, const int* block_tables,     \
+                               const int* table_offset, const int* token_seq, void* out, float scale, void* workspace, size_t workspace_bytes,     \
+                               pkv_stream stream) {                                                                                               \
+    return segment_attn<TYPE>(kPrefix, plan, q, k_cache, v_cache, block_tables, table_offset, token_seq, out, scale, workspace, workspace_bytes,   \
+                              stream);                                                                                                            \
+  }
+PKV_SEGMENT_ATTN(f16, __half)
+PKV_SEGMENT_ATTN(bf16, __nv_bfloat16)
+PKV_SEGMENT_ATTN(f32, float)
+}

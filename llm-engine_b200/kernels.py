@@ -295,6 +295,132 @@ class DecodePlan:
         _lib.check(fn, st)
 
 
+class _SegmentPlan:
+    """Work list of attention in which many rows see the same keys, built once per step on the host and used by
+    every layer's call (include/pkv.h, pkv_segment_plan).  Its calls share one workspace: those that may
+    overlap on the GPU need a plan each."""
+
+    def __init__(self, workspace_bytes, n_tokens: int, q_heads: int, kv_heads: int, head_dim: int, block_size: int, dtype,
+                 num_blocks: int, workspace, device):
+        import torch
+        if str(dtype) not in _SUFFIX:
+            raise TypeError(f"unsupported KV element type {dtype}")
+        self.n_tokens, self.q_heads, self.kv_heads, self.head_dim = n_tokens, q_heads, kv_heads, head_dim
+        self.block_size, self.dtype, self.num_blocks = block_size, dtype, num_blocks
+        L = _lib.lib()
+        if workspace is None:
+            workspace = torch.empty(max(int(getattr(L, workspace_bytes)(n_tokens, q_heads, kv_heads, head_dim)), 256), dtype=torch.uint8, device=device)
+        self.workspace = workspace
+        n = max(int(L.pkv_segment_staging_bytes(n_tokens, q_heads, kv_heads)), 256)
+        self.staging = torch.empty(n, dtype=torch.uint8, pin_memory=torch.cuda.is_available())
+        self.plan = _lib.SegmentPlan()
+        self._out_elems = n_tokens * q_heads * head_dim
+
+    def _geometry(self):
+        return self.q_heads, self.kv_heads, self.head_dim, self.block_size, self.dtype.itemsize
+
+    def _build(self, name, image: bool, *args, stream=None):
+        where = (self.staging.data_ptr(), self.staging.numel())
+        L = _lib.lib()
+        if image:
+            st = getattr(L, name + "_image")(*args, *where, self.workspace.numel(), C.byref(self.plan))
+        else:
+            with _device_of(self.workspace):
+                st = getattr(L, name)(*args, *where, _ptr(self.workspace), self.workspace.numel(), _stream(stream), C.byref(self.plan))
+        _lib.check(name, st)
+        self.plan.num_blocks = self.num_blocks
+
+    def _check(self, q, k_cache, v_cache, out, *ints):
+        for t in (q, k_cache, v_cache, out):
+            if t.dtype != self.dtype:
+                raise TypeError(f"the plan is for {self.dtype}, not {t.dtype}")
+        if q.numel() < self._out_elems or out.numel() < self._out_elems:
+            raise ValueError(f"q and out must have {self.n_tokens} rows of {self.q_heads} heads")
+        _on_device(self.workspace, q, k_cache, v_cache, out, *ints)
+        _ints(*ints)
+
+
+class CrossPlan(_SegmentPlan):
+    """Attention of each sequence's rows to the states of another sequence (an encoder's output), whose K and V lie
+    in blocks of the pools: no causal mask, lengths of their own.  n_tokens: rows of q and out."""
+
+    def __init__(self, n_tokens: int, n_seqs: int, q_heads: int, kv_heads: int, head_dim: int, block_size: int, dtype, num_blocks: int = 0,
+                 workspace=None, device="cuda"):
+        super().__init__("pkv_cross_workspace_bytes", n_tokens, q_heads, kv_heads, head_dim, block_size, dtype, num_blocks, workspace, device)
+        self.n_seqs = n_seqs
+
+    def _lengths(self, q_len, kv_len, q_start):
+        import numpy as np
+        arrays = [None if a is None else np.ascontiguousarray(a, dtype=np.int32) for a in (q_start, q_len, kv_len)]
+        for a in arrays:
+            if a is not None and a.shape != (self.n_seqs,):
+                raise ValueError(f"the plan is for {self.n_seqs} sequences")
+        return arrays
+
+    def build_host(self, q_len, kv_len, q_start=None, stream=None) -> "CrossPlan":
+        """q_len, kv_len, q_start: per sequence, on the host; without q_start the rows are packed one sequence behind
+        the other.  The staging buffer belongs to the upload until it has run."""
+        arrays = self._lengths(q_len, kv_len, q_start)
+        self._build("pkv_cross_plan_host", False, *[None if a is None else a.ctypes.data for a in arrays], self.n_seqs, self.n_tokens,
+                    *self._geometry(), stream=stream)
+        return self
+
+    def build_host_image(self, q_len, kv_len, q_start=None) -> int:
+        """The plan without the upload: bytes of self.staging that must reach the start of self.workspace."""
+        arrays = self._lengths(q_len, kv_len, q_start)
+        self._build("pkv_cross_plan_host", True, *[None if a is None else a.ctypes.data for a in arrays], self.n_seqs, self.n_tokens,
+                    *self._geometry())
+        return int(self.plan.image_bytes)
+
+    def attention(self, q, k_cache, v_cache, block_tables, table_offset, out, scale: float, stream=None) -> None:
+        """out[t] = softmax(q[t] K^T scale) V over all keys of t's sequence; zero where it has none.  table_offset[s] is the
+        start of sequence s's table."""
+        self._check(q, k_cache, v_cache, out, block_tables, table_offset)
+        fn, call = _fn("pkv_cross_attn_", k_cache)
+        with _device_of(k_cache):
+            st = call(C.byref(self.plan), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), _ptr(table_offset), _ptr(out),
+                      scale, _ptr(self.workspace), self.workspace.numel(), _stream(stream))
+        _lib.check(fn, st)
+
+
+class PrefixPlan(_SegmentPlan):
+    """Decode attention of tokens whose sequences all begin with the same blocks: the prefix is worked through once
+    for all of them."""
+
+    def __init__(self, n_tokens: int, q_heads: int, kv_heads: int, head_dim: int, block_size: int, dtype, num_blocks: int = 0, workspace=None,
+                 device="cuda"):
+        super().__init__("pkv_prefix_workspace_bytes", n_tokens, q_heads, kv_heads, head_dim, block_size, dtype, num_blocks, workspace, device)
+
+    def _positions(self, token_pos):
+        import numpy as np
+        pos = np.ascontiguousarray(token_pos, dtype=np.int32)
+        if pos.shape != (self.n_tokens,):
+            raise ValueError(f"the plan is for {self.n_tokens} tokens")
+        return pos
+
+    def build_host(self, token_pos, prefix_len: int, stream=None) -> "PrefixPlan":
+        """token_pos: every token's position, on the host; its sequence's first prefix_len positions lie in the same
+        blocks as everyone's.  The staging buffer belongs to the upload until it has run."""
+        pos = self._positions(token_pos)
+        self._build("pkv_prefix_plan_host", False, pos.ctypes.data, self.n_tokens, prefix_len, *self._geometry(), stream=stream)
+        return self
+
+    def build_host_image(self, token_pos, prefix_len: int) -> int:
+        """The plan without the upload: bytes of self.staging that must reach the start of self.workspace."""
+        pos = self._positions(token_pos)
+        self._build("pkv_prefix_plan_host", True, pos.ctypes.data, self.n_tokens, prefix_len, *self._geometry())
+        return int(self.plan.image_bytes)
+
+    def attention(self, q, k_cache, v_cache, block_tables, table_offset, token_seq, out, scale: float, stream=None) -> None:
+        """As launch_attention_decode with the step's whole tables."""
+        self._check(q, k_cache, v_cache, out, block_tables, table_offset, token_seq)
+        fn, call = _fn("pkv_prefix_attn_", k_cache)
+        with _device_of(k_cache):
+            st = call(C.byref(self.plan), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), _ptr(table_offset), _ptr(token_seq),
+                      _ptr(out), scale, _ptr(self.workspace), self.workspace.numel(), _stream(stream))
+        _lib.check(fn, st)
+
+
 def launch_attention_prefill(q, k_cache, v_cache, block_tables, table_offset, q_start, q_len, ctx_len, out,
                              n_tokens: int, n_seqs: int, max_q_len: int, q_heads: int, kv_heads: int, head_dim: int,
                              block_size: int, num_blocks: int, scale: float, stream=None) -> None:

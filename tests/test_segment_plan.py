@@ -1,0 +1,163 @@
+"""The host planners of pkv_cross_* and pkv_prefix_*: every (row, key) pair is listed exactly once, partials and the
+merge agree, the bounds for workspace and staging hold, and bad arguments are refused before anything is enqueued."""
+import ctypes as C
+import random
+
+import numpy as np
+import pytest
+
+from tests.segment_util import Image, check_cover
+
+GEOMS = [(14, 2, 64), (32, 4, 64), (32, 8, 128), (16, 16, 64), (20, 1, 128), (7, 7, 96), (48, 1, 64)]
+
+
+class Buffers:
+    def __init__(self, pkv, n, qh, kvh, hd, prefix):
+        L = pkv.lib()
+        self.ws = L.pkv_prefix_workspace_bytes(n, qh, kvh, hd) if prefix else L.pkv_cross_workspace_bytes(n, qh, kvh, hd)
+        self.staging = np.zeros(L.pkv_segment_staging_bytes(n, qh, kvh), np.uint8)
+
+
+def cross(pkv, q_len, kv_len, n, geom, bs=16, elem=2, q_start=None, b=None):
+    qh, kvh, hd = geom
+    b = b or Buffers(pkv, n, qh, kvh, hd, False)
+    plan = pkv._lib.SegmentPlan()
+    arr = [None if a is None else np.ascontiguousarray(a, np.int32) for a in (q_start, q_len, kv_len)]
+    st = pkv.lib().pkv_cross_plan_host_image(*[None if a is None else a.ctypes.data for a in arr], len(q_len), n, qh, kvh, hd, bs, elem,
+                                             b.staging.ctypes.data, b.staging.size, b.ws, C.byref(plan))
+    return st, plan, b
+
+
+def prefix(pkv, pos, prefix_len, geom, bs=16, elem=2, b=None):
+    qh, kvh, hd = geom
+    n = len(pos)
+    b = b or Buffers(pkv, n, qh, kvh, hd, True)
+    plan = pkv._lib.SegmentPlan()
+    p = np.ascontiguousarray(pos, np.int32)
+    st = pkv.lib().pkv_prefix_plan_host_image(p.ctypes.data, n, prefix_len, qh, kvh, hd, bs, elem, b.staging.ctypes.data, b.staging.size, b.ws,
+                                              C.byref(plan))
+    return st, plan, b
+
+
+def log_int(r, lo, hi):
+    return int(round(lo * (hi / lo) ** r.random()))
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_cross_covers_every_pair(pkv, seed):
+    r = random.Random(seed)
+    geom = r.choice(GEOMS)
+    n_seqs = log_int(r, 1, 60)
+    top_q, top_k = log_int(r, 1, 600), log_int(r, 1, 9000)
+    q_len = [r.choice([0, 1, r.randrange(1, top_q + 1), top_q]) for _ in range(n_seqs)]
+    kv_len = [r.choice([0, 1, 127, 128, 129, r.randrange(1, top_k + 1), top_k]) for _ in range(n_seqs)]
+    order = r.sample(range(n_seqs), n_seqs)
+    start, at = [0] * n_seqs, r.randrange(3)
+    for s in order:
+        start[s] = at
+        at += q_len[s] + r.randrange(2)
+    n = max(at, 1)
+    st, plan, b = cross(pkv, q_len, kv_len, n, geom, bs=r.choice([16, 64, 8, 48]), elem=r.choice([2, 2, 2, 4]), q_start=start)
+    assert st == 0, pkv._lib.last_error()
+    assert plan.workspace_bytes <= b.ws and plan.image_bytes <= b.staging.size
+    image = Image(b.staging, plan)
+    want = {start[s] + i: kv_len[s] for s in range(n_seqs) for i in range(q_len[s])}
+    check_cover(image, plan, want)
+    for s in range(n_seqs):
+        for i in range(q_len[s]):
+            assert image.seq[start[s] + i] == s and image.pos[start[s] + i] == kv_len[s] - 1
+    assert (np.delete(image.seq, list(want)) == -1).all()
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_prefix_covers_every_pair(pkv, seed):
+    r = random.Random(1000 + seed)
+    geom = r.choice(GEOMS)
+    n = log_int(r, 1, 700)
+    shared = r.choice([0, 1, 15, 16, 17, log_int(r, 16, 20000), 16 * log_int(r, 1, 1000)])
+    tail = log_int(r, 1, 2000)
+    pos = [shared + r.choice([0, 1, 15, 16, r.randrange(tail + 1)]) for _ in range(n)]
+    for i in range(n):
+        if r.random() < 0.05:
+            pos[i] = r.randrange(shared + 1)
+    st, plan, b = prefix(pkv, pos, shared, geom, bs=r.choice([16, 64, 8]), elem=r.choice([2, 2, 2, 4]))
+    assert st == 0, pkv._lib.last_error()
+    assert plan.workspace_bytes <= b.ws and plan.image_bytes <= b.staging.size
+    image = Image(b.staging, plan)
+    check_cover(image, plan, {t: p + 1 for t, p in enumerate(pos)})
+    assert all(begin % 16 == 0 for _, begin, _, _ in image.items.tolist())
+
+
+def test_packed_rows_without_starts_and_empty_steps(pkv):
+    st, plan, b = cross(pkv, [3, 0, 5], [10, 10, 300], 9, GEOMS[0])
+    assert st == 0
+    image = Image(b.staging, plan)
+    assert image.seq.tolist() == [0, 0, 0, 2, 2, 2, 2, 2, -1]
+    for q_len, kv_len, n in (([0, 0], [5, 6], 4), ([], [], 4), ([1], [5], 0)):
+        b = Buffers(pkv, max(n, 1), 14, 2, 64, False)
+        st, plan, _ = cross(pkv, q_len, kv_len, n, GEOMS[0], b=b)
+        assert st == 0 and plan.n_tiles == plan.n_items == plan.n_merged == 0
+        assert pkv.lib().pkv_cross_attn_bf16(C.byref(plan), *[None] * 6, 1.0, None, 0, None) == 0
+
+
+def test_refusals(pkv):
+    L, E = pkv.lib(), pkv._lib
+    g = GEOMS[0]
+    assert cross(pkv, [3, -1], [5, 5], 9, g)[0] == E.PKV_E_ARG
+    assert cross(pkv, [3, 1], [5, -5], 9, g)[0] == E.PKV_E_ARG
+    assert cross(pkv, [3, 7], [5, 5], 9, g)[0] == E.PKV_E_ARG                             # behind the last row
+    assert cross(pkv, [3, 3], [5, 5], 9, g, q_start=[0, 2])[0] == E.PKV_E_ARG             # a row of two sequences
+    assert cross(pkv, [3, 3], [5, 5], 9, g, q_start=[-1, 4])[0] == E.PKV_E_ARG
+    assert cross(pkv, [2], [5], 9, g, elem=1)[0] == E.PKV_E_ARG
+    assert cross(pkv, [2], [5], 9, (14, 4, 64), b=Buffers(pkv, 9, 14, 2, 64, False))[0] == E.PKV_E_UNSUPPORTED
+    assert cross(pkv, [2], [5], 9, (2, 1, 512))[0] == E.PKV_E_UNSUPPORTED
+    assert prefix(pkv, [5, -1], 0, g)[0] == E.PKV_E_ARG
+    assert prefix(pkv, [5, 2 ** 31 - 1], 0, g)[0] == E.PKV_E_ARG
+    assert prefix(pkv, [5], -16, g)[0] == E.PKV_E_ARG
+    small = Buffers(pkv, 64, 14, 2, 64, True)
+    small.ws = 4096
+    assert prefix(pkv, [5000] * 64, 4096, g, b=small)[0] == E.PKV_E_WORKSPACE
+    small = Buffers(pkv, 64, 14, 2, 64, True)
+    small.staging = np.zeros(512, np.uint8)
+    assert prefix(pkv, [5000] * 64, 4096, g, b=small)[0] == E.PKV_E_WORKSPACE
+    assert L.pkv_prefix_plan_host(None, 3, 0, 14, 2, 64, 16, 2, None, 0, None, 0, None, C.byref(E.SegmentPlan())) == E.PKV_E_ARG
+    assert L.pkv_cross_plan_host(None, None, None, 3, 3, 14, 2, 64, 16, 2, None, 0, None, 0, None, None) == E.PKV_E_ARG
+    # the attention calls look at everything before they enqueue
+    st, plan, b = prefix(pkv, [500] * 9, 256, g)
+    one, ws = 256, (1 << 20, b.ws)           # never dereferenced: every call below is refused on the host
+    ok = [one] * 6 + [one]
+    call = lambda kind, suffix, args, scale=1.0, w=ws, p=plan: getattr(L, f"pkv_{kind}_attn_{suffix}")(None if p is None else C.byref(p), *args, scale, *w, None)
+    assert call("prefix", "bf16", ok, p=None) == E.PKV_E_ARG
+    assert call("cross", "bf16", ok[:6]) == E.PKV_E_ARG                                    # a plan of the other kind
+    assert call("prefix", "f32", ok) == E.PKV_E_ARG                                        # made for 16 bits
+    for i in range(7):
+        assert call("prefix", "f16", ok[:i] + [None] + ok[i + 1:]) == E.PKV_E_ARG
+    assert call("prefix", "f16", ok, scale=0.0) == E.PKV_E_ARG
+    assert call("prefix", "f16", ok, scale=float("nan")) == E.PKV_E_ARG
+    assert call("prefix", "f16", ok, w=(None, b.ws)) == E.PKV_E_ARG
+    assert call("prefix", "f16", ok, w=(264, b.ws)) == E.PKV_E_ARG
+    assert call("prefix", "f16", ok, w=(256, 64)) == E.PKV_E_WORKSPACE
+    for i in (0, 1, 2, 6):
+        arg = list(ok)
+        arg[i if i < 6 else 6] = 264
+        assert call("prefix", "f16", arg) == E.PKV_E_ARG                                   # off a 16-byte boundary
+
+
+def test_norm_refusals(pkv):
+    L, E = pkv.lib(), pkv._lib
+    one = 256
+    base = dict(q=one, k=one, v=one, qs=896, ks=128, vs=128, qw=one, kw=one, eps=1e-6, pos=one, cos=one, sin=one, maxp=10, slots=one, qo=512,
+                kc=one, vc=one, n_slots=64, n=3, qh=14, kvh=2, hd=64)
+
+    def call(**kw):
+        a = {**base, **kw}
+        return L.pkv_qk_norm_rope_append_bf16(*[a[k] for k in base], None)
+
+    for p in ("q", "k", "v", "qw", "kw", "pos", "cos", "sin", "slots", "qo", "kc", "vc"):
+        assert call(**{p: None}) == E.PKV_E_ARG, p
+    assert call(hd=65) == E.PKV_E_UNSUPPORTED
+    assert call(eps=-1.0) == E.PKV_E_ARG and call(eps=float("nan")) == E.PKV_E_ARG
+    assert call(qs=895) == E.PKV_E_ARG and call(ks=127) == E.PKV_E_ARG and call(vs=-128) == E.PKV_E_ARG
+    assert call(maxp=0) == E.PKV_E_ARG and call(n_slots=0) == E.PKV_E_ARG and call(qh=-1) == E.PKV_E_ARG
+    assert call(qo=one, qs=1024) == E.PKV_E_ARG                    # in place needs contiguous rows
+    assert call(n=0, q=None) == 0 and call(qh=0, kvh=0, q=None) == 0

@@ -8,15 +8,19 @@
 // 128.  The rows are two groups of 128, each with its own scores S (128 columns of tensor memory) and output O (head_dim
 // columns); a K or V tile is fetched once for both.  While one group's scores are turned into probabilities by its
 // four warps, the tensor cores work on the other group: a 128 x 128 x 128 product takes 512 cycles, the 16,384
-// exponentials of a group's tile 1,024, so at head_dim 128 (two products) both pipes can be busy all the time, and at
-// head_dim 64 the exponentials decide.
+// exponentials of a group's tile 1,024.
 //
 //   warps 0-3, 4-7  softmax of group 0, 1: thread = row.  128 scores to registers, maximum, exponentials, sum; P goes
-//                   back as 16-bit pairs over the first 64 columns of S, where the second product reads its A operand.
-//                   O stays in tensor memory and is rescaled only when a row's maximum has grown by more than 2^8.
+//                   back to tensor memory as 16-bit pairs, the A operand of the second product.  O stays there and is
+//                   rescaled only when a row's maximum has grown by more than 2^8.
 //   warp 8          TMA: K and V tiles through the block table into a ring (boxes of up to 128 slots x 128 bytes).
-//   warp 9          issues the products, one thread: S = Q K^T for either group, then O += P V and the next S in turns.
-//   warp 10         gathers the next item's rows of Q, whatever tokens and heads they are.
+//   warp 9          issues the products, one thread: S = Q K^T and O += P V of both groups in turns.
+//   warps 10, 11    gather group 0's, 1's rows of Q for the next item, whatever tokens and heads they are.
+//
+// head_dim 64: P has 64 columns of its own.  The next scores of a group are issued as soon as its threads hold the present ones
+// in registers, so the softmax warps never wait for a product: the exponentials decide.
+// head_dim 128: S and O fill the group's half of tensor memory, P lies over the first half of S.  The next scores follow
+// the second product, whose first half starts when P's first 64 keys are there.
 //
 // An item of at most 128 rows whose keys are many runs both groups over the same rows, every other key tile each (`halves`).
 // P is rounded to 16 bits for the second product (the sums are of the unrounded ones), as the operands of the
@@ -47,12 +51,12 @@ int check_error_mirror(const char* fn, unsigned int bits = ~0u);
 
 namespace {
 
-constexpr int kTileThreads = 384;                        // 12 warps, the last one idle: registers are split by fours
+constexpr int kTileThreads = 384;
 // Registers a thread of the softmax warps and of the others; launched with 168 each (2 x 208 + 80 <= 3 x 168).
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
-constexpr int kProducer = 8, kIssuer = 9, kGatherer = 10;
+constexpr int kProducer = 8, kIssuer = 9, kGatherer = 10;   // and 11
 constexpr int kBlockBytes = 128 * 128;                   // 128 rows x 64 16-bit elements: one operand block
-constexpr uint32_t kGroupCols = 256, kColO = 128;        // tensor memory of a group: S, then O
+constexpr uint32_t kGroupCols = 256, kColO = 128;        // tensor memory of a group: S, then O ...
 constexpr float kRescale = 8.f;                          // in log2 units: P stays below 2^8
 constexpr int kMinTileTokens = 4;                        // sequences with fewer tokens go to the decode kernels
 constexpr int kMinPrefixTokens = 2;                      // batches of fewer tokens behind the prefix, too
@@ -61,6 +65,8 @@ template <int D> struct TileSmem {
   static constexpr int kHalves = D / 64;
   static constexpr int kTile = kHalves * kBlockBytes;    // a K or V tile, or one group's Q
   static constexpr int kStages = D == 64 ? 8 : 5;
+  static constexpr uint32_t kColP = D == 64 ? 192 : 0;   // ... and P behind O, or over S
+  static constexpr int kLead = D == 64 ? 2 : 1;          // key tiles a group's scores are issued ahead of its values
   static constexpr int kRing = 2 * kTile;
   static constexpr int kBytes = kRing + kStages * kTile + 1024;
 };
@@ -103,6 +109,26 @@ __device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
       : "f"(b0), "f"(b1));
 }
 
+// Eight 16-byte pieces a lane: piece i of lane j of every eight lanes becomes piece j of lane i.
+__device__ __forceinline__ void transpose8(uint32_t (&x)[32], int lane) {
+#pragma unroll
+  for (int s = 1; s < 8; s <<= 1) {
+    const bool upper = (lane & s) != 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i & s) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t& a = x[4 * i + k];
+        uint32_t& b = x[4 * (i | s) + k];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? a : b, s);
+        a = upper ? got : a;
+        b = upper ? b : got;
+      }
+    }
+  }
+}
+
 // The r-th item of a block, or -1.
 __device__ __forceinline__ int work_at(int r, int n_work) {
   const int G = static_cast<int>(gridDim.x), b = static_cast<int>(blockIdx.x);
@@ -124,26 +150,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   constexpr int NS = S::kStages;
 
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[2 + 2 * NS + 6];
+  __shared__ __align__(8) unsigned long long bars[2 * NS + 14];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t ring = base + S::kRing, bar0 = smem_u32(&bars[0]);
-  enum { Q_FULL = 0, Q_EMPTY = 1, KV_FULL = 2, KV_EMPTY = KV_FULL + NS, S_FULL = KV_EMPTY + NS, P_FULL = S_FULL + 2, O_FULL = P_FULL + 2 };
+  enum { KV_FULL = 0, KV_EMPTY = NS, Q_FULL = 2 * NS, Q_EMPTY = Q_FULL + 2, S_FULL = Q_EMPTY + 2, S_READ = S_FULL + 2, P_HALF = S_READ + 2, P_FULL = P_HALF + 2, O_FULL = P_FULL + 2 };
   auto BAR = [&](int i) { return bar0 + 8u * i; };
 
   if (threadIdx.x == 0) {
-    mbar_init(BAR(Q_FULL), 1);          // the gatherer, its copies done
-    mbar_init(BAR(Q_EMPTY), 1);         // commit after the item's last Q K^T
     for (int i = 0; i < NS; ++i) {
       mbar_init(BAR(KV_FULL + i), 1);
       mbar_init(BAR(KV_EMPTY + i), 1);  // commit after the last product that reads the stage
     }
     for (int g = 0; g < 2; ++g) {
+      mbar_init(BAR(Q_FULL + g), 1);    // the group's gatherer, its copies done
+      mbar_init(BAR(Q_EMPTY + g), 1);   // commit after the item's last Q K^T
       mbar_init(BAR(S_FULL + g), 1);    // commit after the group's Q K^T
-      mbar_init(BAR(P_FULL + g), 128);  // the group's softmax threads (32 at a time)
-      mbar_init(BAR(O_FULL + g), 1);    // commit after the group's last P V of an item
+      mbar_init(BAR(S_READ + g), 128);  // kLead 2: the group's softmax threads (32 at a time) hold S in registers
+      mbar_init(BAR(P_HALF + g), 128);  // kLead 1: they have written P for the first 64 keys ...
+      mbar_init(BAR(P_FULL + g), 128);  // ... for all
+      mbar_init(BAR(O_FULL + g), 1);    // commit after the group's P V: kLead 2 each, kLead 1 the item's last
     }
     mbar_fence_init();
   }
@@ -174,9 +202,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (warp >= kProducer) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
     if (warp == kProducer) {
-      // The entries of the ring for an item of n key tiles, in the order the products use them:
-      //   both groups on every tile   K0 V0 K1 V1 ...
-      //   every other tile each       K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1)
+      // The entries of the ring for an item of n key tiles, in the order the products use them: K of the first `lead` tiles,
+      // then V0 K(lead) V1 K(lead + 1) ..., and the last V.
       uint32_t e = 0;
       const int box_rows = 1 << a.box_log2, boxes = kTileKeys >> a.box_log2;
       for (int r = 0; !dead; ++r) {
@@ -185,8 +212,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const TileItem it = load_tile(a.tiles + w / a.kv_heads);
         const int kvh = w % a.kv_heads, n = (it.kv_len + kTileKeys - 1) / kTileKeys, end = it.kv_begin + it.kv_len;
         const int* tbl = a.block_tables + __ldg(a.table_offset + __ldg(a.token_seq + __ldg(&a.rows[it.tok0].token)));
-        auto tile_of = [&](int i) { return !it.halves ? i >> 1 : i < 2 ? i : i == 2 * n - 1 ? n - 1 : (i & 1) ? (i + 1) >> 1 : (i - 2) >> 1; };
-        auto is_v = [&](int i) { return !it.halves ? (i & 1) != 0 : i >= 2 && (i == 2 * n - 1 || (i & 1) == 0); };
+        const int lead = min(n, S::kLead << it.halves), turns = 2 * (n - lead);
+        auto is_v = [&](int i) { return i >= lead && !(i - lead < turns && ((i - lead) & 1)); };
+        auto tile_of = [&](int i) { return i < lead ? i : i - lead >= turns ? i - n : ((i - lead) & 1) ? lead + ((i - lead) >> 1) : (i - lead) >> 1; };
         auto row_of = [&](int i) {           // pool row of this lane's box
           const int pos = it.kv_begin + tile_of(i) * kTileKeys + (lane << a.box_log2);
           if (lane >= boxes || pos >= end) return 0;
@@ -218,117 +246,134 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (uint32_t i = e > NS ? e - NS : 0; i < e; ++i) mbar_wait(BAR(KV_FULL + i % NS), (i / NS) & 1);
       }
       __syncwarp();
-    } else if (warp == kGatherer) {
+    } else if (warp != kIssuer) {
       constexpr int kRowBytes = D * 2;
-      const int half = lane & 7;                                   // 16-byte piece of a 128-byte operand row
+      const int g = warp - kGatherer, piece = lane & 7;              // 16-byte piece of a 128-byte operand row
+      const unsigned char* q = static_cast<const unsigned char*>(a.q);
+      uint32_t items = 0;
       for (int r = 0; !dead; ++r) {
         const int w = work_at(r, a.n_work);
         if (w < 0) break;
         const TileItem it = load_tile(a.tiles + w / a.kv_heads);
-        const int kvh = w % a.kv_heads;
-        if (lane == 0) WAIT(BAR(Q_EMPTY), (r & 1) ^ 1);
+        const int kvh = w % a.kv_heads, rows = it.rows - g * 128;
+        if (rows <= 0) continue;
+        int place[4];                                                // (token, head) row of rows lane, 32 + lane, ... in q, or -1
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          place[u] = -1;
+          if (32 * u + lane < rows) {
+            const int f = it.f0 + g * 128 + 32 * u + lane, t = f / a.group;
+            place[u] = __ldg(&a.rows[it.tok0 + t].token) * a.q_heads + kvh * a.group + (f - t * a.group);
+            // into L2 while the item before is still being worked on: copies that miss it go out few at a time
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + static_cast<size_t>(place[u]) * kRowBytes + h * 128));
+          }
+        }
+        if (lane == 0) WAIT(BAR(Q_EMPTY + g), (items & 1) ^ 1);
         dead = __shfl_sync(0xffffffffu, dead ? 1 : 0, 0) != 0;
         if (dead) break;
-        const unsigned char* q = static_cast<const unsigned char*>(a.q);
-        for (int row0 = 0; row0 < (it.rows > 128 ? 256 : 128); row0 += 32) {
-          unsigned long long src = 0;
-          if (row0 + lane < it.rows) {
-            const int f = it.f0 + row0 + lane, t = f / a.group;
-            const int token = __ldg(&a.rows[it.tok0 + t].token);
-            src = reinterpret_cast<unsigned long long>(q + (static_cast<size_t>(token) * a.q_heads + kvh * a.group + (f - t * a.group)) * kRowBytes);
-          }
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+          const int here = u == 0 ? place[0] : u == 1 ? place[1] : u == 2 ? place[2] : place[3];
+          uint32_t dst = base + g * S::kTile + (32 * u + (lane >> 3)) * 128 + ((piece ^ (lane >> 3)) << 4);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int row = row0 + 4 * i + (lane >> 3);
-            const unsigned long long from = __shfl_sync(0xffffffffu, src, 4 * i + (lane >> 3));
-            const uint32_t dst = base + (row >> 7) * S::kTile + (row & 127) * 128 + ((half ^ (row & 7)) << 4);
+            const int from = __shfl_sync(0xffffffffu, here, 4 * i + (lane >> 3));
+            const unsigned char* src = q + static_cast<size_t>(max(from, 0)) * kRowBytes + piece * 16;
+            const uint32_t to = (dst ^ ((i & 1) << 6)) + i * 512;    // row & 7 is lane / 8 + 4 (i & 1)
 #pragma unroll
-            for (int h = 0; h < S::kHalves; ++h)
-              cp_async16(dst + h * kBlockBytes, from ? reinterpret_cast<const unsigned char*>(from) + h * 128 + half * 16 : q, from ? 16 : 0);
+            for (int h = 0; h < S::kHalves; ++h) cp_async16(to + h * kBlockBytes, src + h * 128, from >= 0 ? 16 : 0);
           }
         }
         cp_async_commit();
         cp_async_wait_all();
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(BAR(Q_FULL));
+        if (lane == 0) mbar_arrive(BAR(Q_FULL + g));
+        ++items;
       }
-    } else if (warp == kIssuer) {
+    } else {
       if (lane == 0) {
-        uint32_t e = 0, done[2] = {0, 0};                          // ring entries; key tiles of either group, over all items
+        uint32_t e = 0, done = 0, read = 0, items = 0;             // ring entries; bit g: parity of group g's P and S taken, of its Q tiles
         for (int r = 0; !dead; ++r) {
           const int w = work_at(r, a.n_work);
           if (w < 0) break;
           const TileItem it = load_tile(a.tiles + w / a.kv_heads);
-          const int n = (it.kv_len + kTileKeys - 1) / kTileKeys;
-          WAIT(BAR(Q_FULL), r & 1);
+          const int n = (it.kv_len + kTileKeys - 1) / kTileKeys, last = it.rows > 128 ? 1 : 0;   // last group
           // waits for the ring entry and returns where it lies
           auto full = [&](uint32_t entry) {
             WAIT(BAR(KV_FULL + entry % NS), (entry / NS) & 1);
             tc::fence_after();
             return ring + (entry % NS) * S::kTile;
           };
-          auto scores = [&](int g, uint32_t k_addr) {
-            const uint64_t qd = tc::operand(base + (it.halves ? 0 : g) * S::kTile), kd = tc::operand(k_addr);
+          // Descriptors differ in their low word only.  It is made opaque at every call: the compiler would otherwise keep two
+          // dozen of them per group at hand, spilled, and a product waited 200 cycles for its own.
+          auto scores = [&](int g, uint32_t k_addr, bool read_first) {
+            if (S::kLead > 1) {
+              if (read_first) {
+                WAIT(BAR(S_READ + g), (read >> g) & 1);
+                tc::fence_after();
+              }
+              // counted by tiles: the phase of an item's last tile, which nobody waits for, is over when its P is there
+              if (read_first) read ^= 1u << g;
+            }
+            uint32_t q_lo = (base + (it.halves ? 0 : g) * S::kTile) >> 4, k_lo = k_addr >> 4;
+            const uint32_t d = tmem + g * kGroupCols;
+            asm volatile("" : "+r"(q_lo), "+r"(k_lo));
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
-              const uint64_t step = static_cast<uint64_t>((ks >> 2) * (kBlockBytes >> 4) + (ks & 3) * 2);
-              tc::mma_ss(tmem + g * kGroupCols, qd + step, kd + step, kInstrQK, ks > 0);
+              const uint32_t step = (ks >> 2) * (kBlockBytes >> 4) + (ks & 3) * 2;
+              tc::mma_ss(d, tc::operand_at(q_lo + step), tc::operand_at(k_lo + step), kInstrQK, ks > 0);
             }
             tc::commit(BAR(S_FULL + g));
           };
-          // The group's S is overwritten by its next scores only behind these products: those of one thread run in order.
-          auto values = [&](int g, uint32_t v_addr, bool first) {
-            WAIT(BAR(P_FULL + g), done[g] & 1);
-            ++done[g];
-            tc::fence_after();
-            const uint64_t vd = tc::operand(v_addr, kBlockBytes);
+          // Products of one thread run in order: where P lies over S, the group's next scores overwrite it behind these.
+          auto values = [&](int g, uint32_t v_addr, bool first, bool final) {
+            uint32_t v_lo = v_addr >> 4, t = tmem + g * kGroupCols;
+            asm volatile("" : "+r"(v_lo), "+r"(t));
 #pragma unroll
-            for (int kk = 0; kk < kTileKeys / 16; ++kk)
-              tc::mma_ts(tmem + g * kGroupCols + kColO, tmem + g * kGroupCols + kk * 8, vd + kk * (2048 >> 4), kInstrPV, !(first && kk == 0));
+            for (int kk = 0; kk < kTileKeys / 16; ++kk) {
+              if (kk == 0 || kk == 4) {
+                if (S::kLead == 1 || kk == 0) WAIT(BAR((S::kLead == 1 && kk == 0 ? P_HALF : P_FULL) + g), (done >> g) & 1);
+                tc::fence_after();
+              }
+              tc::mma_ts(t + kColO, t + S::kColP + kk * 8, tc::operand_at(v_lo + kk * (2048 >> 4), kBlockBytes), kInstrPV, !(first && kk == 0));
+            }
+            done ^= 1u << g;
+            if (final && S::kLead > 1) read ^= 1u << g;              // see scores()
+            if (final || S::kLead > 1) tc::commit(BAR(O_FULL + g));
           };
-          if (!it.halves) {
-            const int last = it.rows > 128 ? 1 : 0;                // last group
-            uint32_t k_addr = full(e);
-            for (int g = 0; g <= last; ++g) scores(g, k_addr);
-            tc::commit(BAR(KV_EMPTY + e % NS));
-            if (n == 1) tc::commit(BAR(Q_EMPTY));
-            ++e;
-            for (int j = 0; j < n && !dead; ++j) {
-              const bool more = j + 1 < n;
-              const uint32_t v_addr = full(e);
-              for (int g = 0; g <= last; ++g) {
-                values(g, v_addr, j == 0);
-                if (g == last) tc::commit(BAR(KV_EMPTY + e % NS));
-                if (!more) { tc::commit(BAR(O_FULL + g)); continue; }
-                if (g == 0) k_addr = full(e + 1);
-                scores(g, k_addr);
-                if (g == last) tc::commit(BAR(KV_EMPTY + (e + 1) % NS));
-              }
-              if (j + 2 == n) tc::commit(BAR(Q_EMPTY));
-              e += more ? 2 : 1;
+          auto free_entry = [&](uint32_t entry) { tc::commit(BAR(KV_EMPTY + entry % NS)); };
+          for (int g = 0; g <= last; ++g, items ^= 1u << (g - 1)) WAIT(BAR(Q_FULL + g), (items >> g) & 1);
+          tc::fence_after();
+          const int lead = min(n, S::kLead << it.halves);
+          for (int t = 0; t < lead; ++t, ++e) {
+            const uint32_t k_addr = full(e);
+            if (it.halves) {
+              scores(t & 1, k_addr, t >= 2);
+            } else {
+              for (int g = 0; g <= last; ++g) scores(g, k_addr, t >= 1);
             }
-          } else {
-            for (int g = 0; g < 2; ++g, ++e) {
-              scores(g, full(e));
-              tc::commit(BAR(KV_EMPTY + e % NS));
+            free_entry(e);
+            if (t == n - 1)
+              for (int g = 0; g <= last; ++g) tc::commit(BAR(Q_EMPTY + g));
+          }
+          for (int t = 0; t < n && !dead; ++t) {
+            const int kt = t + lead;
+            const bool more = kt < n;
+            const uint32_t v_addr = full(e);
+            uint32_t k_addr = 0;
+            const int g0 = it.halves ? t & 1 : 0, g1 = it.halves ? t & 1 : last;
+            for (int g = g0; g <= g1; ++g) {
+              values(g, v_addr, t < 1 + it.halves, t + 1 + it.halves >= n);
+              if (g == g1) free_entry(e);
+              if (!more) continue;
+              if (g == g0) k_addr = full(e + 1);
+              scores(g, k_addr, true);
+              if (g == g1) free_entry(e + 1);
+              if (kt == n - 1) tc::commit(BAR(Q_EMPTY + (it.halves ? 0 : g)));
             }
-            if (n == 2) tc::commit(BAR(Q_EMPTY));
-            for (int t = 0; t < n && !dead; ++t) {
-              const int g = t & 1;
-              const uint32_t v_addr = full(e);
-              values(g, v_addr, t < 2);
-              tc::commit(BAR(KV_EMPTY + e % NS));
-              ++e;
-              if (t + 2 < n) {
-                scores(g, full(e));
-                tc::commit(BAR(KV_EMPTY + e % NS));
-                ++e;
-                if (t + 3 == n) tc::commit(BAR(Q_EMPTY));
-              } else {
-                tc::commit(BAR(O_FULL + g));
-              }
-            }
+            e += more ? 2 : 1;
           }
         }
       }
@@ -338,9 +383,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
     // ---- softmax: thread = row of its group = lane of tensor memory ----
     const int g = warp >> 2, r_in = threadIdx.x & 127;
-    const uint32_t t_s = tmem + g * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16), t_o = t_s + kColO;
+    const uint32_t t_s = tmem + g * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16), t_o = t_s + kColO, t_p = t_s + S::kColP;
     const float sl2 = a.scale * kLog2e;
-    uint32_t e0 = 0, done = 0, finished = 0;                     // ring entries before this item; the group's key tiles and items
+    uint32_t e0 = 0, done = 0, finished = 0;                     // ring entries before this item; the group's key tiles; its commits to O_FULL awaited
     for (int r = 0; !dead; ++r) {
       const int w = work_at(r, a.n_work);
       if (w < 0) break;
@@ -369,6 +414,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const bool working = (row & ~31) < it.rows;                // some row of this warp is the item's
       float m_used = -INFINITY, l0 = 0.f, l1 = 0.f;
       const int step = it.halves ? 2 : 1;
+      // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring held.  Cleared
+      // before the group's threads report the tile's P, so that 0 * x stays 0.
+      auto clear_tail = [&](int t, int valid) {
+        if (t < n - 1 || valid >= kTileKeys || (g == 1 && !it.halves)) return;
+        WAIT(BAR(KV_FULL + last_v % NS), (last_v / NS) & 1);
+        if (r_in >= valid) {
+#pragma unroll
+          for (int h = 0; h < S::kHalves; ++h) {
+            unsigned char* v = base_ptr + S::kRing + (last_v % NS) * S::kTile + h * kBlockBytes + r_in * 128;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      };
       for (int t = it.halves ? g : 0; t < n; t += step, ++done) {
         WAIT(BAR(S_FULL + g), done & 1);
         tc::fence_after();
@@ -378,6 +438,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
           for (int c = 0; c < kTileKeys; c += 32) tc::ld32(t_s + c, reinterpret_cast<uint32_t*>(sc) + c);
           tc::wait_ld();
+          if constexpr (S::kLead > 1) {
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_warp(BAR(S_READ + g));
+          }
           if (valid < kTileKeys) {
 #pragma unroll
             for (int i = 0; i < kTileKeys; ++i)
@@ -394,7 +459,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (t < step) {
             m_used = mx;
           } else if (__any_sync(0xffffffffu, (mx - m_used) * sl2 > kRescale)) {
-            // The group's product before this one is complete: its next scores, which have arrived, were issued behind it.
+            // The group's product before this one is complete: where nothing is waited for, its next scores, which have arrived,
+            // were issued behind it.
+            if constexpr (S::kLead > 1) {
+              WAIT(BAR(O_FULL + g), finished & 1);
+              tc::fence_after();
+            }
             const float m_new = (mx - m_used) * sl2 > kRescale ? mx : m_used;
             const float f = ex2((m_used - m_new) * sl2);
             m_used = m_new;
@@ -411,6 +481,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
           }
           const float neg = -m_used * sl2;
+          if constexpr (S::kLead > 1) {                          // P of the tile before has been read
+            if (t >= step) {
+              WAIT(BAR(O_FULL + g), finished & 1);
+              ++finished;
+              tc::fence_after();
+            }
+          }
 #pragma unroll
           for (int c = 0; c < kTileKeys; c += 32) {
             uint32_t pk[16];
@@ -423,25 +500,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               add2(l0, l1, x0, x1);
               pk[i] = pack2<T>(x0, x1);
             }
-            tc::st16(t_s + c / 2, pk);
-          }
-        }
-        if (t == n - 1 && valid < kTileKeys && (g == 0 || it.halves)) {
-          // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring
-          // held.  Cleared, so that 0 * x stays 0.
-          WAIT(BAR(KV_FULL + last_v % NS), (last_v / NS) & 1);
-          if (r_in >= valid) {
-#pragma unroll
-            for (int h = 0; h < S::kHalves; ++h) {
-              unsigned char* v = base_ptr + S::kRing + (last_v % NS) * S::kTile + h * kBlockBytes + r_in * 128;
-#pragma unroll
-              for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            tc::st16(t_p + c / 2, pk);
+            if (S::kLead == 1 && c == 32) {
+              clear_tail(t, valid);
+              tc::wait_st();
+              tc::fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_warp(BAR(P_HALF + g));
             }
           }
-          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+          if (S::kLead > 1) clear_tail(t, valid);
+          tc::wait_st();
+          tc::fence_before();
+        } else {
+          // no row of this warp's is the item's: it keeps step only
+          if constexpr (S::kLead > 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive_warp(BAR(S_READ + g));
+            if (t >= step) {
+              WAIT(BAR(O_FULL + g), finished & 1);
+              ++finished;
+            }
+          }
+          clear_tail(t, valid);
+          if constexpr (S::kLead == 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive_warp(BAR(P_HALF + g));
+          }
         }
-        if (working) tc::wait_st();
-        tc::fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_warp(BAR(P_FULL + g));
       }
@@ -450,40 +536,44 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       ++finished;
       tc::fence_after();
       if (!working) continue;
+      // A thread holds a row; stored as it is, every instruction would touch 32 rows, 16 bytes each (an item's output then took
+      // 20,000 cycles, the next one's Q behind it).  Eight lanes exchange their pieces instead and store whole lines.
       const float l = l0 + l1;
-      if (it.part < 0) {
-        const float inv = 1.f / l;
-        T* o = static_cast<T*>(a.out) + (static_cast<size_t>(rt.token) * a.q_heads + head) * D;
+      const bool partial = it.part >= 0;
+      const size_t p = static_cast<size_t>(rt.part_base + it.part + (it.halves ? g : 0)) * a.q_heads + head;
+      unsigned long long to = 0;
+      if (mine) {
+        to = partial ? reinterpret_cast<unsigned long long>(a.part_acc + p * D)
+                     : reinterpret_cast<unsigned long long>(static_cast<T*>(a.out) + (static_cast<size_t>(rt.token) * a.q_heads + head) * D);
+        if (partial) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_used * a.ml_scale, l);
+      }
+      const float inv = 1.f / l;
+      auto store_line = [&](uint32_t (&x)[32], int at) {       // 128 bytes of every lane's row, at byte `at` of the row
+        transpose8(x, lane);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const unsigned long long row_to = __shfl_sync(0xffffffffu, to, (lane & 24) + i);
+          if (row_to) *reinterpret_cast<uint4*>(row_to + at + (lane & 7) * 16) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        }
+      };
+      if (partial) {
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           uint32_t v[32];
           tc::ld32(t_o + c, v);
           tc::wait_ld();
-          if (mine) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 x;
-              x.x = pack2<T>(__uint_as_float(v[i]) * inv, __uint_as_float(v[i + 1]) * inv);
-              x.y = pack2<T>(__uint_as_float(v[i + 2]) * inv, __uint_as_float(v[i + 3]) * inv);
-              x.z = pack2<T>(__uint_as_float(v[i + 4]) * inv, __uint_as_float(v[i + 5]) * inv);
-              x.w = pack2<T>(__uint_as_float(v[i + 6]) * inv, __uint_as_float(v[i + 7]) * inv);
-              *reinterpret_cast<uint4*>(o + c + i) = x;
-            }
-          }
+          store_line(v, c * 4);
         }
       } else {
-        const size_t p = static_cast<size_t>(rt.part_base + it.part + (it.halves ? g : 0)) * a.q_heads + head;
-        float* o = a.part_acc + p * D;
-        if (mine) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_used * a.ml_scale, l);
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t v[32];
+        for (int c = 0; c < D; c += 64) {
+          uint32_t v[64], x[32];
           tc::ld32(t_o + c, v);
+          tc::ld32(t_o + c + 32, v + 32);
           tc::wait_ld();
-          if (mine) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(o + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-          }
+          for (int i = 0; i < 32; ++i) x[i] = pack2<T>(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
+          store_line(x, c * 2);
         }
       }
       tc::fence_before();

@@ -65,9 +65,10 @@ template <int COLUMNS> __device__ __forceinline__ void dealloc(uint32_t tmem) {
 // Shared-memory operand with the 128-byte swizzle: rows of 128 bytes, 8 to a 1,024-byte group.  K-major operands (rows
 // are M or N, a row's 64 elements K) step 32 bytes a K = 16; MN-major ones (rows are K, a row's 64 elements N) step 16
 // rows, and `block` is the distance from one 64-element block of N to the next.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t block = 16) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | static_cast<uint64_t>((block >> 4) & 0x3FFFu) << 16 |
-         static_cast<uint64_t>(1024u >> 4) << 32 | static_cast<uint64_t>(1u) << 46 | static_cast<uint64_t>(2u) << 61;
+// (address / 16; the rest is a constant.)
+__device__ __forceinline__ uint64_t operand_at(uint32_t addr16, uint32_t block = 16) {
+  const uint32_t lo = addr16 | (block >> 4) << 16, hi = (1024u >> 4) | 1u << 14 | 2u << 29;
+  return static_cast<uint64_t>(hi) << 32 | lo;
 }
 // kind::f16, fp32 accumulators, M = 128
 __host__ __device__ constexpr uint32_t instruction(bool bf16, int n, bool b_mn_major) {

@@ -15,7 +15,7 @@
 //                   rescaled only when a row's maximum has grown by more than 2^8.
 //   warp 8          TMA: K and V tiles through the block table into a ring (boxes of up to 128 slots x 128 bytes).
 //   warp 9          issues the products, one thread: S = Q K^T and O += P V of both groups in turns.
-//   warps 10, 11    gather group 0's, 1's rows of Q for the next item, whatever tokens and heads they are.
+//   warp 10         TMA: the next item's rows of Q, a box for each token's heads, or for several consecutive tokens'.
 //
 // head_dim 64: P has 64 columns of its own.  The next scores of a group are issued as soon as its threads hold the present ones
 // in registers, so the softmax warps never wait for a product: the exponentials decide.
@@ -54,10 +54,11 @@ namespace {
 constexpr int kTileThreads = 384;
 // Registers a thread of the softmax warps and of the others; launched with 168 each (2 x 208 + 80 <= 3 x 168).
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
-constexpr int kProducer = 8, kIssuer = 9, kGatherer = 10;   // and 11
+constexpr int kProducer = 8, kIssuer = 9, kRowsLoader = 10;   // the 12th warp idles: registers are split by fours
 constexpr int kBlockBytes = 128 * 128;                   // 128 rows x 64 16-bit elements: one operand block
 constexpr uint32_t kGroupCols = 256, kColO = 128;        // tensor memory of a group: S, then O ...
 constexpr float kRescale = 8.f;                          // in log2 units: P stays below 2^8
+constexpr int kBoxRows = 64;                             // rows of Q, at most, that a box of several tokens brings
 constexpr int kMinTileTokens = 4;                        // sequences with fewer tokens go to the decode kernels
 constexpr int kMinPrefixTokens = 2;                      // batches of fewer tokens behind the prefix, too
 
@@ -67,12 +68,13 @@ template <int D> struct TileSmem {
   static constexpr int kStages = D == 64 ? 8 : 5;
   static constexpr uint32_t kColP = D == 64 ? 192 : 0;   // ... and P behind O, or over S
   static constexpr int kLead = D == 64 ? 2 : 1;          // key tiles a group's scores are issued ahead of its values
-  static constexpr int kRing = 2 * kTile;
+  // Q: half (64 dims) by half, 256 rows each; the next item's beside the present one's where there is room
+  static constexpr int kQ = 2 * kTile, kQBufs = D == 64 ? 2 : 1, kQHalf = 2 * kBlockBytes;
+  static constexpr int kRing = kQBufs * kQ;
   static constexpr int kBytes = kRing + kStages * kTile + 1024;
 };
 
 struct TileArgs {
-  const void* q;
   const int *block_tables, *table_offset, *token_seq;
   const RowToken* rows;
   const TileItem* tiles;
@@ -81,6 +83,7 @@ struct TileArgs {
   int n_work;                        // items x kv heads
   int q_heads, kv_heads, group;
   int block_size, bs_log2, box_log2; // a TMA box is 1 << box_log2 slots
+  int box_tokens;                    // tokens of a box of the second Q map (the first: one)
   float scale;
   float ml_scale;                    // what partial maxima are multiplied with: scale, or scale log2 e
   unsigned int* host_err;
@@ -137,12 +140,13 @@ __device__ __forceinline__ int work_at(int r, int n_work) {
 }
 __device__ __forceinline__ TileItem load_tile(const TileItem* p) {
   const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
-  return TileItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  return TileItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z != 0, b.w};
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    tile_attn_kernel(const TileArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    tile_attn_kernel(const TileArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap qmap_many,
+                     const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using S = TileSmem<D>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kInstrQK = tc::instruction(kBf16, kTileKeys, false), kInstrPV = tc::instruction(kBf16, D, true);
@@ -165,7 +169,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(BAR(KV_EMPTY + i), 1);  // commit after the last product that reads the stage
     }
     for (int g = 0; g < 2; ++g) {
-      mbar_init(BAR(Q_FULL + g), 1);    // the group's gatherer, its copies done
+      mbar_init(BAR(Q_FULL + g), 1);    // (of a buffer, not of a group)
       mbar_init(BAR(Q_EMPTY + g), 1);   // commit after the item's last Q K^T
       mbar_init(BAR(S_FULL + g), 1);    // commit after the group's Q K^T
       mbar_init(BAR(S_READ + g), 128);  // kLead 2: the group's softmax threads (32 at a time) hold S in registers
@@ -246,60 +250,42 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (uint32_t i = e > NS ? e - NS : 0; i < e; ++i) mbar_wait(BAR(KV_FULL + i % NS), (i / NS) & 1);
       }
       __syncwarp();
-    } else if (warp != kIssuer) {
-      constexpr int kRowBytes = D * 2;
-      const int g = warp - kGatherer, piece = lane & 7;              // 16-byte piece of a 128-byte operand row
-      const unsigned char* q = static_cast<const unsigned char*>(a.q);
-      uint32_t items = 0;
-      for (int r = 0; !dead; ++r) {
+    } else if (warp == kRowsLoader) {
+      int r = 0;
+      for (; !dead; ++r) {
         const int w = work_at(r, a.n_work);
         if (w < 0) break;
         const TileItem it = load_tile(a.tiles + w / a.kv_heads);
-        const int kvh = w % a.kv_heads, rows = it.rows - g * 128;
-        if (rows <= 0) continue;
-        int place[4];                                                // (token, head) row of rows lane, 32 + lane, ... in q, or -1
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          place[u] = -1;
-          if (32 * u + lane < rows) {
-            const int f = it.f0 + g * 128 + 32 * u + lane, t = f / a.group;
-            place[u] = __ldg(&a.rows[it.tok0 + t].token) * a.q_heads + kvh * a.group + (f - t * a.group);
-            // into L2 while the item before is still being worked on: copies that miss it go out few at a time
-#pragma unroll
-            for (int h = 0; h < S::kHalves; ++h) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + static_cast<size_t>(place[u]) * kRowBytes + h * 128));
-          }
+        const int kvh = w % a.kv_heads, qb = r % S::kQBufs;
+        const uint32_t bar = BAR(Q_FULL + qb), dst = base + qb * S::kQ;
+        const int many = (it.flags & kConsecutive) ? it.n_tok / a.box_tokens : 0, boxes = many + it.n_tok - many * a.box_tokens;
+        if (lane == 0) {
+          WAIT(BAR(Q_EMPTY + qb), ((r / S::kQBufs) & 1) ^ 1);
+          if (!dead) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(it.n_tok * a.group) * 128u * S::kHalves);
         }
-        if (lane == 0) WAIT(BAR(Q_EMPTY + g), (items & 1) ^ 1);
         dead = __shfl_sync(0xffffffffu, dead ? 1 : 0, 0) != 0;
         if (dead) break;
-#pragma unroll 1
-        for (int u = 0; u < 4; ++u) {
-          const int here = u == 0 ? place[0] : u == 1 ? place[1] : u == 2 ? place[2] : place[3];
-          uint32_t dst = base + g * S::kTile + (32 * u + (lane >> 3)) * 128 + ((piece ^ (lane >> 3)) << 4);
+        for (int b = lane; b < boxes; b += 32) {
+          const int first = b < many ? b * a.box_tokens : b + many * (a.box_tokens - 1);   // its first token
+          const int token = __ldg(&a.rows[it.tok0 + first].token);
+          const uint32_t to = dst + first * a.group * 128;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int from = __shfl_sync(0xffffffffu, here, 4 * i + (lane >> 3));
-            const unsigned char* src = q + static_cast<size_t>(max(from, 0)) * kRowBytes + piece * 16;
-            const uint32_t to = (dst ^ ((i & 1) << 6)) + i * 512;    // row & 7 is lane / 8 + 4 (i & 1)
-#pragma unroll
-            for (int h = 0; h < S::kHalves; ++h) cp_async16(to + h * kBlockBytes, src + h * 128, from >= 0 ? 16 : 0);
-          }
+          for (int h = 0; h < S::kHalves; ++h) tma_load_3d(to + h * S::kQHalf, b < many ? &qmap_many : &qmap, h * 64, kvh * a.group, token, bar);
         }
-        cp_async_commit();
-        cp_async_wait_all();
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(BAR(Q_FULL + g));
-        ++items;
       }
-    } else {
       if (lane == 0) {
-        uint32_t e = 0, done = 0, read = 0, items = 0;             // ring entries; bit g: parity of group g's P and S taken, of its Q tiles
+        for (int i = max(r - S::kQBufs, 0); i < r; ++i) mbar_wait(BAR(Q_FULL + i % S::kQBufs), (i / S::kQBufs) & 1);
+      }
+      __syncwarp();
+    } else if (warp == kIssuer) {
+      if (lane == 0) {
+        uint32_t e = 0, done = 0, read = 0;                        // ring entries; bit g: parity of group g's P and S taken
         for (int r = 0; !dead; ++r) {
           const int w = work_at(r, a.n_work);
           if (w < 0) break;
           const TileItem it = load_tile(a.tiles + w / a.kv_heads);
-          const int n = (it.kv_len + kTileKeys - 1) / kTileKeys, last = it.rows > 128 ? 1 : 0;   // last group
+          const int n = (it.kv_len + kTileKeys - 1) / kTileKeys, last = it.n_tok * a.group > 128 ? 1 : 0, qb = r % S::kQBufs;   // last group; buffer of Q
           // waits for the ring entry and returns where it lies
           auto full = [&](uint32_t entry) {
             WAIT(BAR(KV_FULL + entry % NS), (entry / NS) & 1);
@@ -317,13 +303,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               // counted by tiles: the phase of an item's last tile, which nobody waits for, is over when its P is there
               if (read_first) read ^= 1u << g;
             }
-            uint32_t q_lo = (base + (it.halves ? 0 : g) * S::kTile) >> 4, k_lo = k_addr >> 4;
+            uint32_t q_lo = (base + qb * S::kQ + (it.halves ? 0 : g) * kBlockBytes) >> 4, k_lo = k_addr >> 4;
             const uint32_t d = tmem + g * kGroupCols;
             asm volatile("" : "+r"(q_lo), "+r"(k_lo));
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
-              const uint32_t step = (ks >> 2) * (kBlockBytes >> 4) + (ks & 3) * 2;
-              tc::mma_ss(d, tc::operand_at(q_lo + step), tc::operand_at(k_lo + step), kInstrQK, ks > 0);
+              tc::mma_ss(d, tc::operand_at(q_lo + (ks >> 2) * (S::kQHalf >> 4) + (ks & 3) * 2),
+                         tc::operand_at(k_lo + (ks >> 2) * (kBlockBytes >> 4) + (ks & 3) * 2), kInstrQK, ks > 0);
             }
             tc::commit(BAR(S_FULL + g));
           };
@@ -344,7 +330,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (final || S::kLead > 1) tc::commit(BAR(O_FULL + g));
           };
           auto free_entry = [&](uint32_t entry) { tc::commit(BAR(KV_EMPTY + entry % NS)); };
-          for (int g = 0; g <= last; ++g, items ^= 1u << (g - 1)) WAIT(BAR(Q_FULL + g), (items >> g) & 1);
+          WAIT(BAR(Q_FULL + qb), (r / S::kQBufs) & 1);
           tc::fence_after();
           const int lead = min(n, S::kLead << it.halves);
           for (int t = 0; t < lead; ++t, ++e) {
@@ -355,8 +341,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               for (int g = 0; g <= last; ++g) scores(g, k_addr, t >= 1);
             }
             free_entry(e);
-            if (t == n - 1)
-              for (int g = 0; g <= last; ++g) tc::commit(BAR(Q_EMPTY + g));
+            if (t == n - 1) tc::commit(BAR(Q_EMPTY + qb));
           }
           for (int t = 0; t < n && !dead; ++t) {
             const int kt = t + lead;
@@ -370,8 +355,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               if (!more) continue;
               if (g == g0) k_addr = full(e + 1);
               scores(g, k_addr, true);
-              if (g == g1) free_entry(e + 1);
-              if (kt == n - 1) tc::commit(BAR(Q_EMPTY + (it.halves ? 0 : g)));
+              if (g == g1) {
+                free_entry(e + 1);
+                if (kt == n - 1) tc::commit(BAR(Q_EMPTY + qb));
+              }
             }
             e += more ? 2 : 1;
           }
@@ -394,24 +381,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const uint32_t last_v = e0 + 2 * n - 1;                    // ring entry of the last V tile
       e0 += 2 * n;
       const int row = it.halves ? r_in : g * 128 + r_in;         // row of the item
-      const bool mine = row < it.rows;
+      const int rows = it.n_tok * a.group;
+      const bool mine = row < rows;
       RowToken rt{0, 0};
       int head = 0;
       if (mine) {
-        const int f = it.f0 + row, t = f / a.group;
+        const int t = row / a.group;
         const int2 x = __ldg(reinterpret_cast<const int2*>(a.rows + it.tok0 + t));
         rt = RowToken{x.x, x.y};
-        head = kvh * a.group + (f - t * a.group);
+        head = kvh * a.group + (row - t * a.group);
       }
-      if (g == 1 && !it.halves && it.rows <= 128) {
-        if (it.pad && r_in < it.rows) {                          // the others of the segment leave two partials
-          const int f = it.f0 + r_in, t = f / a.group;
-          const size_t p = static_cast<size_t>(__ldg(&a.rows[it.tok0 + t].part_base) + it.part + 1) * a.q_heads + kvh * a.group + (f - t * a.group);
+      if (g == 1 && !it.halves && rows <= 128) {
+        if ((it.flags & kEmptySecond) && r_in < rows) {          // the others of the segment leave two partials
+          const int t = r_in / a.group;
+          const size_t p = static_cast<size_t>(__ldg(&a.rows[it.tok0 + t].part_base) + it.part + 1) * a.q_heads + kvh * a.group + (r_in - t * a.group);
           *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(-INFINITY, 0.f);
         }
         continue;
       }
-      const bool working = (row & ~31) < it.rows;                // some row of this warp is the item's
+      const bool working = (row & ~31) < rows;                // some row of this warp is the item's
       float m_used = -INFINITY, l0 = 0.f, l1 = 0.f;
       const int step = it.halves ? 2 : 1;
       // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring held.  Cleared
@@ -470,7 +458,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             m_used = m_new;
             l0 *= f;
             l1 *= f;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D; c += 32) {
               uint32_t v[32];
               tc::ld32(t_o + c, v);
@@ -557,7 +545,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       };
       if (partial) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t v[32];
           tc::ld32(t_o + c, v);
@@ -565,7 +553,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           store_line(v, c * 4);
         }
       } else {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D; c += 64) {
           uint32_t v[64], x[32];
           tc::ld32(t_o + c, v);
@@ -660,8 +648,19 @@ __global__ void __launch_bounds__(kMergeThreads) segment_merge_kernel(const Merg
 }
 
 // ---------------------------------------------------------------- launches ----
+// Rows of q as [tokens][heads][head_dim], fetched in boxes of 64 dims x heads x tokens.
+int make_q_map(CUtensorMap* map, const void* q, PoolElem elem, int head_dim, int heads, int n_tokens, int box_heads, int box_tokens) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(n_tokens)};
+  const cuuint64_t strides[2] = {dims[0] * 2, dims[0] * dims[1] * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)}, step[3] = {1, 1, 1};
+  const CUresult r = tensor_map_encoder()(map, elem == PoolElem::kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                                          const_cast<void*>(q), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? PKV_OK : fail(PKV_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+}
+
 template <typename T, int D>
-int launch_tiles(const TileArgs& a, const void* k_cache, const void* v_cache, uint64_t pool_rows, cudaStream_t stream) {
+int launch_tiles(const TileArgs& a, const void* q, int n_tokens, const void* k_cache, const void* v_cache, uint64_t pool_rows, cudaStream_t stream) {
   using S = TileSmem<D>;
   auto kern = tile_attn_kernel<T, D>;
   static thread_local int configured_device = -1;
@@ -673,11 +672,13 @@ int launch_tiles(const TileArgs& a, const void* k_cache, const void* v_cache, ui
     configured_device = dev;
   }
   constexpr PoolElem elem = std::is_same<T, __half>::value ? PoolElem::kF16 : PoolElem::kBF16;
-  alignas(64) CUtensorMap kmap, vmap;
-  int st = make_pool_tensor_map(&kmap, k_cache, elem, a.kv_heads * D, 1u << a.box_log2, pool_rows);
+  alignas(64) CUtensorMap qmap, qmap_many, kmap, vmap;
+  int st = make_q_map(&qmap, q, elem, D, a.q_heads, n_tokens, a.group, 1);
+  if (st == PKV_OK) st = make_q_map(&qmap_many, q, elem, D, a.q_heads, n_tokens, a.group, a.box_tokens);
+  if (st == PKV_OK) st = make_pool_tensor_map(&kmap, k_cache, elem, a.kv_heads * D, 1u << a.box_log2, pool_rows);
   if (st == PKV_OK) st = make_pool_tensor_map(&vmap, v_cache, elem, a.kv_heads * D, 1u << a.box_log2, pool_rows);
   if (st != PKV_OK) return st;
-  launch_pdl(kern, dim3(static_cast<unsigned>(std::min(a.n_work, decode_sms()))), dim3(kTileThreads), S::kBytes, stream, a, kmap, vmap);
+  launch_pdl(kern, dim3(static_cast<unsigned>(std::min(a.n_work, decode_sms()))), dim3(kTileThreads), S::kBytes, stream, a, qmap, qmap_many, kmap, vmap);
   return check_launch("tile_attn_kernel");
 }
 
@@ -706,7 +707,7 @@ SegmentOffsets segment_offsets(const SegmentGeometry& g, size_t rows, size_t ite
 // For any step of these sizes: tiles of uncut segments, and one more item at most for every partial.
 SegmentOffsets segment_bounds(const SegmentGeometry& g, bool prefix) {
   const size_t n = static_cast<size_t>(g.n_tokens), slots = static_cast<size_t>(tile_slots(g, decode_sms())) + (prefix ? n : 0);
-  const size_t tiles = n * g.group() / kTileRows + n + slots;
+  const size_t tiles = n + slots;                            // (an uncut tile has a token at least)
   const size_t items = n + own_extra(g) + 2;
   return segment_offsets(g, n, items, items + 1, tiles, n, static_cast<size_t>(most_parts(g, decode_sms(), prefix)));
 }
@@ -865,18 +866,19 @@ int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const v
     if constexpr (sizeof(T) == 2) {
       if (!tensor_map_encoder()) return fail(PKV_E_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", fn);
       TileArgs a;
-      a.q = q; a.block_tables = block_tables; a.table_offset = table_offset; a.token_seq = seq;
+      a.block_tables = block_tables; a.table_offset = table_offset; a.token_seq = seq;
       a.rows = reinterpret_cast<const RowToken*>(ws + plan->off_rows);
       a.tiles = reinterpret_cast<const TileItem*>(ws + plan->off_tiles);
       a.out = out; a.part_ml = ml; a.part_acc = acc;
       a.n_work = plan->n_tiles * plan->kv_heads;
       a.q_heads = plan->q_heads; a.kv_heads = plan->kv_heads; a.group = group;
       a.block_size = plan->block_size; a.bs_log2 = log2_floor(plan->block_size); a.box_log2 = std::min(a.bs_log2, 7);
+      a.box_tokens = std::max(1, kBoxRows / group);
       a.scale = scale;
       a.ml_scale = log2_domain ? scale * 1.4426950408889634f : scale;
       a.host_err = host_err;
       const uint64_t rows = pool_rows ? pool_rows : 1ull << 30;
-      st = D == 64 ? launch_tiles<T, 64>(a, k_cache, v_cache, rows, s) : launch_tiles<T, 128>(a, k_cache, v_cache, rows, s);
+      st = D == 64 ? launch_tiles<T, 64>(a, q, plan->n_tokens, k_cache, v_cache, rows, s) : launch_tiles<T, 128>(a, q, plan->n_tokens, k_cache, v_cache, rows, s);
       if (st != PKV_OK) return st;
     }
   }

@@ -29,22 +29,26 @@ constexpr int kTileRows = 256;      // rows of a tile item: two groups of 128
 constexpr int kTileKeys = 128;      // keys per step of the tile kernel
 
 struct RowToken { int token, part_base; };
-// Rows f0 .. f0 + rows - 1 of a segment whose tokens are row_tokens[tok0 ..]: row f is token f / group, head f % group.
+// The rows of tokens row_tokens[tok0 ..] of a segment: row r is token r / group, head r % group.
 struct TileItem {
-  int tok0, f0, rows;
+  int tok0, n_tok;
   int kv_begin, kv_len;             // kv_begin a multiple of kTileKeys
   int part;                         // partial slot behind the token's part_base, or -1: write the output
+  int flags;
   int halves;                       // 1: at most 128 rows; the two groups take every other key tile, partials part and part + 1
   int pad;
 };
+constexpr int kConsecutive = 1;     // the tokens are consecutive rows of q
+constexpr int kEmptySecond = 2;     // the others of the segment are halved: leave an empty partial part + 1
 struct MergeRow { int token, part_base, n_parts, pad; };   // n_parts 0: no keys, the output is zero
 
 struct SegmentGeometry {
   int n_tokens, q_heads, kv_heads, head_dim, block_size, elem_bytes;
   int group() const { return q_heads / kv_heads; }
+  int tile_tokens() const { return kTileRows / group(); }      // of a full tile
   // whether the tile kernel is written for it
   bool tiles() const {
-    return elem_bytes == 2 && (head_dim == 64 || head_dim == 128) && block_size >= 16 && (block_size & (block_size - 1)) == 0;
+    return elem_bytes == 2 && group() <= kTileRows && (head_dim == 64 || head_dim == 128) && block_size >= 16 && (block_size & (block_size - 1)) == 0;
   }
 };
 
@@ -67,7 +71,7 @@ struct SegmentLists {
 
 // Partials that tile items may leave in all, beyond one per token: two rounds of tile items on every SM.
 inline long long tile_slots(const SegmentGeometry& g, int sms) {
-  return static_cast<long long>((2 * sms + g.kv_heads - 1) / g.kv_heads) * (kTileRows / g.group() + 2);
+  return static_cast<long long>((2 * sms + g.kv_heads - 1) / g.kv_heads) * (g.group() <= kTileRows ? g.tile_tokens() + 2 : 0);
 }
 inline int own_extra(const SegmentGeometry& g) { return decode_max_extra(g.kv_heads); }
 // Most partials of a step: prefix steps leave one of each kind per token even when nothing is cut.
@@ -90,7 +94,8 @@ inline void cut_segments(std::vector<Segment>& segs, const SegmentGeometry& g, i
     long long used = 0;
     for (const Segment& s : segs) {
       const int kt = (s.kv_len + kTileKeys - 1) / kTileKeys, c = (kt + len - 1) / len, per = (kt + c - 1) / c;
-      const long long rows = static_cast<long long>(s.n_tok) * g.group(), full = rows / kTileRows, rest = rows - full * kTileRows;
+      const long long full = s.n_tok / g.tile_tokens(), rest = (s.n_tok - full * g.tile_tokens()) * static_cast<long long>(g.group());
+      const long long rows = static_cast<long long>(s.n_tok) * g.group();
       const bool halves = rest > 0 && rest <= kTileRows / 2 && (prefix || c > 1) && per > 1;
       if (prefix || c > 1) used += s.n_tok * static_cast<long long>(c * (rows <= kTileRows / 2 && per > 1 ? 2 : 1));
       const double two = kItemCost + kTwoGroups * per, one = kItemCost + (halves ? 0.55 : 1.0) * per;
@@ -159,8 +164,7 @@ inline void list_segments(std::vector<Segment>& segs, const std::vector<OwnRange
   cut_segments(segs, g, sms, tile_slots(g, sms) + (prefix ? g.n_tokens : 0), prefix);
   std::vector<int> pieces;
   cut_own(own, g, own_extra(g), out, pieces);
-  // the tiles, with the partials of each of their tokens numbered from 0; a token whose rows lie in two items is counted by
-  // the larger number (the merge reads what was written: see `halves` below)
+  // the tiles, with the partials of each of their tokens numbered from 0
   const int group = g.group();
   for (Segment& s : segs) {
     const int kt = (s.kv_len + kTileKeys - 1) / kTileKeys, per = (kt + s.chunks - 1) / s.chunks;
@@ -173,14 +177,17 @@ inline void list_segments(std::vector<Segment>& segs, const std::vector<OwnRange
     for (int c = 0; c < s.chunks; ++c) {
       const int begin = c * per * kTileKeys, len = std::min(per * kTileKeys, s.kv_len - begin);
       const bool two = halves && len > kTileKeys;
-      for (long long f = 0; f < rows; f += kTileRows)
-        out.tiles.push_back(TileItem{s.tok0, static_cast<int>(f), static_cast<int>(std::min<long long>(kTileRows, rows - f)), begin, len,
-                                     partial ? c * (halves ? 2 : 1) : -1, two ? 1 : 0, halves && !two ? 1 : 0});
+      for (int t = 0; t < s.n_tok; t += g.tile_tokens()) {
+        const int n = std::min(g.tile_tokens(), s.n_tok - t), tok0 = s.tok0 + t;
+        const bool row = out.rows[tok0 + n - 1].token - out.rows[tok0].token == n - 1;      // (they ascend)
+        out.tiles.push_back(TileItem{tok0, n, begin, len, partial ? c * (halves ? 2 : 1) : -1,
+                                     (row ? kConsecutive : 0) | (halves && !two ? kEmptySecond : 0), two ? 1 : 0, 0});
+      }
     }
   }
-  auto cost = [](const TileItem& t) {
+  auto cost = [group](const TileItem& t) {
     const int kt = (t.kv_len + kTileKeys - 1) / kTileKeys;
-    return t.halves ? (kt + 1) / 2 * 2 : kt * (t.rows > kTileRows / 2 ? 3 : 2);
+    return t.halves ? (kt + 1) / 2 * 2 : kt * (t.n_tok * group > kTileRows / 2 ? 3 : 2);
   };
   std::stable_sort(out.tiles.begin(), out.tiles.end(), [&](const TileItem& x, const TileItem& y) { return cost(x) > cost(y); });
   // partial slots: a token's tiles' first, then its own pieces'

@@ -14,7 +14,7 @@ class Image:
             return raw[off:off + 4 * n * width].copy().view(np.int32).reshape(n, width)
 
         self.items = ints(p.off_items, p.n_items, 4)                      # token, kv_begin, kv_len, part
-        self.tiles = ints(p.off_tiles, p.n_tiles, 8)                      # tok0, f0, rows, kv_begin, kv_len, part, halves, empty second
+        self.tiles = ints(p.off_tiles, p.n_tiles, 8)                      # tok0, n_tok, kv_begin, kv_len, part, flags, halves, -
         self.merge = ints(p.off_merge, p.n_merged, 4)                     # token, part_base, n_parts, -
         n_rows = (p.off_items - p.off_rows) // 8
         self.rows = ints(p.off_rows, n_rows, 2)                           # token, part_base
@@ -42,12 +42,15 @@ def check_cover(image, plan, want):
     for token, begin, n, part in image.items.tolist():
         assert n > 0 and begin >= 0
         add(token, None, begin, n, part)
-    for tok0, f0, rows, begin, n, part, halves, empty in image.tiles.tolist():
+    for tok0, n_tok, begin, n, part, flags, halves, _ in image.tiles.tolist():
+        rows = n_tok * group
         assert 1 <= rows <= 256 and n > 0 and begin % 128 == 0 and not (halves and (rows > 128 or n <= 128 or part < 0))
-        for f in range(f0, f0 + rows):
+        tokens = image.rows[tok0:tok0 + n_tok, 0]
+        assert bool(flags & 1) == bool((np.diff(tokens) == 1).all())
+        for f in range(rows):
             token, base = image.rows[tok0 + f // group].tolist()
             add(token, f % group, begin, n, base + part if part >= 0 else -1)
-            if halves or empty:
+            if halves or flags & 2:
                 slots[token, f % group].append(base + part + 1)
     merged = {t: (base, n) for t, base, n, _ in image.merge.tolist()}
     assert len(merged) == len(image.merge)

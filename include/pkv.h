@@ -478,10 +478,11 @@ int pkv_prefill_attn_f16(const void* q, const void* k_cache, const void* v_cache
 typedef struct pkv_segment_plan {
   int kind, n_tokens, q_heads, kv_heads, head_dim, block_size, elem_bytes;
   int num_blocks;
-  int n_tiles, n_items, n_merged, n_parts;   /* tensor-core items, decode items, tokens that the merge writes, partials */
+  int n_tiles, n_items, n_merged;   /* tensor-core items, decode items, (token, kv head) pairs that the merge writes */
+  int n_lists, n_tile_rows, n_parts;
   int cluster, cluster_least;
   size_t image_bytes, workspace_bytes;
-  size_t off_seq, off_pos, off_rows, off_items, off_tiles, off_merge, off_ml, off_acc;
+  size_t off_seq, off_pos, off_rows, off_items, off_lists, off_tiles, off_merge, off_tile_ml, off_tile_acc, off_ml, off_acc;
 } pkv_segment_plan;
 
 size_t pkv_cross_workspace_bytes(int n_tokens, int q_heads, int kv_heads, int head_dim);

@@ -31,9 +31,9 @@ class DecodePlan(C.Structure):
 class SegmentPlan(C.Structure):
     """Mirror of struct pkv_segment_plan."""
     _fields_ = [(n, C.c_int) for n in ("kind", "n_tokens", "q_heads", "kv_heads", "head_dim", "block_size", "elem_bytes", "num_blocks",
-                                       "n_tiles", "n_items", "n_merged", "n_parts", "cluster", "cluster_least")] + \
-               [(n, C.c_size_t) for n in ("image_bytes", "workspace_bytes", "off_seq", "off_pos", "off_rows", "off_items", "off_tiles",
-                                          "off_merge", "off_ml", "off_acc")]
+                                       "n_tiles", "n_items", "n_merged", "n_lists", "n_tile_rows", "n_parts", "cluster", "cluster_least")] + \
+               [(n, C.c_size_t) for n in ("image_bytes", "workspace_bytes", "off_seq", "off_pos", "off_rows", "off_items", "off_lists", "off_tiles",
+                                          "off_merge", "off_tile_ml", "off_tile_acc", "off_ml", "off_acc")]
 
 
 _vp, _i, _f, _sz, _u64, _ll = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64, C.c_longlong

@@ -22,12 +22,12 @@
 // head_dim 128: S and O fill the group's half of tensor memory, P lies over the first half of S.  The next scores follow
 // the second product, whose first half starts when P's first 64 keys are there.
 //
-// An item of at most 128 rows whose keys are many runs both groups over the same rows, every other key tile each (`halves`).
+// An item of at most 128 rows brings those of two kv heads, one for each group, whose K and V tiles alternate in the ring.
 // P is rounded to 16 bits for the second product (the sums are of the unrounded ones), as the operands of the
 // tensor cores are; scores, sums and accumulators are fp32.
 //
-// Blocks are persistent, one on an SM, and take the list of items in a serpentine, longest first.  Every wait is
-// bounded: one that runs out sets bit 32 of the error word and the block winds down.
+// Blocks are persistent, one on an SM, each with a list of items of its own.  Every wait is bounded: one that runs
+// out sets bit 32 of the error word and the block winds down.
 #include <algorithm>
 #include <new>
 #include <type_traits>
@@ -53,7 +53,7 @@ namespace {
 
 constexpr int kTileThreads = 384;
 // Registers a thread of the softmax warps and of the others; launched with 168 each (2 x 208 + 80 <= 3 x 168).
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 constexpr int kProducer = 8, kIssuer = 9, kRowsLoader = 10;   // the 12th warp idles: registers are split by fours
 constexpr int kBlockBytes = 128 * 128;                   // 128 rows x 64 16-bit elements: one operand block
 constexpr uint32_t kGroupCols = 256, kColO = 128;        // tensor memory of a group: S, then O ...
@@ -76,12 +76,11 @@ template <int D> struct TileSmem {
 
 struct TileArgs {
   const int *block_tables, *table_offset, *token_seq;
-  const RowToken* rows;
+  const int *row_token, *list_first;
   const TileItem* tiles;
   void* out;
-  float *part_ml, *part_acc;
-  int n_work;                        // items x kv heads
-  int q_heads, kv_heads, group;
+  float *part_ml, *part_acc;         // by partial row
+  int q_heads, group;
   int block_size, bs_log2, box_log2; // a TMA box is 1 << box_log2 slots
   int box_tokens;                    // tokens of a box of the second Q map (the first: one)
   float scale;
@@ -99,19 +98,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// (a0, a1) * (s, s) + (n, n) and (a0, a1) + (b0, b1), two at a time
-__device__ __forceinline__ void fma2(float a0, float a1, float s, float n, float& r0, float& r1) {
-  asm("{\n .reg .b64 ra, rs, rn, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rs, {%4, %4};\n mov.b64 rn, {%5, %5};\n"
-      " fma.rn.f32x2 rd, ra, rs, rn;\n mov.b64 {%0, %1}, rd;\n}\n"
-      : "=f"(r0), "=f"(r1)
-      : "f"(a0), "f"(a1), "f"(s), "f"(n));
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 ra, rb, rc, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n mov.b64 rc, {%6, %7};\n"
+      " fma.rn.f32x2 rd, ra, rb, rc;\n mov.b64 {%0, %1}, rd;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
-__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
-  asm("{\n .reg .b64 ra, rb;\n mov.b64 ra, {%0, %1};\n mov.b64 rb, {%2, %3};\n add.rn.f32x2 ra, ra, rb;\n mov.b64 {%0, %1}, ra;\n}\n"
-      : "+f"(a0), "+f"(a1)
-      : "f"(b0), "f"(b1));
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n add.rn.f32x2 rd, ra, rb;\n mov.b64 {%0, %1}, rd;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
-
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // Eight 16-byte pieces a lane: piece i of lane j of every eight lanes becomes piece j of lane i.
 __device__ __forceinline__ void transpose8(uint32_t (&x)[32], int lane) {
 #pragma unroll
@@ -132,15 +135,9 @@ __device__ __forceinline__ void transpose8(uint32_t (&x)[32], int lane) {
   }
 }
 
-// The r-th item of a block, or -1.
-__device__ __forceinline__ int work_at(int r, int n_work) {
-  const int G = static_cast<int>(gridDim.x), b = static_cast<int>(blockIdx.x);
-  const long long w = static_cast<long long>(r) * G + ((r & 1) ? G - 1 - b : b);
-  return w < n_work ? static_cast<int>(w) : -1;
-}
 __device__ __forceinline__ TileItem load_tile(const TileItem* p) {
   const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
-  return TileItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z != 0, b.w};
+  return TileItem{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 }
 
 template <typename T, int D>
@@ -185,10 +182,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc::fence_after();
   const uint32_t tmem = tmem_slot;
 
+  // The plan and the index arrays were complete before the launch ahead of this one began, so the look-ups that lead to the
+  // first loads run while it is finishing; what it may have written (K, V, q, the partials' space) is touched only behind the wait.
   // The launch behind this one may be the decode kernel of the same call, which does not wait for this one before
   // it reads (decode_list.hpp): it may start once everything before this launch is complete.
-  pdl_wait();
-  pdl_launch_dependents();
+  auto after_previous = [] {
+    pdl_wait();
+    pdl_launch_dependents();
+  };
+
+  const TileItem* tiles = a.tiles + __ldg(a.list_first + blockIdx.x);
+  const int n_items = __ldg(a.list_first + blockIdx.x + 1) - __ldg(a.list_first + blockIdx.x);
 
   bool dead = false;
   auto WAIT = [&](uint32_t bar, uint32_t parity) {
@@ -209,25 +213,31 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // The entries of the ring for an item of n key tiles, in the order the products use them: K of the first `lead` tiles,
       // then V0 K(lead) V1 K(lead + 1) ..., and the last V.
       uint32_t e = 0;
+      bool first = true;
+      if (lane == 0) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&vmap) : "memory");
+      }
       const int box_rows = 1 << a.box_log2, boxes = kTileKeys >> a.box_log2;
-      for (int r = 0; !dead; ++r) {
-        const int w = work_at(r, a.n_work);
-        if (w < 0) break;
-        const TileItem it = load_tile(a.tiles + w / a.kv_heads);
-        const int kvh = w % a.kv_heads, n = (it.kv_len + kTileKeys - 1) / kTileKeys, end = it.kv_begin + it.kv_len;
-        const int* tbl = a.block_tables + __ldg(a.table_offset + __ldg(a.token_seq + __ldg(&a.rows[it.tok0].token)));
-        const int lead = min(n, S::kLead << it.halves), turns = 2 * (n - lead);
+      for (int r = 0; r < n_items && !dead; ++r) {
+        const TileItem it = load_tile(tiles + r);
+        const int pair = it.flags & kPair ? 1 : 0, n = (it.kv_len + kTileKeys - 1) / kTileKeys << pair, end = it.kv_begin + it.kv_len;
+        const int* tbl = a.block_tables + __ldg(a.table_offset + (it.source < 0 ? ~it.source : __ldg(a.token_seq + it.source)));
+        const int lead = min(n, S::kLead << pair), turns = 2 * (n - lead);
         auto is_v = [&](int i) { return i >= lead && !(i - lead < turns && ((i - lead) & 1)); };
         auto tile_of = [&](int i) { return i < lead ? i : i - lead >= turns ? i - n : ((i - lead) & 1) ? lead + ((i - lead) >> 1) : (i - lead) >> 1; };
         auto row_of = [&](int i) {           // pool row of this lane's box
-          const int pos = it.kv_begin + tile_of(i) * kTileKeys + (lane << a.box_log2);
+          const int pos = it.kv_begin + (tile_of(i) >> pair) * kTileKeys + (lane << a.box_log2);
           if (lane >= boxes || pos >= end) return 0;
           return (__ldg(tbl + (pos >> a.bs_log2)) << a.bs_log2) + (pos & (a.block_size - 1));
         };
         int y = row_of(0);
+        if (first) after_previous();
+        first = false;
         for (int i = 0; i < 2 * n; ++i, ++e) {
           const int y_next = i + 1 < 2 * n ? row_of(i + 1) : 0;
-          const int st = static_cast<int>(e % NS), left = it.kv_len - tile_of(i) * kTileKeys;
+          const int t = tile_of(i), st = static_cast<int>(e % NS), left = it.kv_len - (t >> pair) * kTileKeys;
+          const int x = (it.kvh + (t & pair)) * D;
           const int valid = min(boxes, (left + box_rows - 1) >> a.box_log2);
           if (lane == 0) {
             WAIT(BAR(KV_EMPTY + st), ((e / NS) & 1) ^ 1);
@@ -239,7 +249,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const uint32_t dst = ring + st * S::kTile + (lane << a.box_log2) * 128;
             const CUtensorMap* map = is_v(i) ? &vmap : &kmap;
 #pragma unroll
-            for (int h = 0; h < S::kHalves; ++h) tma_load_2d(dst + h * kBlockBytes, map, kvh * D + h * 64, y, BAR(KV_FULL + st));
+            for (int h = 0; h < S::kHalves; ++h) tma_load_2d(dst + h * kBlockBytes, map, x + h * 64, y, BAR(KV_FULL + st));
           }
           __syncwarp();
           y = y_next;
@@ -252,25 +262,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       __syncwarp();
     } else if (warp == kRowsLoader) {
       int r = 0;
-      for (; !dead; ++r) {
-        const int w = work_at(r, a.n_work);
-        if (w < 0) break;
-        const TileItem it = load_tile(a.tiles + w / a.kv_heads);
-        const int kvh = w % a.kv_heads, qb = r % S::kQBufs;
+      if (lane == 0) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&qmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&qmap_many) : "memory");
+      }
+      for (; r < n_items && !dead; ++r) {
+        const TileItem it = load_tile(tiles + r);
+        const int heads = it.flags & kPair ? 2 : 1, qb = r % S::kQBufs;
         const uint32_t bar = BAR(Q_FULL + qb), dst = base + qb * S::kQ;
         const int many = (it.flags & kConsecutive) ? it.n_tok / a.box_tokens : 0, boxes = many + it.n_tok - many * a.box_tokens;
+        int token = 0;
+        auto first_of = [&](int b) { return b < many ? b * a.box_tokens : b + many * (a.box_tokens - 1); };   // first token of a box
+        if (lane < boxes) token = __ldg(a.row_token + it.tok0 + first_of(lane));
+        if (r == 0) after_previous();
         if (lane == 0) {
           WAIT(BAR(Q_EMPTY + qb), ((r / S::kQBufs) & 1) ^ 1);
-          if (!dead) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(it.n_tok * a.group) * 128u * S::kHalves);
+          if (!dead) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(heads * it.n_tok * a.group) * 128u * S::kHalves);
         }
         dead = __shfl_sync(0xffffffffu, dead ? 1 : 0, 0) != 0;
         if (dead) break;
         for (int b = lane; b < boxes; b += 32) {
-          const int first = b < many ? b * a.box_tokens : b + many * (a.box_tokens - 1);   // its first token
-          const int token = __ldg(&a.rows[it.tok0 + first].token);
-          const uint32_t to = dst + first * a.group * 128;
+          if (b >= 32) token = __ldg(a.row_token + it.tok0 + first_of(b));
+          const uint32_t to = dst + first_of(b) * a.group * 128;
+          for (int i = 0; i < heads; ++i)
 #pragma unroll
-          for (int h = 0; h < S::kHalves; ++h) tma_load_3d(to + h * S::kQHalf, b < many ? &qmap_many : &qmap, h * 64, kvh * a.group, token, bar);
+            for (int h = 0; h < S::kHalves; ++h)
+              tma_load_3d(to + i * kBlockBytes + h * S::kQHalf, b < many ? &qmap_many : &qmap, h * 64, (it.kvh + i) * a.group, token, bar);
         }
         __syncwarp();
       }
@@ -279,13 +296,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       __syncwarp();
     } else if (warp == kIssuer) {
+      after_previous();
       if (lane == 0) {
         uint32_t e = 0, done = 0, read = 0;                        // ring entries; bit g: parity of group g's P and S taken
-        for (int r = 0; !dead; ++r) {
-          const int w = work_at(r, a.n_work);
-          if (w < 0) break;
-          const TileItem it = load_tile(a.tiles + w / a.kv_heads);
-          const int n = (it.kv_len + kTileKeys - 1) / kTileKeys, last = it.n_tok * a.group > 128 ? 1 : 0, qb = r % S::kQBufs;   // last group; buffer of Q
+        for (int r = 0; r < n_items && !dead; ++r) {
+          const TileItem it = load_tile(tiles + r);
+          const int pair = it.flags & kPair ? 1 : 0, n = (it.kv_len + kTileKeys - 1) / kTileKeys << pair;
+          const int last = it.n_tok * a.group > 128 ? 1 : 0, qb = r % S::kQBufs;   // last group, if both take every tile; buffer of Q
           // waits for the ring entry and returns where it lies
           auto full = [&](uint32_t entry) {
             WAIT(BAR(KV_FULL + entry % NS), (entry / NS) & 1);
@@ -303,7 +320,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               // counted by tiles: the phase of an item's last tile, which nobody waits for, is over when its P is there
               if (read_first) read ^= 1u << g;
             }
-            uint32_t q_lo = (base + qb * S::kQ + (it.halves ? 0 : g) * kBlockBytes) >> 4, k_lo = k_addr >> 4;
+            uint32_t q_lo = (base + qb * S::kQ + g * kBlockBytes) >> 4, k_lo = k_addr >> 4;
             const uint32_t d = tmem + g * kGroupCols;
             asm volatile("" : "+r"(q_lo), "+r"(k_lo));
 #pragma unroll
@@ -332,10 +349,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           auto free_entry = [&](uint32_t entry) { tc::commit(BAR(KV_EMPTY + entry % NS)); };
           WAIT(BAR(Q_FULL + qb), (r / S::kQBufs) & 1);
           tc::fence_after();
-          const int lead = min(n, S::kLead << it.halves);
+          const int lead = min(n, S::kLead << pair);
           for (int t = 0; t < lead; ++t, ++e) {
             const uint32_t k_addr = full(e);
-            if (it.halves) {
+            if (pair) {
               scores(t & 1, k_addr, t >= 2);
             } else {
               for (int g = 0; g <= last; ++g) scores(g, k_addr, t >= 1);
@@ -348,9 +365,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const bool more = kt < n;
             const uint32_t v_addr = full(e);
             uint32_t k_addr = 0;
-            const int g0 = it.halves ? t & 1 : 0, g1 = it.halves ? t & 1 : last;
+            const int g0 = pair ? t & 1 : 0, g1 = pair ? t & 1 : last;
             for (int g = g0; g <= g1; ++g) {
-              values(g, v_addr, t < 1 + it.halves, t + 1 + it.halves >= n);
+              values(g, v_addr, t <= pair, t + 1 + pair >= n);
               if (g == g1) free_entry(e);
               if (!more) continue;
               if (g == g0) k_addr = full(e + 1);
@@ -365,47 +382,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
       __syncwarp();
+    } else {
+      after_previous();
     }
   } else {
+    after_previous();
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
     // ---- softmax: thread = row of its group = lane of tensor memory ----
     const int g = warp >> 2, r_in = threadIdx.x & 127;
     const uint32_t t_s = tmem + g * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16), t_o = t_s + kColO, t_p = t_s + S::kColP;
     const float sl2 = a.scale * kLog2e;
     uint32_t e0 = 0, done = 0, finished = 0;                     // ring entries before this item; the group's key tiles; its commits to O_FULL awaited
-    for (int r = 0; !dead; ++r) {
-      const int w = work_at(r, a.n_work);
-      if (w < 0) break;
-      const TileItem it = load_tile(a.tiles + w / a.kv_heads);
-      const int kvh = w % a.kv_heads, n = (it.kv_len + kTileKeys - 1) / kTileKeys;
-      const uint32_t last_v = e0 + 2 * n - 1;                    // ring entry of the last V tile
+    for (int r = 0; r < n_items && !dead; ++r) {
+      const TileItem it = load_tile(tiles + r);
+      const int pair = it.flags & kPair ? 1 : 0, n = (it.kv_len + kTileKeys - 1) / kTileKeys << pair;
       e0 += 2 * n;
-      const int row = it.halves ? r_in : g * 128 + r_in;         // row of the item
-      const int rows = it.n_tok * a.group;
+      const uint32_t last_v = e0 - 1 - pair + (pair & g);        // ring entry of the group's last V tile
+      const int rows = it.n_tok * a.group, row = pair ? r_in : g * 128 + r_in;   // row of the item
+      if (g == 1 && !pair && rows <= 128) continue;
       const bool mine = row < rows;
-      RowToken rt{0, 0};
-      int head = 0;
+      int token = 0, head = 0;
       if (mine) {
         const int t = row / a.group;
-        const int2 x = __ldg(reinterpret_cast<const int2*>(a.rows + it.tok0 + t));
-        rt = RowToken{x.x, x.y};
-        head = kvh * a.group + (row - t * a.group);
-      }
-      if (g == 1 && !it.halves && rows <= 128) {
-        if ((it.flags & kEmptySecond) && r_in < rows) {          // the others of the segment leave two partials
-          const int t = r_in / a.group;
-          const size_t p = static_cast<size_t>(__ldg(&a.rows[it.tok0 + t].part_base) + it.part + 1) * a.q_heads + kvh * a.group + (r_in - t * a.group);
-          *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(-INFINITY, 0.f);
-        }
-        continue;
+        token = __ldg(a.row_token + it.tok0 + t);
+        head = (it.kvh + (pair & g)) * a.group + (row - t * a.group);
       }
       const bool working = (row & ~31) < rows;                // some row of this warp is the item's
-      float m_used = -INFINITY, l0 = 0.f, l1 = 0.f;
-      const int step = it.halves ? 2 : 1;
+      float m_used = -INFINITY;
+      float2 l = both(0.f);
+      const int step = 1 + pair;
       // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring held.  Cleared
       // before the group's threads report the tile's P, so that 0 * x stays 0.
       auto clear_tail = [&](int t, int valid) {
-        if (t < n - 1 || valid >= kTileKeys || (g == 1 && !it.halves)) return;
+        if (t + step < n || valid >= kTileKeys || (g == 1 && !pair)) return;
         WAIT(BAR(KV_FULL + last_v % NS), (last_v / NS) & 1);
         if (r_in >= valid) {
 #pragma unroll
@@ -417,10 +426,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       };
-      for (int t = it.halves ? g : 0; t < n; t += step, ++done) {
+      for (int t = pair & g; t < n; t += step, ++done) {
         WAIT(BAR(S_FULL + g), done & 1);
         tc::fence_after();
-        const int valid = it.kv_len - t * kTileKeys;             // keys of this tile, if fewer than kTileKeys
+        const int valid = it.kv_len - (t >> pair) * kTileKeys;             // keys of this tile, if fewer than kTileKeys
         if (working) {
           float sc[kTileKeys];
 #pragma unroll
@@ -436,67 +445,86 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (int i = 0; i < kTileKeys; ++i)
               if (i >= valid) sc[i] = -INFINITY;
           }
-          float mx8[8];
+          auto row_max = [&]() {
+            float mx8[8];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) mx8[u] = fmaxf(sc[u], sc[8 + u]);
+            for (int u = 0; u < 8; ++u) mx8[u] = fmaxf(sc[u], sc[8 + u]);
 #pragma unroll
-          for (int i = 16; i < kTileKeys; i += 16)
+            for (int i = 16; i < kTileKeys; i += 16)
 #pragma unroll
-            for (int u = 0; u < 8; ++u) mx8[u] = max3(mx8[u], sc[i + u], sc[i + 8 + u]);
-          const float mx = fmaxf(max3(mx8[0], mx8[1], mx8[2]), fmaxf(max3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-          if (t < step) {
-            m_used = mx;
-          } else if (__any_sync(0xffffffffu, (mx - m_used) * sl2 > kRescale)) {
-            // The group's product before this one is complete: where nothing is waited for, its next scores, which have arrived,
-            // were issued behind it.
-            if constexpr (S::kLead > 1) {
-              WAIT(BAR(O_FULL + g), finished & 1);
-              tc::fence_after();
+              for (int u = 0; u < 8; ++u) mx8[u] = max3(mx8[u], sc[i + u], sc[i + 8 + u]);
+            return fmaxf(max3(mx8[0], mx8[1], mx8[2]), fmaxf(max3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+          };
+          // P of 64 keys, packed, and its sum.
+          auto weights = [&](int c0, uint32_t (&pk)[32]) {
+            const float2 neg = both(-m_used * sl2), by = both(sl2);
+            float2 sum[2] = {both(0.f), both(0.f)};
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float2 x = fma2(make_float2(sc[c0 + 2 * i], sc[c0 + 2 * i + 1]), by, neg);
+              x = make_float2(ex2(x.x), ex2(x.y));
+              sum[i & 1] = add2(sum[i & 1], x);
+              pk[i] = pack2<T>(x.x, x.y);
             }
-            const float m_new = (mx - m_used) * sl2 > kRescale ? mx : m_used;
-            const float f = ex2((m_used - m_new) * sl2);
-            m_used = m_new;
-            l0 *= f;
-            l1 *= f;
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t v[32];
-              tc::ld32(t_o + c, v);
-              tc::wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-              tc::st32(t_o + c, v);
-            }
+            return add2(sum[0], sum[1]);
+          };
+          // The first half is worked out with the maximum in use while this tile's is still being looked for: it is
+          // hardly ever too small.
+          uint32_t pk[32];
+          float2 half = both(0.f);
+          const bool opening = t < step;
+          float mx;
+          if (!opening) {
+            half = weights(0, pk);
+            mx = row_max();
+          } else {
+            mx = row_max();
           }
-          const float neg = -m_used * sl2;
+          if (opening || __any_sync(0xffffffffu, (mx - m_used) * sl2 > kRescale)) {
+            if (opening) {
+              m_used = mx;
+            } else {
+              // The group's product before this one is complete: where nothing is waited for, its next scores, which have arrived,
+              // were issued behind it.
+              if constexpr (S::kLead > 1) {
+                WAIT(BAR(O_FULL + g), finished & 1);
+                tc::fence_after();
+              }
+              const float m_new = (mx - m_used) * sl2 > kRescale ? mx : m_used;
+              const float f = ex2((m_used - m_new) * sl2);
+              m_used = m_new;
+              l.x *= f;
+              l.y *= f;
+#pragma unroll 1
+              for (int c = 0; c < D; c += 32) {
+                uint32_t v[32];
+                tc::ld32(t_o + c, v);
+                tc::wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                tc::st32(t_o + c, v);
+              }
+            }
+            half = weights(0, pk);
+          }
+          l = add2(l, half);
           if constexpr (S::kLead > 1) {                          // P of the tile before has been read
-            if (t >= step) {
+            if (!opening) {
               WAIT(BAR(O_FULL + g), finished & 1);
               ++finished;
               tc::fence_after();
             }
           }
-#pragma unroll
-          for (int c = 0; c < kTileKeys; c += 32) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float x0, x1;
-              fma2(sc[c + 2 * i], sc[c + 2 * i + 1], sl2, neg, x0, x1);
-              x0 = ex2(x0);
-              x1 = ex2(x1);
-              add2(l0, l1, x0, x1);
-              pk[i] = pack2<T>(x0, x1);
-            }
-            tc::st16(t_p + c / 2, pk);
-            if (S::kLead == 1 && c == 32) {
-              clear_tail(t, valid);
-              tc::wait_st();
-              tc::fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_warp(BAR(P_HALF + g));
-            }
+          tc::st32(t_p, pk);
+          if constexpr (S::kLead == 1) {
+            clear_tail(t, valid);
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_warp(BAR(P_HALF + g));
           }
+          l = add2(l, weights(64, pk));
+          tc::st32(t_p + 32, pk);
           if (S::kLead > 1) clear_tail(t, valid);
           tc::wait_st();
           tc::fence_before();
@@ -526,16 +554,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (!working) continue;
       // A thread holds a row; stored as it is, every instruction would touch 32 rows, 16 bytes each (an item's output then took
       // 20,000 cycles, the next one's Q behind it).  Eight lanes exchange their pieces instead and store whole lines.
-      const float l = l0 + l1;
+      const float sum = l.x + l.y;
       const bool partial = it.part >= 0;
-      const size_t p = static_cast<size_t>(rt.part_base + it.part + (it.halves ? g : 0)) * a.q_heads + head;
+      const size_t p = static_cast<size_t>(it.part + (pair & g) * rows + row);
       unsigned long long to = 0;
       if (mine) {
         to = partial ? reinterpret_cast<unsigned long long>(a.part_acc + p * D)
-                     : reinterpret_cast<unsigned long long>(static_cast<T*>(a.out) + (static_cast<size_t>(rt.token) * a.q_heads + head) * D);
-        if (partial) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_used * a.ml_scale, l);
+                     : reinterpret_cast<unsigned long long>(static_cast<T*>(a.out) + (static_cast<size_t>(token) * a.q_heads + head) * D);
+        if (partial) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_used * a.ml_scale, sum);
       }
-      const float inv = 1.f / l;
+      const float inv = 1.f / sum;
       auto store_line = [&](uint32_t (&x)[32], int at) {       // 128 bytes of every lane's row, at byte `at` of the row
         transpose8(x, lane);
 #pragma unroll
@@ -575,32 +603,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
-// Folds each listed token's partials: thread = (row of the list, head, VEC dims).  Partials sit in L2; a batch of loads is in
-// flight before the first is used.
+// Folds the partials of each listed (token, kv head): thread = (record, head of the group, VEC dims).  Partials sit in L2; a
+// batch of loads is in flight before the first is used.
 constexpr int kMergeThreads = 256, kMergeBatch = 8;
 struct MergeArgs {
   const MergeRow* rows;
-  int n_rows, q_heads, head_dim;
-  const float *part_ml, *part_acc;
+  int n_rows, q_heads, group, head_dim;
+  const float *tile_ml, *tile_acc, *own_ml, *own_acc;
   void* out;
 };
 template <typename T, bool LOG2, int VEC>
 __global__ void __launch_bounds__(kMergeThreads) segment_merge_kernel(const MergeArgs a) {
   pdl_launch_dependents();
-  const int per_head = a.head_dim / VEC;
-  const long long per_row = static_cast<long long>(a.q_heads) * per_head, i = blockIdx.x * static_cast<long long>(kMergeThreads) + threadIdx.x;
-  const long long row = i / per_row;
+  const int per_head = a.head_dim / VEC, per_row = a.group * per_head;
+  const long long i = blockIdx.x * static_cast<long long>(kMergeThreads) + threadIdx.x, row = i / per_row;
   const bool live = row < a.n_rows;
-  int4 m = make_int4(0, 0, 0, 0);
-  if (live) m = __ldg(reinterpret_cast<const int4*>(a.rows) + row);      // part of the plan, complete before the kernels that wrote the partials began
+  MergeRow m{};
+  if (live) {                                            // part of the plan, complete before the kernels that wrote the partials began
+    const int4 x = __ldg(reinterpret_cast<const int4*>(a.rows + row)), y = __ldg(reinterpret_cast<const int4*>(a.rows + row) + 1);
+    m = MergeRow{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  }
   pdl_wait();
   if (!live) return;
-  const int at = static_cast<int>(i - row * per_row), head = at / per_head, d = (at - head * per_head) * VEC;
-  const MergeRow mr{m.x, m.y, m.z, m.w};
+  const int at = static_cast<int>(i - row * per_row), h = at / per_head, d = (at - h * per_head) * VEC, head = m.kvh * a.group + h;
+  const int n = m.n_tile + m.n_own;
   float run = -INFINITY, sum = 0.f, acc[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
-  for (int p0 = 0; p0 < mr.n_parts; p0 += kMergeBatch) {
+  for (int p0 = 0; p0 < n; p0 += kMergeBatch) {
     float2 ml[kMergeBatch];
     float x[kMergeBatch][VEC];
 #pragma unroll
@@ -608,14 +638,18 @@ __global__ void __launch_bounds__(kMergeThreads) segment_merge_kernel(const Merg
       ml[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) x[u][v] = 0.f;
-      if (p0 + u < mr.n_parts) {
-        const size_t p = static_cast<size_t>(mr.part_base + p0 + u) * a.q_heads + head;
-        ml[u] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + p);
+      const int p = p0 + u;
+      if (p < n) {
+        const bool tile = p < m.n_tile;
+        const size_t r = tile ? static_cast<size_t>(m.tile_row) + h + static_cast<size_t>(p) * m.tile_stride
+                              : static_cast<size_t>(m.own_part + p - m.n_tile) * a.q_heads + head;
+        ml[u] = __ldcg(reinterpret_cast<const float2*>(tile ? a.tile_ml : a.own_ml) + r);
+        const float* src = (tile ? a.tile_acc : a.own_acc) + r * a.head_dim + d;
         if constexpr (VEC == 4) {
-          const float4 f = __ldcg(reinterpret_cast<const float4*>(a.part_acc + p * a.head_dim + d));
+          const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
           x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
         } else {
-          x[u][0] = __ldcg(a.part_acc + p * a.head_dim + d);
+          x[u][0] = __ldcg(src);
         }
       }
     }
@@ -632,12 +666,12 @@ __global__ void __launch_bounds__(kMergeThreads) segment_merge_kernel(const Merg
       const float f = weight(ml[u].x);
       sum += f * ml[u].y;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) acc[v] += ml[u].x == -INFINITY ? 0.f : f * x[u][v];   // an empty partial's accumulator is not written
+      for (int v = 0; v < VEC; ++v) acc[v] += f * x[u][v];
     }
     run = top;
   }
-  const float inv = mr.n_parts > 0 ? 1.f / sum : 0.f;
-  T* o = static_cast<T*>(a.out) + (static_cast<size_t>(mr.token) * a.q_heads + head) * a.head_dim + d;
+  const float inv = n > 0 ? 1.f / sum : 0.f;
+  T* o = static_cast<T*>(a.out) + (static_cast<size_t>(m.token) * a.q_heads + head) * a.head_dim + d;
   if constexpr (VEC == 4 && sizeof(T) == 2) {
     *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
   } else if constexpr (VEC == 4) {
@@ -660,7 +694,7 @@ int make_q_map(CUtensorMap* map, const void* q, PoolElem elem, int head_dim, int
 }
 
 template <typename T, int D>
-int launch_tiles(const TileArgs& a, const void* q, int n_tokens, const void* k_cache, const void* v_cache, uint64_t pool_rows, cudaStream_t stream) {
+int launch_tiles(const TileArgs& a, int blocks, int kv_heads, const void* q, int n_tokens, const void* k_cache, const void* v_cache, uint64_t pool_rows, cudaStream_t stream) {
   using S = TileSmem<D>;
   auto kern = tile_attn_kernel<T, D>;
   static thread_local int configured_device = -1;
@@ -675,10 +709,10 @@ int launch_tiles(const TileArgs& a, const void* q, int n_tokens, const void* k_c
   alignas(64) CUtensorMap qmap, qmap_many, kmap, vmap;
   int st = make_q_map(&qmap, q, elem, D, a.q_heads, n_tokens, a.group, 1);
   if (st == PKV_OK) st = make_q_map(&qmap_many, q, elem, D, a.q_heads, n_tokens, a.group, a.box_tokens);
-  if (st == PKV_OK) st = make_pool_tensor_map(&kmap, k_cache, elem, a.kv_heads * D, 1u << a.box_log2, pool_rows);
-  if (st == PKV_OK) st = make_pool_tensor_map(&vmap, v_cache, elem, a.kv_heads * D, 1u << a.box_log2, pool_rows);
+  if (st == PKV_OK) st = make_pool_tensor_map(&kmap, k_cache, elem, kv_heads * D, 1u << a.box_log2, pool_rows);
+  if (st == PKV_OK) st = make_pool_tensor_map(&vmap, v_cache, elem, kv_heads * D, 1u << a.box_log2, pool_rows);
   if (st != PKV_OK) return st;
-  launch_pdl(kern, dim3(static_cast<unsigned>(std::min(a.n_work, decode_sms()))), dim3(kTileThreads), S::kBytes, stream, a, qmap, qmap_many, kmap, vmap);
+  launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(kTileThreads), S::kBytes, stream, a, qmap, qmap_many, kmap, vmap);
   return check_launch("tile_attn_kernel");
 }
 
@@ -688,28 +722,37 @@ int log2_floor(int x) {
   return l;
 }
 
-struct SegmentOffsets { size_t seq, pos, rows, items, tiles, merge, image, ml, acc, total; };
-SegmentOffsets segment_offsets(const SegmentGeometry& g, size_t rows, size_t items, size_t first, size_t tiles, size_t merge, size_t parts) {
+struct SegmentOffsets { size_t seq, pos, rows, items, lists, tiles, merge, image, tile_ml, tile_acc, ml, acc, total; };
+struct SegmentCounts { size_t rows, items, shares, lists, tiles, merge, tile_rows, parts; };   // shares, lists: with the end
+SegmentOffsets segment_offsets(const SegmentGeometry& g, const SegmentCounts& c) {
   SegmentOffsets o;
   size_t at = align256(sizeof(PlanHeader));
-  o.seq = at;   at = align256(at + sizeof(int) * static_cast<size_t>(g.n_tokens));
-  o.pos = at;   at = align256(at + sizeof(int) * static_cast<size_t>(g.n_tokens));
-  o.rows = at;  at = align256(at + sizeof(RowToken) * rows);
-  o.items = at; at = align256(at + sizeof(WorkItem) * items + sizeof(int) * first);
-  o.tiles = at; at = align256(at + sizeof(TileItem) * tiles);
-  o.merge = at; at = align256(at + sizeof(MergeRow) * merge);
+  auto region = [&](size_t bytes) {
+    const size_t here = at;
+    at = align256(at + bytes);
+    return here;
+  };
+  o.seq = region(sizeof(int) * g.n_tokens);
+  o.pos = region(sizeof(int) * g.n_tokens);
+  o.rows = region(sizeof(int) * c.rows);
+  o.items = region(sizeof(WorkItem) * c.items + sizeof(int) * c.shares);
+  o.lists = region(sizeof(int) * c.lists);
+  o.tiles = region(sizeof(TileItem) * c.tiles);
+  o.merge = region(sizeof(MergeRow) * c.merge);
   o.image = at;
-  o.ml = at;    at = align256(at + sizeof(float) * 2 * parts * g.q_heads);
-  o.acc = at;   at = align256(at + sizeof(float) * parts * g.q_heads * g.head_dim);
+  o.tile_ml = region(sizeof(float) * 2 * c.tile_rows);
+  o.tile_acc = region(sizeof(float) * c.tile_rows * g.head_dim);
+  o.ml = region(sizeof(float) * 2 * c.parts * g.q_heads);
+  o.acc = region(sizeof(float) * c.parts * g.q_heads * g.head_dim);
   o.total = at;
   return o;
 }
-// For any step of these sizes: tiles of uncut segments, and one more item at most for every partial.
+// For any step of these sizes: a tile has a token at least, and every block cuts one at most.
 SegmentOffsets segment_bounds(const SegmentGeometry& g, bool prefix) {
-  const size_t n = static_cast<size_t>(g.n_tokens), slots = static_cast<size_t>(tile_slots(g, decode_sms())) + (prefix ? n : 0);
-  const size_t tiles = n + slots;                            // (an uncut tile has a token at least)
+  const size_t n = static_cast<size_t>(g.n_tokens), sms = static_cast<size_t>(decode_sms());
   const size_t items = n + own_extra(g) + 2;
-  return segment_offsets(g, n, items, items + 1, tiles, n, static_cast<size_t>(most_parts(g, decode_sms(), prefix)));
+  return segment_offsets(g, SegmentCounts{n, items, items + 1, sms + 1, n * g.kv_heads + 2 * sms, n * g.kv_heads,
+                                          static_cast<size_t>(most_tile_rows(g, decode_sms(), prefix)), static_cast<size_t>(most_parts(g, prefix))});
 }
 
 int check_geometry(const char* fn, const SegmentGeometry& g) {
@@ -726,11 +769,12 @@ enum Kind { kCross = 1, kPrefix = 2 };
 
 int write_image(const char* fn, Kind kind, const SegmentGeometry& g, const SegmentLists& l, const std::vector<int>& seq, const std::vector<int>& pos,
                 bool cluster, void* h_staging, size_t staging_bytes, size_t workspace_bytes, pkv_segment_plan* plan) {
-  const SegmentOffsets o = segment_offsets(g, l.rows.size(), l.items.size(), l.first.size(), l.tiles.size(), l.merge.size(), static_cast<size_t>(l.n_parts));
+  const SegmentOffsets o = segment_offsets(g, SegmentCounts{l.row_token.size(), l.items.size(), l.first.size(), l.list_first.size(), l.tiles.size(),
+                                                            l.merge.size(), static_cast<size_t>(l.n_tile_rows), static_cast<size_t>(l.n_parts)});
   if (o.total > workspace_bytes) return fail(PKV_E_WORKSPACE, "%s: workspace of %zu bytes; this step takes %zu", fn, workspace_bytes, o.total);
   if (o.image > staging_bytes) return fail(PKV_E_WORKSPACE, "%s: staging buffer of %zu bytes; this step's plan takes %zu", fn, staging_bytes, o.image);
-  if (static_cast<long long>(l.tiles.size()) * g.kv_heads > 0x7fffffffll || static_cast<long long>(l.items.size()) * g.kv_heads > 0x7fffffffll)
-    return fail(PKV_E_UNSUPPORTED, "%s: more than 2^31 - 1 work items", fn);
+  if (l.n_tile_rows > 0x7fffffffll || static_cast<long long>(l.items.size()) * g.kv_heads > 0x7fffffffll)
+    return fail(PKV_E_UNSUPPORTED, "%s: more than 2^31 - 1 work items or partial rows", fn);
   char* img = static_cast<char*>(h_staging);
   std::memset(img, 0, o.seq);
   PlanHeader* hd = reinterpret_cast<PlanHeader*>(img);
@@ -744,9 +788,10 @@ int write_image(const char* fn, Kind kind, const SegmentGeometry& g, const Segme
   auto put = [&](size_t at, const void* p, size_t bytes) { if (bytes) std::memcpy(img + at, p, bytes); };
   put(o.seq, seq.data(), seq.size() * sizeof(int));
   put(o.pos, pos.data(), pos.size() * sizeof(int));
-  put(o.rows, l.rows.data(), l.rows.size() * sizeof(RowToken));
+  put(o.rows, l.row_token.data(), l.row_token.size() * sizeof(int));
   put(o.items, l.items.data(), l.items.size() * sizeof(WorkItem));
   put(o.items + l.items.size() * sizeof(WorkItem), l.first.data(), l.first.size() * sizeof(int));
+  put(o.lists, l.list_first.data(), l.list_first.size() * sizeof(int));
   put(o.tiles, l.tiles.data(), l.tiles.size() * sizeof(TileItem));
   put(o.merge, l.merge.data(), l.merge.size() * sizeof(MergeRow));
   std::memset(plan, 0, sizeof(*plan));
@@ -757,10 +802,13 @@ int write_image(const char* fn, Kind kind, const SegmentGeometry& g, const Segme
   plan->n_items = static_cast<int>(l.items.size());
   plan->n_merged = static_cast<int>(l.merge.size());
   plan->n_parts = l.n_parts;
+  plan->n_lists = l.list_first.empty() ? 0 : static_cast<int>(l.list_first.size()) - 1;
+  plan->n_tile_rows = static_cast<int>(l.n_tile_rows);
   plan->image_bytes = o.image;
   plan->workspace_bytes = o.total;
   plan->off_seq = o.seq; plan->off_pos = o.pos; plan->off_rows = o.rows; plan->off_items = o.items;
-  plan->off_tiles = o.tiles; plan->off_merge = o.merge; plan->off_ml = o.ml; plan->off_acc = o.acc;
+  plan->off_lists = o.lists; plan->off_tiles = o.tiles; plan->off_merge = o.merge;
+  plan->off_tile_ml = o.tile_ml; plan->off_tile_acc = o.tile_acc; plan->off_ml = o.ml; plan->off_acc = o.acc;
   if (cluster && l.n_parts > 0) plan->cluster = decode_cluster_size(g.n_tokens, l.longest, g.q_heads, g.kv_heads, g.head_dim, &plan->cluster_least);
   return PKV_OK;
 }
@@ -786,14 +834,14 @@ int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* 
     next = start + q_len[s];
     listed += q_len[s];
     const bool tiled = kv_len[s] > 0 && g.tiles() && q_len[s] >= kMinTileTokens;
-    if (tiled) segs.push_back(Segment{static_cast<int>(l.rows.size()), q_len[s], kv_len[s], 1, 0});
+    if (tiled) segs.push_back(Segment{static_cast<int>(l.row_token.size()), q_len[s], kv_len[s], ~s});
     for (int i = 0; i < q_len[s]; ++i) {
       const int t = static_cast<int>(start) + i;
       if (seq[t] >= 0) return fail(PKV_E_ARG, "%s: row %d belongs to sequences %d and %d", fn, t, seq[t], s);
       seq[t] = s;
       pos[t] = kv_len[s] - 1;
       if (kv_len[s] == 0) empty.push_back(t);
-      else if (tiled) l.rows.push_back(RowToken{t, 0});
+      else if (tiled) l.row_token.push_back(t);
       else own.push_back(OwnRange{t, 0, kv_len[s]});
     }
   }
@@ -818,15 +866,15 @@ int plan_prefix(const char* fn, const int* token_pos, int prefix_len, const Segm
   SegmentLists l;
   for (int t = 0; t < g.n_tokens; ++t) {
     if (token_pos[t] < 0 || token_pos[t] == 0x7fffffff) return fail(PKV_E_ARG, "%s: token %d has position %d", fn, t, token_pos[t]);
-    if (shared > 0 && token_pos[t] >= shared - 1) l.rows.push_back(RowToken{t, 0});
+    if (shared > 0 && token_pos[t] >= shared - 1) l.row_token.push_back(t);
   }
-  const bool together = static_cast<int>(l.rows.size()) >= kMinPrefixTokens;
-  if (!together) l.rows.clear();
+  const bool together = static_cast<int>(l.row_token.size()) >= kMinPrefixTokens;
+  if (!together) l.row_token.clear();
   for (int t = 0; t < g.n_tokens; ++t) {
     const int begin = together && token_pos[t] >= shared - 1 ? shared : 0, len = token_pos[t] + 1 - begin;
     if (len > 0) own.push_back(OwnRange{t, begin, len});
   }
-  if (together) segs.push_back(Segment{0, static_cast<int>(l.rows.size()), shared, 1, 0});
+  if (together) segs.push_back(Segment{0, static_cast<int>(l.row_token.size()), shared, l.row_token[0]});
   list_segments(segs, own, empty, g, decode_sms(), true, l);
   return write_image(fn, kPrefix, g, l, none, pos, segs.empty(), h_staging, staging_bytes, workspace_bytes, plan);
 }
@@ -861,24 +909,25 @@ int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const v
   const bool log2_domain = decode_log2_domain<T>(plan->q_heads, plan->kv_heads, D, plan->block_size, scale);
   const int* seq = kind == kCross ? reinterpret_cast<const int*>(ws + plan->off_seq) : token_seq;
   float *ml = reinterpret_cast<float*>(ws + plan->off_ml), *acc = reinterpret_cast<float*>(ws + plan->off_acc);
+  float *tile_ml = reinterpret_cast<float*>(ws + plan->off_tile_ml), *tile_acc = reinterpret_cast<float*>(ws + plan->off_tile_acc);
   unsigned int* host_err = error_mirror(true);
   if (plan->n_tiles > 0) {
     if constexpr (sizeof(T) == 2) {
       if (!tensor_map_encoder()) return fail(PKV_E_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", fn);
       TileArgs a;
       a.block_tables = block_tables; a.table_offset = table_offset; a.token_seq = seq;
-      a.rows = reinterpret_cast<const RowToken*>(ws + plan->off_rows);
+      a.row_token = reinterpret_cast<const int*>(ws + plan->off_rows);
+      a.list_first = reinterpret_cast<const int*>(ws + plan->off_lists);
       a.tiles = reinterpret_cast<const TileItem*>(ws + plan->off_tiles);
-      a.out = out; a.part_ml = ml; a.part_acc = acc;
-      a.n_work = plan->n_tiles * plan->kv_heads;
-      a.q_heads = plan->q_heads; a.kv_heads = plan->kv_heads; a.group = group;
+      a.out = out; a.part_ml = tile_ml; a.part_acc = tile_acc;
+      a.q_heads = plan->q_heads; a.group = group;
       a.block_size = plan->block_size; a.bs_log2 = log2_floor(plan->block_size); a.box_log2 = std::min(a.bs_log2, 7);
       a.box_tokens = std::max(1, kBoxRows / group);
       a.scale = scale;
       a.ml_scale = log2_domain ? scale * 1.4426950408889634f : scale;
       a.host_err = host_err;
       const uint64_t rows = pool_rows ? pool_rows : 1ull << 30;
-      st = D == 64 ? launch_tiles<T, 64>(a, q, plan->n_tokens, k_cache, v_cache, rows, s) : launch_tiles<T, 128>(a, q, plan->n_tokens, k_cache, v_cache, rows, s);
+      st = D == 64 ? launch_tiles<T, 64>(a, plan->n_lists, plan->kv_heads, q, plan->n_tokens, k_cache, v_cache, rows, s) : launch_tiles<T, 128>(a, plan->n_lists, plan->kv_heads, q, plan->n_tokens, k_cache, v_cache, rows, s);
       if (st != PKV_OK) return st;
     }
   }
@@ -902,9 +951,9 @@ int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const v
     if (st != PKV_OK || merged) return st;
   }
   if (plan->n_merged > 0) {
-    MergeArgs m{reinterpret_cast<const MergeRow*>(ws + plan->off_merge), plan->n_merged, plan->q_heads, D, ml, acc, out};
+    MergeArgs m{reinterpret_cast<const MergeRow*>(ws + plan->off_merge), plan->n_merged, plan->q_heads, group, D, tile_ml, tile_acc, ml, acc, out};
     const int vec = D % 4 == 0 ? 4 : 1;
-    const long long blocks = (static_cast<long long>(plan->n_merged) * plan->q_heads * (D / vec) + kMergeThreads - 1) / kMergeThreads;
+    const long long blocks = (static_cast<long long>(plan->n_merged) * group * (D / vec) + kMergeThreads - 1) / kMergeThreads;
     if (blocks > 0x7fffffffll) return fail(PKV_E_UNSUPPORTED, "%s: %lld blocks to merge", fn, blocks);
     auto kern = vec == 4 ? (log2_domain ? segment_merge_kernel<T, true, 4> : segment_merge_kernel<T, false, 4>)
                          : (log2_domain ? segment_merge_kernel<T, true, 1> : segment_merge_kernel<T, false, 1>);

@@ -2,7 +2,7 @@
 // of a batch that shares a long prefix.  Host code only.
 //
 // Both are made of two kinds of work:
-//   tiles   up to 256 (token, query head) rows of one kv head against one range of keys that all of them see, on
+//   tiles   up to 256 (token, query head) rows of one kv head, or up to 128 of each of two, against one range of keys that all of them see, on
 //           the tensor cores (the tokens of a sequence against its encoder's states; all the tokens of a batch
 //           against the shared prefix);
 //   items   one token against a range of its own keys, on the decode kernels (sequences with few tokens; each
@@ -10,13 +10,21 @@
 // A token that is worked on in one piece is written by the kernel that does it; of any other every piece leaves a
 // partial (maximum, sum, accumulator), and the merge kernel folds them.
 //
+// Tiles are dealt to blocks here, one list of items for each block of the tile kernel (one per SM): either whole, the
+// longest first to the block with the least to do, or laid end to end and cut into equal shares, whichever ends first.
+//
 // Image in the workspace (every region 256-byte aligned, offsets in pkv_segment_plan):
-//   PlanHeader | token_seq[n_tokens] | token_pos[n_tokens] | RowToken[..] | WorkItem[..] (and the first item of every
-//   share) | TileItem[..] | MergeRow[..]
-// and behind it the partials: float2 (maximum, sum) [part][q_heads], float [part][q_heads][head_dim].
+//   PlanHeader | token_seq[n_tokens] | token_pos[n_tokens] | row_token[..] | WorkItem[..] (and the first item of every
+//   share) | int first tile of every list, and the end | TileItem[..] | MergeRow[..]
+// and behind it the partials.  Of the tiles: float2 (maximum, sum) [row], float [row][head_dim], where an item's rows lie
+// one behind the other; of the decode kernels: float2 [part][q_heads], float [part][q_heads][head_dim].
 #pragma once
 #include <algorithm>
 #include <cstring>
+#include <functional>
+#include <map>
+#include <queue>
+#include <utility>
 #include <vector>
 
 #include "decode_list.hpp"
@@ -28,19 +36,19 @@ namespace pkv {
 constexpr int kTileRows = 256;      // rows of a tile item: two groups of 128
 constexpr int kTileKeys = 128;      // keys per step of the tile kernel
 
-struct RowToken { int token, part_base; };
-// The rows of tokens row_tokens[tok0 ..] of a segment: row r is token r / group, head r % group.
+// Tokens row_token[tok0 .. tok0 + n_tok - 1] of a segment: row r of the item is token r / group, head r % group.
 struct TileItem {
-  int tok0, n_tok;
+  int tok0, n_tok, kvh;
   int kv_begin, kv_len;             // kv_begin a multiple of kTileKeys
-  int part;                         // partial slot behind the token's part_base, or -1: write the output
+  int part;                         // first of its partial rows, or -1: write the output
   int flags;
-  int halves;                       // 1: at most 128 rows; the two groups take every other key tile, partials part and part + 1
-  int pad;
+  int source;                       // whose block table: the sequence of this token, or (< 0) sequence ~source
 };
 constexpr int kConsecutive = 1;     // the tokens are consecutive rows of q
-constexpr int kEmptySecond = 2;     // the others of the segment are halved: leave an empty partial part + 1
-struct MergeRow { int token, part_base, n_parts, pad; };   // n_parts 0: no keys, the output is zero
+constexpr int kPair = 2;            // at most 128 rows, of kv head kvh for one group and kvh + 1 for the other
+// Partials of a token's heads of one kv head: of tiles, n_tile of them, tile_stride rows apart; of the decode kernels, n_own.
+// None at all: there are no keys, the output is zero.
+struct MergeRow { int token, kvh, tile_row, tile_stride, n_tile, own_part, n_own, pad; };
 
 struct SegmentGeometry {
   int n_tokens, q_heads, kv_heads, head_dim, block_size, elem_bytes;
@@ -52,67 +60,104 @@ struct SegmentGeometry {
   }
 };
 
-// A sequence whose tokens (row_tokens[tok0 .. tok0 + n_tok - 1]) all see keys 0 .. kv_len - 1.
-struct Segment {
-  int tok0, n_tok, kv_len;
-  int chunks, slots;                // ranges its keys are cut into; partials each of its tokens gets from them
-};
+// A sequence whose tokens (row_token[tok0 .. tok0 + n_tok - 1]) all see keys 0 .. kv_len - 1.
+struct Segment { int tok0, n_tok, kv_len, source; };   // source: as in its tiles
 // A token of the decode kernels: keys begin .. begin + len - 1, len > 0.
 struct OwnRange { int token, begin, len; };
 
 struct SegmentLists {
-  std::vector<RowToken> rows;
+  std::vector<int> row_token;
   std::vector<WorkItem> items;
   std::vector<int> first;           // of every share, and the end; empty: no shares
+  std::vector<int> list_first;      // tiles of every block
   std::vector<TileItem> tiles;
   std::vector<MergeRow> merge;
+  long long n_tile_rows = 0;
   int n_parts = 0, chunk = 0, longest = 0;
 };
 
-// Partials that tile items may leave in all, beyond one per token: two rounds of tile items on every SM.
-inline long long tile_slots(const SegmentGeometry& g, int sms) {
-  return static_cast<long long>((2 * sms + g.kv_heads - 1) / g.kv_heads) * (g.group() <= kTileRows ? g.tile_tokens() + 2 : 0);
-}
 inline int own_extra(const SegmentGeometry& g) { return decode_max_extra(g.kv_heads); }
-// Most partials of a step: prefix steps leave one of each kind per token even when nothing is cut.
-inline long long most_parts(const SegmentGeometry& g, int sms, bool prefix) {
-  return (prefix ? 2ll * g.n_tokens : 0ll) + tile_slots(g, sms) + 2ll * own_extra(g);
+// Most partials of a step.  A block's list begins and ends with a piece of a tile at most; prefix steps leave one of
+// each kind per token even where nothing is cut.
+inline long long most_tile_rows(const SegmentGeometry& g, int sms, bool prefix) {
+  return 2ll * sms * kTileRows + (prefix ? static_cast<long long>(g.n_tokens) * g.q_heads : 0ll);
+}
+inline long long most_parts(const SegmentGeometry& g, bool prefix) { return (prefix ? g.n_tokens : 0ll) + 2ll * own_extra(g); }
+
+// What a block needs for an item, in cycles (measured on B200, head_dim 64 and 128 alike within a tenth): start and end, and a
+// key tile of two groups, of one alone, of a pair of heads.
+constexpr int kItemCycles = 4500, kTwoGroupCycles = 3500, kOneGroupCycles = 2600, kPairCycles = 3600;
+constexpr int kLeastTiles = 2;      // key tiles of a piece, at least
+// Partials cost a merge launch, and their way to L2 and back (rows of head_dim, cycles each for the whole GPU).
+constexpr int kMergeCycles = 5000;
+inline long long partial_cycles(long long rows, int head_dim) { return rows * head_dim / 1024; }
+
+struct TileUnit { TileItem item; int n_kt, per_tile; long long cycles() const { return kItemCycles + static_cast<long long>(n_kt) * per_tile; } };
+struct TileDeal { std::vector<std::vector<TileItem>> lists; long long cycles = 0, part_rows = 0; };
+
+inline long long item_rows(const TileItem& t, const SegmentGeometry& g) { return static_cast<long long>(t.n_tok) * g.group() * (t.flags & kPair ? 2 : 1); }
+
+// Whole, longest first, each to the block with the least to do so far.
+inline TileDeal deal_whole(std::vector<TileUnit> units, int sms) {
+  std::stable_sort(units.begin(), units.end(), [](const TileUnit& x, const TileUnit& y) { return x.cycles() > y.cycles(); });
+  TileDeal d;
+  d.lists.resize(std::min<size_t>(units.size(), sms));
+  using Load = std::pair<long long, int>;
+  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least;
+  for (size_t b = 0; b < d.lists.size(); ++b) least.push({0, static_cast<int>(b)});
+  for (const TileUnit& u : units) {
+    Load l = least.top();
+    least.pop();
+    d.lists[l.second].push_back(u.item);
+    l.first += u.cycles();
+    d.cycles = std::max(d.cycles, l.first);
+    least.push(l);
+  }
+  return d;
 }
 
-// In how many ranges each segment's keys are cut.  One SM works an item off in about one unit per key tile and row
-// group (less than two for both groups) and kItemCost for its start and end; a range more costs its partials.  The
-// cut that ends first by that account, over all item lengths.
-inline void cut_segments(std::vector<Segment>& segs, const SegmentGeometry& g, int sms, long long slots, bool prefix) {
-  constexpr double kItemCost = 2.0, kTwoGroups = 1.5, kMerge = 3.0;
-  int longest = 0;
-  for (const Segment& s : segs) longest = std::max(longest, (s.kv_len + kTileKeys - 1) / kTileKeys);
-  double best = -1;
-  int best_len = longest;
-  for (int n = 1; n <= 64 && n <= longest; ++n) {
-    const int len = (longest + n - 1) / n;
-    double total = 0, most = 0;
-    long long used = 0;
-    for (const Segment& s : segs) {
-      const int kt = (s.kv_len + kTileKeys - 1) / kTileKeys, c = (kt + len - 1) / len, per = (kt + c - 1) / c;
-      const long long full = s.n_tok / g.tile_tokens(), rest = (s.n_tok - full * g.tile_tokens()) * static_cast<long long>(g.group());
-      const long long rows = static_cast<long long>(s.n_tok) * g.group();
-      const bool halves = rest > 0 && rest <= kTileRows / 2 && (prefix || c > 1) && per > 1;
-      if (prefix || c > 1) used += s.n_tok * static_cast<long long>(c * (rows <= kTileRows / 2 && per > 1 ? 2 : 1));
-      const double two = kItemCost + kTwoGroups * per, one = kItemCost + (halves ? 0.55 : 1.0) * per;
-      total += g.kv_heads * c * (full * two + (rest > kTileRows / 2 ? two : rest > 0 ? one : 0.0));
-      most = std::max(most, full > 0 || rest > kTileRows / 2 ? two : one);
+// End to end, cut into equal shares.  `part` numbers the pieces' partial rows; pieces of a unit lie one behind the other.
+inline TileDeal deal_shares(const std::vector<TileUnit>& units, int sms, const SegmentGeometry& g, bool prefix) {
+  TileDeal d;
+  long long total = 0, longest = 0;
+  for (const TileUnit& u : units) {
+    total += u.cycles();
+    longest = std::max<long long>(longest, u.per_tile);
+  }
+  // every cut costs an item's start and end again
+  const long long share = std::max<long long>((total + static_cast<long long>(sms) * kItemCycles) / sms, kItemCycles + kLeastTiles * longest);
+  long long room = 0, done = 0;
+  for (const TileUnit& u : units) {
+    int at = 0;
+    std::vector<std::pair<size_t, size_t>> pieces;                       // (list, place)
+    while (at < u.n_kt) {
+      const bool last = static_cast<int>(d.lists.size()) >= sms;
+      if (d.lists.empty() || (!last && !d.lists.back().empty() && room < kItemCycles + std::min(kLeastTiles, u.n_kt - at) * static_cast<long long>(u.per_tile))) {
+        d.lists.emplace_back();
+        room += share;                                                   // (what a list leaves, the next one gets)
+        done = 0;
+        continue;
+      }
+      int n = last ? u.n_kt - at : static_cast<int>(std::min<long long>(u.n_kt - at, std::max<long long>(kLeastTiles, (room - kItemCycles) / u.per_tile)));
+      if (u.n_kt - at - n < kLeastTiles) n = u.n_kt - at;                // nothing worth a piece would be left
+      TileItem t = u.item;
+      t.kv_begin = at * kTileKeys;
+      t.kv_len = std::min(n * kTileKeys, u.item.kv_len - t.kv_begin);
+      pieces.push_back({d.lists.size() - 1, d.lists.back().size()});
+      d.lists.back().push_back(t);
+      const long long took = kItemCycles + static_cast<long long>(n) * u.per_tile;
+      room -= took;
+      done += took;
+      d.cycles = std::max(d.cycles, done);
+      at += n;
     }
-    if (used > slots) continue;
-    // longest items first, dealt in turn: at worst an even share and most of the last item
-    const double even = total / sms, time = std::max(most, even > most ? even + 0.5 * most : even) + (n > 1 && !prefix ? kMerge : 0.0) +
-                                            4.0 * static_cast<double>(used) * g.q_heads * g.head_dim / 1e6;
-    if (best < 0 || time < best) { best = time; best_len = len; }
+    if (prefix || pieces.size() > 1)
+      for (const auto& p : pieces) {
+        d.lists[p.first][p.second].part = static_cast<int>(d.part_rows);
+        d.part_rows += item_rows(u.item, g);
+      }
   }
-  for (Segment& s : segs) {
-    const int kt = (s.kv_len + kTileKeys - 1) / kTileKeys;
-    s.chunks = best < 0 ? 1 : (kt + best_len - 1) / best_len;
-    s.slots = 0;
-  }
+  return d;
 }
 
 // Cuts the decode kernels' tokens, as pkv_decode_plan_host does: equal shares where there are enough keys, else chunks,
@@ -158,63 +203,75 @@ inline void cut_own(const std::vector<OwnRange>& own, const SegmentGeometry& g, 
   std::stable_sort(out.items.begin(), out.items.end(), [](const WorkItem& x, const WorkItem& y) { return x.kv_len > y.kv_len; });
 }
 
-// Puts everything together.  out.rows holds the segments' tokens already; `empty`: tokens without keys.
-inline void list_segments(std::vector<Segment>& segs, const std::vector<OwnRange>& own, const std::vector<int>& empty, const SegmentGeometry& g,
+// Puts everything together.  out.row_token holds the segments' tokens already; `empty`: tokens without keys.
+inline void list_segments(const std::vector<Segment>& segs, const std::vector<OwnRange>& own, const std::vector<int>& empty, const SegmentGeometry& g,
                           int sms, bool prefix, SegmentLists& out) {
-  cut_segments(segs, g, sms, tile_slots(g, sms) + (prefix ? g.n_tokens : 0), prefix);
   std::vector<int> pieces;
   cut_own(own, g, own_extra(g), out, pieces);
-  // the tiles, with the partials of each of their tokens numbered from 0
   const int group = g.group();
-  for (Segment& s : segs) {
-    const int kt = (s.kv_len + kTileKeys - 1) / kTileKeys, per = (kt + s.chunks - 1) / s.chunks;
-    s.chunks = (kt + per - 1) / per;
-    const long long rows = static_cast<long long>(s.n_tok) * group;
-    const bool partial = prefix || s.chunks > 1;
-    // all of a segment's rows leave the same number of partials: only one that fits a single group is halved
-    const bool halves = partial && rows <= kTileRows / 2 && per > 1;
-    s.slots = partial ? s.chunks * (halves ? 2 : 1) : 0;
-    for (int c = 0; c < s.chunks; ++c) {
-      const int begin = c * per * kTileKeys, len = std::min(per * kTileKeys, s.kv_len - begin);
-      const bool two = halves && len > kTileKeys;
+  std::vector<TileUnit> units;
+  for (const Segment& s : segs) {
+    const int n_kt = (s.kv_len + kTileKeys - 1) / kTileKeys;
+    for (int kvh = 0; kvh < g.kv_heads; ++kvh)
       for (int t = 0; t < s.n_tok; t += g.tile_tokens()) {
         const int n = std::min(g.tile_tokens(), s.n_tok - t), tok0 = s.tok0 + t;
-        const bool row = out.rows[tok0 + n - 1].token - out.rows[tok0].token == n - 1;      // (they ascend)
-        out.tiles.push_back(TileItem{tok0, n, begin, len, partial ? c * (halves ? 2 : 1) : -1,
-                                     (row ? kConsecutive : 0) | (halves && !two ? kEmptySecond : 0), two ? 1 : 0, 0});
+        const bool small = n * group <= kTileRows / 2, pair = small && (kvh ^ 1) < g.kv_heads;
+        if (pair && (kvh & 1)) continue;
+        const bool row = out.row_token[tok0 + n - 1] - out.row_token[tok0] == n - 1;      // (they ascend)
+        units.push_back(TileUnit{TileItem{tok0, n, kvh, 0, s.kv_len, -1, (row ? kConsecutive : 0) | (pair ? kPair : 0), s.source}, n_kt,
+                                 pair ? kPairCycles : small ? kOneGroupCycles : kTwoGroupCycles});
       }
-    }
   }
-  auto cost = [group](const TileItem& t) {
-    const int kt = (t.kv_len + kTileKeys - 1) / kTileKeys;
-    return t.halves ? (kt + 1) / 2 * 2 : kt * (t.n_tok * group > kTileRows / 2 ? 3 : 2);
-  };
-  std::stable_sort(out.tiles.begin(), out.tiles.end(), [&](const TileItem& x, const TileItem& y) { return cost(x) > cost(y); });
-  // partial slots: a token's tiles' first, then its own pieces'
+  if (!units.empty()) {
+    TileDeal deal = deal_shares(units, sms, g, prefix);
+    if (!prefix) {
+      TileDeal whole = deal_whole(units, sms);
+      if (whole.cycles <= deal.cycles + (deal.part_rows > 0 ? kMergeCycles + partial_cycles(deal.part_rows, g.head_dim) : 0) ||
+          deal.part_rows > most_tile_rows(g, sms, false))
+        deal = std::move(whole);
+    }
+    out.n_tile_rows = deal.part_rows;
+    for (const auto& list : deal.lists) {
+      out.list_first.push_back(static_cast<int>(out.tiles.size()));
+      out.tiles.insert(out.tiles.end(), list.begin(), list.end());
+    }
+    out.list_first.push_back(static_cast<int>(out.tiles.size()));
+  }
+  // what is merged: tokens of tiles with partials, one record for each kv head, found through the tile's first piece
   std::vector<int> own_of(g.n_tokens, -1), base(own.size(), -1);
   for (size_t i = 0; i < own.size(); ++i) own_of[own[i].token] = static_cast<int>(i);
-  for (const Segment& s : segs)
-    for (int t = 0; t < s.n_tok; ++t) {
-      RowToken& r = out.rows[s.tok0 + t];
-      const int o = own_of[r.token], n = s.slots + (o >= 0 ? pieces[o] : 0);
-      r.part_base = out.n_parts;
-      if (s.slots == 0 && o < 0) continue;
-      if (o >= 0) base[o] = out.n_parts + s.slots;
-      out.merge.push_back(MergeRow{r.token, out.n_parts, n, 0});
-      out.n_parts += n;
+  std::vector<char> seen(own.size(), 0);
+  auto parts_of = [&](int o) {
+    if (base[o] < 0) {
+      base[o] = out.n_parts;
+      out.n_parts += pieces[o];
     }
+    return base[o];
+  };
+  std::map<std::pair<int, int>, int> n_pieces;                                            // of a unit: (tok0, kvh)
+  for (const TileItem& t : out.tiles)
+    if (t.part >= 0) ++n_pieces[{t.tok0, t.kvh}];
+  for (const TileItem& t : out.tiles) {
+    if (t.part < 0 || t.kv_begin > 0) continue;
+    const int rows = t.n_tok * group, heads = t.flags & kPair ? 2 : 1, n = n_pieces[{t.tok0, t.kvh}];
+    for (int h = 0; h < heads; ++h)
+      for (int i = 0; i < t.n_tok; ++i) {
+        const int token = out.row_token[t.tok0 + i], o = own_of[token];
+        out.merge.push_back(MergeRow{token, t.kvh + h, t.part + h * rows + i * group, heads * rows, n, o >= 0 ? parts_of(o) : 0, o >= 0 ? pieces[o] : 0, 0});
+        if (o >= 0) seen[o] = 1;
+      }
+  }
   for (size_t i = 0; i < own.size(); ++i)
-    if (base[i] < 0 && pieces[i] > 1) {
-      base[i] = out.n_parts;
-      out.merge.push_back(MergeRow{own[i].token, out.n_parts, pieces[i], 0});
-      out.n_parts += pieces[i];
-    }
+    if (!seen[i] && pieces[i] > 1)
+      for (int kvh = 0, at = parts_of(static_cast<int>(i)); kvh < g.kv_heads; ++kvh)
+        out.merge.push_back(MergeRow{own[i].token, kvh, 0, 0, 0, at, pieces[i], 0});
   for (WorkItem& w : out.items) {
     const int i = w.token;
     w.token = own[i].token;
     w.part = base[i] < 0 ? -1 : base[i] + w.part;
   }
-  for (int t : empty) out.merge.push_back(MergeRow{t, 0, 0, 0});
+  for (int t : empty)
+    for (int kvh = 0; kvh < g.kv_heads; ++kvh) out.merge.push_back(MergeRow{t, kvh, 0, 0, 0, 0, 0, 0});
 }
 
 }  // namespace pkv

@@ -14,10 +14,10 @@ class Image:
             return raw[off:off + 4 * n * width].copy().view(np.int32).reshape(n, width)
 
         self.items = ints(p.off_items, p.n_items, 4)                      # token, kv_begin, kv_len, part
-        self.tiles = ints(p.off_tiles, p.n_tiles, 8)                      # tok0, n_tok, kv_begin, kv_len, part, flags, halves, -
-        self.merge = ints(p.off_merge, p.n_merged, 4)                     # token, part_base, n_parts, -
-        n_rows = (p.off_items - p.off_rows) // 8
-        self.rows = ints(p.off_rows, n_rows, 2)                           # token, part_base
+        self.tiles = ints(p.off_tiles, p.n_tiles, 8)                      # tok0, n_tok, kvh, kv_begin, kv_len, part, flags, -
+        self.merge = ints(p.off_merge, p.n_merged, 8)                     # token, kvh, tile row, stride, n, own part, n, -
+        self.rows = raw[p.off_rows:p.off_items].view(np.int32)
+        self.lists = ints(p.off_lists, p.n_lists + 1, 1)[:, 0] if p.n_lists else None
         self.seq = ints(p.off_seq, p.n_tokens, 1)[:, 0]
         self.pos = ints(p.off_pos, p.n_tokens, 1)[:, 0]
         first = p.off_items + 16 * p.n_items
@@ -25,57 +25,62 @@ class Image:
 
 
 def check_cover(image, plan, want):
-    """want: {token: number of keys}.  Every (token, head of a group, key) is worked on exactly once; a token's pieces are
-    either one that writes its output, or fill exactly the partials that the merge reads."""
-    group = plan.q_heads // plan.kv_heads
-    keys, slots, direct = {}, {}, {}
-
-    def add(token, head, begin, n, part):
-        heads = range(group) if head is None else [head]
-        for h in heads:
-            keys.setdefault((token, h), []).append((begin, n))
-            if part < 0:
-                direct[token, h] = direct.get((token, h), 0) + 1
-            else:
-                slots.setdefault((token, h), []).append(part)
-
+    """want: {token: number of keys}.  Every (token, kv head, key) is worked on exactly once; what is done in one piece writes
+    the output, and the merge reads every other piece's partial, each row and part used once."""
+    group, kvh_n = plan.q_heads // plan.kv_heads, plan.kv_heads
+    keys, direct, tile_rows, parts = {}, set(), {}, {}
     for token, begin, n, part in image.items.tolist():
         assert n > 0 and begin >= 0
-        add(token, None, begin, n, part)
-    for tok0, n_tok, begin, n, part, flags, halves, _ in image.tiles.tolist():
+        for h in range(kvh_n):
+            keys.setdefault((token, h), []).append((begin, n))
+            if part < 0:
+                assert (token, h) not in direct
+                direct.add((token, h))
+        if part >= 0:
+            parts.setdefault(token, []).append(part)
+    used_rows = np.zeros(plan.n_tile_rows, np.int32)
+    for tok0, n_tok, kvh, begin, n, part, flags, _ in image.tiles.tolist():
+        pair = bool(flags & 2)
         rows = n_tok * group
-        assert 1 <= rows <= 256 and n > 0 and begin % 128 == 0 and not (halves and (rows > 128 or n <= 128 or part < 0))
-        tokens = image.rows[tok0:tok0 + n_tok, 0]
+        assert 1 <= rows <= (128 if pair else 256) and n > 0 and begin % 128 == 0 and kvh + pair < kvh_n
+        tokens = image.rows[tok0:tok0 + n_tok]
         assert bool(flags & 1) == bool((np.diff(tokens) == 1).all())
-        for f in range(rows):
-            token, base = image.rows[tok0 + f // group].tolist()
-            add(token, f % group, begin, n, base + part if part >= 0 else -1)
-            if halves or flags & 2:
-                slots[token, f % group].append(base + part + 1)
-    merged = {t: (base, n) for t, base, n, _ in image.merge.tolist()}
-    assert len(merged) == len(image.merge)
-    used = []
+        for h in range(1 + pair):
+            for i, token in enumerate(tokens.tolist()):
+                keys.setdefault((token, kvh + h), []).append((begin, n))
+                if part < 0:
+                    assert (token, kvh + h) not in direct
+                    direct.add((token, kvh + h))
+                else:
+                    tile_rows.setdefault((token, kvh + h), []).append(part + h * rows + i * group)
+        if part >= 0:
+            used_rows[part:part + rows * (1 + pair)] += 1
+    assert (used_rows == 1).all()
+    merged = {}
+    for token, kvh, row, stride, n_tile, own, n_own, _ in image.merge.tolist():
+        assert (token, kvh) not in merged
+        merged[token, kvh] = ([row + i * stride for i in range(n_tile)], list(range(own, own + n_own)))
+    used_parts = []
     for token, n_keys in want.items():
-        for h in range(group):
+        for h in range(kvh_n):
             got = sorted(keys.get((token, h), []))
             at = 0
             for begin, n in got:
                 assert begin == at, (token, h, got)
                 at += n
             assert at == n_keys, (token, h, at, n_keys)
-            if n_keys == 0:
-                assert merged[token][1] == 0 and (token, h) not in direct
-            elif (token, h) in direct:
-                assert direct[token, h] == 1 and len(got) == 1 and token not in merged
+            if (token, h) in direct:
+                assert len(got) == 1 and (token, h) not in merged
             else:
-                base, n = merged[token]
-                assert sorted(slots[token, h]) == list(range(base, base + n))
-                if h == 0:
-                    used += range(base, base + n)
-    assert set(t for t, _ in keys) <= set(want)
-    assert sorted(used) == list(range(plan.n_parts))
+                assert merged[token, h] == (sorted(tile_rows.get((token, h), [])), sorted(parts.get(token, [])))
+                assert bool(n_keys) == bool(merged[token, h][0] or merged[token, h][1])
+        used_parts += parts.get(token, [])
+    assert set(t for t, _ in keys) <= set(want) and set(t for t, _ in merged) <= set(want)
+    assert sorted(used_parts) == list(range(plan.n_parts))
     if image.first is not None:
         assert image.first[0] == 0 and image.first[-1] == len(image.items) and (np.diff(image.first) >= 0).all()
+    if image.lists is not None:
+        assert image.lists[0] == 0 and image.lists[-1] == len(image.tiles) and (np.diff(image.lists) > 0).all()
 
 
 # ---- steps on the device, and the definition in 64 bits ----

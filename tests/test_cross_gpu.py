@@ -73,7 +73,7 @@ def test_many_items_on_every_block(pkv, torch_cuda):
     lens = [300 + 61 * (i % 7) for i in range(30)]
     step = Step(torch_cuda, "bf16", PAIRED, [130 + 40 * (i % 5) for i in range(30)], lens, 16, seed=5)
     plan = run(pkv, step)
-    assert plan.plan.n_tiles * step.kvh > 148
+    assert plan.plan.n_tiles > 148
     step.check(pkv)
 
 

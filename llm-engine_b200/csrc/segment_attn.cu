@@ -6,21 +6,22 @@
 //
 // A tile item is up to 256 rows (token, query head of one kv head's group) that all see the same keys, walked in tiles of
 // 128.  The rows are two groups of 128, each with its own scores S (128 columns of tensor memory) and output O (head_dim
-// columns); a K or V tile is fetched once for both.  While one group's scores are turned into probabilities by its
-// four warps, the tensor cores work on the other group: a 128 x 128 x 128 product takes 512 cycles, the 16,384
-// exponentials of a group's tile 1,024.
+// columns); a K or V tile is fetched once for both.  While one group's scores are turned into probabilities, the tensor
+// cores work on the other group: a 128 x 128 x 128 product takes 512 cycles, the 16,384 exponentials of a group's tile 1,024.
 //
-//   warps 0-3, 4-7  softmax of group 0, 1: thread = row.  128 scores to registers, maximum, exponentials, sum; P goes
-//                   back to tensor memory as 16-bit pairs, the A operand of the second product.  O stays there and is
-//                   rescaled only when a row's maximum has grown by more than 2^8.
-//   warp 8          TMA: K and V tiles through the block table into a ring (boxes of up to 128 slots x 128 bytes).
-//   warp 9          issues the products, one thread: S = Q K^T and O += P V of both groups in turns.
-//   warp 10         TMA: the next item's rows of Q, a box for each token's heads, or for several consecutive tokens'.
+//   warps 0-7, 8-15 softmax of group 0, 1: a row is two threads, of 64 keys each, which exchange their maxima through shared
+//                   memory.  (One thread a row, eight warps in all, left the exponential unit half idle: 3,850 cycles for a
+//                   tile of both groups at head_dim 128, 3,300 at 64.)  P goes back to tensor memory as 16-bit pairs, the A
+//                   operand of the second product.  O stays there and is rescaled only when a row's maximum has grown by
+//                   more than 2^8.
+//   warp 16         TMA: K and V tiles through the block table into a ring (boxes of up to 128 slots x 128 bytes).
+//   warp 17         issues the products, one thread: S = Q K^T and O += P V of both groups in turns.
+//   warp 18         TMA: the next item's rows of Q, a box for each token's heads, or for several consecutive tokens'.
 //
 // head_dim 64: P has 64 columns of its own.  The next scores of a group are issued as soon as its threads hold the present ones
 // in registers, so the softmax warps never wait for a product: the exponentials decide.
-// head_dim 128: S and O fill the group's half of tensor memory, P lies over the first half of S.  The next scores follow
-// the second product, whose first half starts when P's first 64 keys are there.
+// head_dim 128: S and O fill the group's half of tensor memory, P lies over the first half of S, and the next scores follow
+// the second product.
 //
 // An item of at most 128 rows brings those of two kv heads, one for each group, whose K and V tiles alternate in the ring.
 // P is rounded to 16 bits for the second product (the sums are of the unrounded ones), as the operands of the
@@ -51,10 +52,10 @@ int check_error_mirror(const char* fn, unsigned int bits = ~0u);
 
 namespace {
 
-constexpr int kTileThreads = 384;
-// Registers a thread of the softmax warps and of the others; launched with 168 each (2 x 208 + 80 <= 3 x 168).
-constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
-constexpr int kProducer = 8, kIssuer = 9, kRowsLoader = 10;   // the 12th warp idles: registers are split by fours
+constexpr int kTileThreads = 640;
+// Registers a thread of the softmax warps and of the others; launched with 96 each (4 x 104 + 64 <= 5 x 96).
+constexpr int kSoftmaxRegs = 104, kOtherRegs = 64;
+constexpr int kProducer = 16, kIssuer = 17, kRowsLoader = 18;   // the 20th warp idles: registers are split by fours
 constexpr int kBlockBytes = 128 * 128;                   // 128 rows x 64 16-bit elements: one operand block
 constexpr uint32_t kGroupCols = 256, kColO = 128;        // tensor memory of a group: S, then O ...
 constexpr float kRescale = 8.f;                          // in log2 units: P stays below 2^8
@@ -65,7 +66,7 @@ constexpr int kMinPrefixTokens = 2;                      // batches of fewer tok
 template <int D> struct TileSmem {
   static constexpr int kHalves = D / 64;
   static constexpr int kTile = kHalves * kBlockBytes;    // a K or V tile, or one group's Q
-  static constexpr int kStages = D == 64 ? 8 : 5;
+  static constexpr int kStages = D == 64 ? 8 : 4;
   static constexpr uint32_t kColP = D == 64 ? 192 : 0;   // ... and P behind O, or over S
   static constexpr int kLead = D == 64 ? 2 : 1;          // key tiles a group's scores are issued ahead of its values
   // Q: half (64 dims) by half, 256 rows each; the next item's beside the present one's where there is room
@@ -115,13 +116,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-// Eight 16-byte pieces a lane: piece i of lane j of every eight lanes becomes piece j of lane i.
-__device__ __forceinline__ void transpose8(uint32_t (&x)[32], int lane) {
+// N 16-byte pieces a lane: piece i of lane j of every N lanes becomes piece j of lane i.
+template <int N>
+__device__ __forceinline__ void transpose(uint32_t (&x)[4 * N], int lane) {
 #pragma unroll
-  for (int s = 1; s < 8; s <<= 1) {
+  for (int s = 1; s < N; s <<= 1) {
     const bool upper = (lane & s) != 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
       if (i & s) continue;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -151,13 +153,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   constexpr int NS = S::kStages;
 
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[2 * NS + 14];
+  __shared__ __align__(8) unsigned long long bars[2 * NS + 12];
+  __shared__ float sm_max[2][2][2][128], sm_sum[2][2][128];   // [tile parity][group][half][row]; [group][half][row]
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t ring = base + S::kRing, bar0 = smem_u32(&bars[0]);
-  enum { KV_FULL = 0, KV_EMPTY = NS, Q_FULL = 2 * NS, Q_EMPTY = Q_FULL + 2, S_FULL = Q_EMPTY + 2, S_READ = S_FULL + 2, P_HALF = S_READ + 2, P_FULL = P_HALF + 2, O_FULL = P_FULL + 2 };
+  enum { KV_FULL = 0, KV_EMPTY = NS, Q_FULL = 2 * NS, Q_EMPTY = Q_FULL + 2, S_FULL = Q_EMPTY + 2, S_READ = S_FULL + 2, P_FULL = S_READ + 2, O_FULL = P_FULL + 2 };
   auto BAR = [&](int i) { return bar0 + 8u * i; };
 
   if (threadIdx.x == 0) {
@@ -169,9 +172,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(BAR(Q_FULL + g), 1);    // (of a buffer, not of a group)
       mbar_init(BAR(Q_EMPTY + g), 1);   // commit after the item's last Q K^T
       mbar_init(BAR(S_FULL + g), 1);    // commit after the group's Q K^T
-      mbar_init(BAR(S_READ + g), 128);  // kLead 2: the group's softmax threads (32 at a time) hold S in registers
-      mbar_init(BAR(P_HALF + g), 128);  // kLead 1: they have written P for the first 64 keys ...
-      mbar_init(BAR(P_FULL + g), 128);  // ... for all
+      mbar_init(BAR(S_READ + g), 256);  // kLead 2: the group's softmax threads (32 at a time) hold S in registers
+      mbar_init(BAR(P_FULL + g), 256);  // they have written P
       mbar_init(BAR(O_FULL + g), 1);    // commit after the group's P V: kLead 2 each, kLead 1 the item's last
     }
     mbar_fence_init();
@@ -332,16 +334,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           };
           // Products of one thread run in order: where P lies over S, the group's next scores overwrite it behind these.
           auto values = [&](int g, uint32_t v_addr, bool first, bool final) {
+            WAIT(BAR(P_FULL + g), (done >> g) & 1);
+            tc::fence_after();
             uint32_t v_lo = v_addr >> 4, t = tmem + g * kGroupCols;
             asm volatile("" : "+r"(v_lo), "+r"(t));
 #pragma unroll
-            for (int kk = 0; kk < kTileKeys / 16; ++kk) {
-              if (kk == 0 || kk == 4) {
-                if (S::kLead == 1 || kk == 0) WAIT(BAR((S::kLead == 1 && kk == 0 ? P_HALF : P_FULL) + g), (done >> g) & 1);
-                tc::fence_after();
-              }
+            for (int kk = 0; kk < kTileKeys / 16; ++kk)
               tc::mma_ts(t + kColO, t + S::kColP + kk * 8, tc::operand_at(v_lo + kk * (2048 >> 4), kBlockBytes), kInstrPV, !(first && kk == 0));
-            }
             done ^= 1u << g;
             if (final && S::kLead > 1) read ^= 1u << g;              // see scores()
             if (final || S::kLead > 1) tc::commit(BAR(O_FULL + g));
@@ -388,208 +387,175 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   } else {
     after_previous();
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
-    // ---- softmax: thread = row of its group = lane of tensor memory ----
-    const int g = warp >> 2, r_in = threadIdx.x & 127;
-    const uint32_t t_s = tmem + g * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16), t_o = t_s + kColO, t_p = t_s + S::kColP;
+    // ---- softmax: thread = 64 keys (half) of a row of its group = lane of tensor memory ----
+    const int g = warp >> 3, half = (warp >> 2) & 1, r_in = (warp & 3) * 32 + lane;
+    const uint32_t t_g = tmem + g * kGroupCols + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t t_s = t_g + half * 64, t_p = t_g + S::kColP + half * 32, t_o = t_g + kColO + half * (D / 2);   // its share of each
     const float sl2 = a.scale * kLog2e;
+    // the two warps of a row's threads
+    auto meet = [&] { asm volatile("bar.sync %0, 64;\n" ::"r"(1 + g * 4 + (warp & 3)) : "memory"); };
     uint32_t e0 = 0, done = 0, finished = 0;                     // ring entries before this item; the group's key tiles; its commits to O_FULL awaited
     for (int r = 0; r < n_items && !dead; ++r) {
-      const TileItem it = load_tile(tiles + r);
-      const int pair = it.flags & kPair ? 1 : 0, n = (it.kv_len + kTileKeys - 1) / kTileKeys << pair;
+      int pair, n, rows, kv_len;
+      {
+        const TileItem it = load_tile(tiles + r);
+        pair = it.flags & kPair ? 1 : 0;
+        n = (it.kv_len + kTileKeys - 1) / kTileKeys << pair;
+        rows = it.n_tok * a.group;
+        kv_len = it.kv_len;
+      }
+      const int step = 1 + pair;
       e0 += 2 * n;
       const uint32_t last_v = e0 - 1 - pair + (pair & g);        // ring entry of the group's last V tile
-      const int rows = it.n_tok * a.group, row = pair ? r_in : g * 128 + r_in;   // row of the item
+      const int row = pair ? r_in : g * 128 + r_in;   // row of the item
       if (g == 1 && !pair && rows <= 128) continue;
-      const bool mine = row < rows;
-      int token = 0, head = 0;
-      if (mine) {
-        const int t = row / a.group;
-        token = __ldg(a.row_token + it.tok0 + t);
-        head = (it.kvh + (pair & g)) * a.group + (row - t * a.group);
-      }
-      const bool working = (row & ~31) < rows;                // some row of this warp is the item's
+      const bool working = (row & ~31) < rows;                   // some row of this warp is the item's
       float m_used = -INFINITY;
       float2 l = both(0.f);
-      const int step = 1 + pair;
-      // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring held.  Cleared
-      // before the group's threads report the tile's P, so that 0 * x stays 0.
-      auto clear_tail = [&](int t, int valid) {
-        if (t + step < n || valid >= kTileKeys || (g == 1 && !pair)) return;
-        WAIT(BAR(KV_FULL + last_v % NS), (last_v / NS) & 1);
-        if (r_in >= valid) {
-#pragma unroll
-          for (int h = 0; h < S::kHalves; ++h) {
-            unsigned char* v = base_ptr + S::kRing + (last_v % NS) * S::kTile + h * kBlockBytes + r_in * 128;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-          }
-        }
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      };
       for (int t = pair & g; t < n; t += step, ++done) {
         WAIT(BAR(S_FULL + g), done & 1);
         tc::fence_after();
-        const int valid = it.kv_len - (t >> pair) * kTileKeys;             // keys of this tile, if fewer than kTileKeys
+        const int valid = kv_len - (t >> pair) * kTileKeys;   // keys of this tile, if fewer than kTileKeys
+        const bool opening = t < step;
+        float sc[64];
         if (working) {
-          float sc[kTileKeys];
-#pragma unroll
-          for (int c = 0; c < kTileKeys; c += 32) tc::ld32(t_s + c, reinterpret_cast<uint32_t*>(sc) + c);
+          tc::ld32(t_s, reinterpret_cast<uint32_t*>(sc));
+          tc::ld32(t_s + 32, reinterpret_cast<uint32_t*>(sc) + 32);
           tc::wait_ld();
-          if constexpr (S::kLead > 1) {
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_warp(BAR(S_READ + g));
-          }
+          tc::fence_before();
+        }
+        if constexpr (S::kLead > 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive_warp(BAR(S_READ + g));
+        }
+        if (working) {
           if (valid < kTileKeys) {
 #pragma unroll
-            for (int i = 0; i < kTileKeys; ++i)
-              if (i >= valid) sc[i] = -INFINITY;
+            for (int i = 0; i < 64; ++i)
+              if (half * 64 + i >= valid) sc[i] = -INFINITY;
           }
-          auto row_max = [&]() {
-            float mx8[8];
+          float mx4[4];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) mx8[u] = fmaxf(sc[u], sc[8 + u]);
+          for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(sc[u], sc[4 + u]);
 #pragma unroll
-            for (int i = 16; i < kTileKeys; i += 16)
+          for (int i = 8; i < 64; i += 8)
 #pragma unroll
-              for (int u = 0; u < 8; ++u) mx8[u] = max3(mx8[u], sc[i + u], sc[i + 8 + u]);
-            return fmaxf(max3(mx8[0], mx8[1], mx8[2]), fmaxf(max3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-          };
-          // P of 64 keys, packed, and its sum.
-          auto weights = [&](int c0, uint32_t (&pk)[32]) {
-            const float2 neg = both(-m_used * sl2), by = both(sl2);
-            float2 sum[2] = {both(0.f), both(0.f)};
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float2 x = fma2(make_float2(sc[c0 + 2 * i], sc[c0 + 2 * i + 1]), by, neg);
-              x = make_float2(ex2(x.x), ex2(x.y));
-              sum[i & 1] = add2(sum[i & 1], x);
-              pk[i] = pack2<T>(x.x, x.y);
-            }
-            return add2(sum[0], sum[1]);
-          };
-          // The first half is worked out with the maximum in use while this tile's is still being looked for: it is
-          // hardly ever too small.
-          uint32_t pk[32];
-          float2 half = both(0.f);
-          const bool opening = t < step;
-          float mx;
-          if (!opening) {
-            half = weights(0, pk);
-            mx = row_max();
-          } else {
-            mx = row_max();
-          }
-          if (opening || __any_sync(0xffffffffu, (mx - m_used) * sl2 > kRescale)) {
-            if (opening) {
-              m_used = mx;
-            } else {
-              // The group's product before this one is complete: where nothing is waited for, its next scores, which have arrived,
-              // were issued behind it.
-              if constexpr (S::kLead > 1) {
-                WAIT(BAR(O_FULL + g), finished & 1);
-                tc::fence_after();
-              }
-              const float m_new = (mx - m_used) * sl2 > kRescale ? mx : m_used;
-              const float f = ex2((m_used - m_new) * sl2);
-              m_used = m_new;
-              l.x *= f;
-              l.y *= f;
-#pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                uint32_t v[32];
-                tc::ld32(t_o + c, v);
-                tc::wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                tc::st32(t_o + c, v);
-              }
-            }
-            half = weights(0, pk);
-          }
-          l = add2(l, half);
-          if constexpr (S::kLead > 1) {                          // P of the tile before has been read
+            for (int u = 0; u < 4; ++u) mx4[u] = max3(mx4[u], sc[i + u], sc[i + 4 + u]);
+          float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          sm_max[done & 1][g][half][r_in] = mx;
+          meet();
+          mx = fmaxf(mx, sm_max[done & 1][g][half ^ 1][r_in]);
+          // O is free of the group's product before this one where that is awaited here, or where the next scores, which have
+          // arrived, were issued behind it; so is P's place.
+          if constexpr (S::kLead > 1) {
             if (!opening) {
               WAIT(BAR(O_FULL + g), finished & 1);
-              ++finished;
               tc::fence_after();
             }
           }
-          tc::st32(t_p, pk);
-          if constexpr (S::kLead == 1) {
-            clear_tail(t, valid);
-            tc::wait_st();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_warp(BAR(P_HALF + g));
-          }
-          l = add2(l, weights(64, pk));
-          tc::st32(t_p + 32, pk);
-          if (S::kLead > 1) clear_tail(t, valid);
-          tc::wait_st();
-          tc::fence_before();
-        } else {
-          // no row of this warp's is the item's: it keeps step only
-          if constexpr (S::kLead > 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive_warp(BAR(S_READ + g));
-            if (t >= step) {
-              WAIT(BAR(O_FULL + g), finished & 1);
-              ++finished;
+          if (opening) {
+            m_used = mx;
+          } else if (__any_sync(0xffffffffu, (mx - m_used) * sl2 > kRescale)) {
+            const float m_new = (mx - m_used) * sl2 > kRescale ? mx : m_used;
+            const float f = ex2((m_used - m_new) * sl2);
+            m_used = m_new;
+            l.x *= f;
+            l.y *= f;
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 16) {
+              uint32_t v[16];
+              tc::ld16(t_o + c, v);
+              tc::wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+              tc::st16(t_o + c, v);
             }
           }
-          clear_tail(t, valid);
-          if constexpr (S::kLead == 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive_warp(BAR(P_HALF + g));
+          const float2 neg = both(-m_used * sl2), by = both(sl2);
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float2 x = fma2(make_float2(sc[c + 2 * i], sc[c + 2 * i + 1]), by, neg);
+              x = make_float2(ex2(x.x), ex2(x.y));
+              l = add2(l, x);
+              pk[i] = pack2<T>(x.x, x.y);
+            }
+            tc::st16(t_p + c / 2, pk);
           }
+        } else if constexpr (S::kLead > 1) {
+          // no row of this warp is the item's: it keeps step only
+          if (!opening) WAIT(BAR(O_FULL + g), finished & 1);
         }
+        if (S::kLead > 1 && !opening) ++finished;
+        if (t + step >= n && valid < kTileKeys && (g == 0 || pair)) {
+          // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring held.  Cleared
+          // before the group's threads report the tile's P, so that 0 * x stays 0.
+          WAIT(BAR(KV_FULL + last_v % NS), (last_v / NS) & 1);
+          if (r_in >= valid && half < S::kHalves) {
+            unsigned char* v = base_ptr + S::kRing + (last_v % NS) * S::kTile + half * kBlockBytes + r_in * 128;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        }
+        if (working) tc::wait_st();
+        tc::fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_warp(BAR(P_FULL + g));
       }
       // ---- epilogue: the next item's first product cannot touch O before this thread has arrived with its P ----
+      float sum = l.x + l.y;
+      if (working) {
+        sm_sum[g][half][r_in] = sum;
+        meet();
+        sum += sm_sum[g][half ^ 1][r_in];
+      }
+      // A thread holds (half) a row; stored as it is, every instruction would touch 32 rows, 16 bytes each (an item's output then
+      // took 20,000 cycles).  Lanes exchange their pieces instead and store whole sectors.
+      const TileItem* again = tiles + r;                         // (not held in registers through the tiles)
+      asm volatile("" : "+l"(again));
+      const TileItem it = load_tile(again);
+      const bool partial = it.part >= 0;
+      unsigned long long to = 0;
+      if (row < rows) {
+        if (partial) {
+          const size_t p = static_cast<size_t>(it.part + (pair & g) * rows + row);
+          to = reinterpret_cast<unsigned long long>(a.part_acc + p * D + half * (D / 2));
+          if (half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_used * a.ml_scale, sum);
+        } else {
+          const int t = row / a.group, token = __ldg(a.row_token + it.tok0 + t), head = (it.kvh + (pair & g)) * a.group + (row - t * a.group);
+          to = reinterpret_cast<unsigned long long>(static_cast<T*>(a.out) + (static_cast<size_t>(token) * a.q_heads + head) * D + half * (D / 2));
+        }
+      }
       WAIT(BAR(O_FULL + g), finished & 1);
       ++finished;
       tc::fence_after();
       if (!working) continue;
-      // A thread holds a row; stored as it is, every instruction would touch 32 rows, 16 bytes each (an item's output then took
-      // 20,000 cycles, the next one's Q behind it).  Eight lanes exchange their pieces instead and store whole lines.
-      const float sum = l.x + l.y;
-      const bool partial = it.part >= 0;
-      const size_t p = static_cast<size_t>(it.part + (pair & g) * rows + row);
-      unsigned long long to = 0;
-      if (mine) {
-        to = partial ? reinterpret_cast<unsigned long long>(a.part_acc + p * D)
-                     : reinterpret_cast<unsigned long long>(static_cast<T*>(a.out) + (static_cast<size_t>(token) * a.q_heads + head) * D);
-        if (partial) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_used * a.ml_scale, sum);
-      }
       const float inv = 1.f / sum;
-      auto store_line = [&](uint32_t (&x)[32], int at) {       // 128 bytes of every lane's row, at byte `at` of the row
-        transpose8(x, lane);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const unsigned long long row_to = __shfl_sync(0xffffffffu, to, (lane & 24) + i);
-          if (row_to) *reinterpret_cast<uint4*>(row_to + at + (lane & 7) * 16) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-        }
-      };
-      if (partial) {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t v[32];
-          tc::ld32(t_o + c, v);
-          tc::wait_ld();
-          store_line(v, c * 4);
-        }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 64) {
-          uint32_t v[64], x[32];
-          tc::ld32(t_o + c, v);
-          tc::ld32(t_o + c + 32, v + 32);
-          tc::wait_ld();
+      for (int c = 0; c < D / 2; c += 32) {
+        uint32_t v[32];
+        tc::ld32(t_o + c, v);
+        tc::wait_ld();
+        if (partial) {                                         // 128 bytes of every lane's row: whole lines
+          transpose<8>(v, lane);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = pack2<T>(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
-          store_line(x, c * 2);
+          for (int i = 0; i < 8; ++i) {
+            const unsigned long long row_to = __shfl_sync(0xffffffffu, to, (lane & 24) + i);
+            if (row_to) *reinterpret_cast<uint4*>(row_to + c * 4 + (lane & 7) * 16) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        } else {                                               // 64 bytes
+          uint32_t x[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = pack2<T>(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
+          transpose<4>(x, lane);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const unsigned long long row_to = __shfl_sync(0xffffffffu, to, (lane & 28) + i);
+            if (row_to) *reinterpret_cast<uint4*>(row_to + c * 2 + (lane & 3) * 16) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          }
         }
       }
       tc::fence_before();

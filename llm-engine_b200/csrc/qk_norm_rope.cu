@@ -8,9 +8,11 @@
 // The rows are read once and written once, so a large step is bound by HBM and a small one by the launch.
 // D / 2 / (16 bytes) neighbouring lanes hold a head, each a 16-byte piece of either half: a lane owns whole
 // rotation pairs, the sum of squares is a few shuffles inside the lanes of the head, and every load and store is
-// 16 bytes.  A v head is a head without the arithmetic.  Large steps give a lane the same piece of several heads of
-// one token, whose loads are all in flight before the first is used and which share the token's cos / sin and the
-// weights: see kHeadsEach.
+// 16 bytes.  A v head is a head without the arithmetic.  Steps that fill the GPU give a lane the same piece of two heads of
+// one token, which share the token's cos / sin: 8,191 tokens of 32/8 heads of 128, bf16 (206 MB), 48 us with one head a
+// lane, 43 with two, 71 with four (94 registers).  Steps whose rows do not fit L2 read and write them as data that is
+// not used again: 36.5 us, 5.6 TB/s; 1,024 tokens lose a tenth that way (6.2 and 6.9), and the launch behind them finds
+// its q, K and V in L2.
 #include "common.cuh"
 #include "launch_util.hpp"
 #include "status.hpp"
@@ -18,7 +20,7 @@
 namespace pkv {
 namespace {
 
-constexpr int kNormThreads = 256;
+constexpr int kNormThreads = 128;
 
 template <typename T>
 struct NormArgs {
@@ -70,17 +72,16 @@ __device__ __forceinline__ void load_floats(const float* p, float (&f)[16 / size
   }
 }
 
-// LANES lanes a head, HEADS heads a lane.  q_out may be q: a lane reads the pieces it writes before it writes them.
-template <typename T, int LANES, int HEADS>
+// LANES lanes a head, HEADS heads a lane; STREAM: nothing is kept in L2.  q_out may be q: a lane reads the pieces it writes before it writes them.
+template <typename T, int LANES, int HEADS, bool STREAM>
 __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormArgs<T> a) {
   constexpr int E = 16 / sizeof(T);
   pdl_launch_dependents();
   pdl_wait();
-  const int heads = a.q_heads + 2 * a.kv_heads, per_token = (heads + HEADS - 1) / HEADS;
-  const long long group = (blockIdx.x * static_cast<long long>(kNormThreads) + threadIdx.x) / LANES;
-  const long long at = group / per_token;
+  const unsigned heads = a.q_heads + 2 * a.kv_heads, per_token = (heads + HEADS - 1) / HEADS;
+  const unsigned group = blockIdx.x * (kNormThreads / LANES) + threadIdx.x / LANES, at = group / per_token;
   // lanes of a group leave together, and so do whole warps of them or not: the shuffles below name the group's lanes
-  if (at >= a.n_tokens) return;
+  if (at >= static_cast<unsigned>(a.n_tokens)) return;
   const int token = static_cast<int>(at), head0 = static_cast<int>(group - at * per_token) * HEADS;
   const int piece = threadIdx.x % LANES, half = a.head_dim / 2;
   const unsigned lanes = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
@@ -93,12 +94,13 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormAr
   for (int u = 0; u < HEADS; ++u) {
     dst[u] = nullptr;
     lo[u] = hi[u] = make_uint4(0u, 0u, 0u, 0u);
-    if (head0 + u < heads) {
+    if (head0 + u < static_cast<int>(heads)) {
       const T* src;
       head_rows(a, token, head0 + u, slot, src, dst[u]);
       // plain loads: q_out may be q
-      lo[u] = *reinterpret_cast<const uint4*>(src + piece * E);
-      hi[u] = *reinterpret_cast<const uint4*>(src + half + piece * E);
+      const uint4 *x = reinterpret_cast<const uint4*>(src + piece * E), *y = reinterpret_cast<const uint4*>(src + half + piece * E);
+      lo[u] = STREAM ? __ldcs(x) : *x;
+      hi[u] = STREAM ? __ldcs(y) : *y;
     }
   }
   float c[E], s[E];
@@ -130,8 +132,14 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormAr
       }
     }
     if (dst[u]) {
-      *reinterpret_cast<uint4*>(dst[u] + piece * E) = lo[u];
-      *reinterpret_cast<uint4*>(dst[u] + half + piece * E) = hi[u];
+      uint4 *x = reinterpret_cast<uint4*>(dst[u] + piece * E), *y = reinterpret_cast<uint4*>(dst[u] + half + piece * E);
+      if (STREAM) {
+        __stcs(x, lo[u]);
+        __stcs(y, hi[u]);
+      } else {
+        *x = lo[u];
+        *y = hi[u];
+      }
     }
   }
 }
@@ -175,21 +183,24 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_pairs_kernel(const 
   }
 }
 
-// Heads a lane takes in large steps.
-constexpr int kHeadsEach = 4;
-constexpr long long kManyLanes = 148ll * 2048;
+constexpr int kHeadsEach = 2;
+constexpr long long kManyLanes = 148ll * 2048;              // more lanes than the GPU holds at once
+constexpr long long kStreamBytes = 96ll << 20;              // of rows read and written
 
 template <typename T, int LANES>
 void launch_lanes(const NormArgs<T>& a, cudaStream_t stream) {
   const int heads = a.q_heads + 2 * a.kv_heads;
   auto blocks = [&](int each) {
-    const long long lanes = static_cast<long long>(a.n_tokens) * ((heads + each - 1) / each) * LANES;
-    return dim3(static_cast<unsigned>((lanes + kNormThreads - 1) / kNormThreads));
+    const long long groups = static_cast<long long>(a.n_tokens) * ((heads + each - 1) / each), per_block = kNormThreads / LANES;
+    return dim3(static_cast<unsigned>((groups + per_block - 1) / per_block));
   };
-  if (static_cast<long long>(a.n_tokens) * heads * LANES > kManyLanes)
-    launch_pdl(qk_norm_rope_kernel<T, LANES, kHeadsEach>, blocks(kHeadsEach), dim3(kNormThreads), 0, stream, a);
+  const long long all = static_cast<long long>(a.n_tokens) * heads;
+  if (2 * all * a.head_dim * static_cast<long long>(sizeof(T)) > kStreamBytes)
+    launch_pdl(qk_norm_rope_kernel<T, LANES, kHeadsEach, true>, blocks(kHeadsEach), dim3(kNormThreads), 0, stream, a);
+  else if (all * LANES > kManyLanes)
+    launch_pdl(qk_norm_rope_kernel<T, LANES, kHeadsEach, false>, blocks(kHeadsEach), dim3(kNormThreads), 0, stream, a);
   else
-    launch_pdl(qk_norm_rope_kernel<T, LANES, 1>, blocks(1), dim3(kNormThreads), 0, stream, a);
+    launch_pdl(qk_norm_rope_kernel<T, LANES, 1, false>, blocks(1), dim3(kNormThreads), 0, stream, a);
 }
 
 template <typename T>
@@ -228,8 +239,8 @@ int qk_norm_rope_impl(const void* q, const void* k, const void* v, long long q_s
                    aligned16(k_cache) && aligned16(v_cache) && (q_heads == 0 || rows16(q, n_tokens > 1 ? q_stride : 0)) &&
                    (kv_heads == 0 || (rows16(k, n_tokens > 1 ? k_stride : 0) && rows16(v, n_tokens > 1 ? v_stride : 0)));
   const long long heads = static_cast<long long>(q_heads) + 2ll * kv_heads;
-  if (heads > 0x3fffffff || heads * n_tokens > (1ll << 36))
-    return fail(PKV_E_UNSUPPORTED, "%s: %d tokens of %lld heads exceed one launch", fn, n_tokens, heads);
+  if (heads * n_tokens > 0x7fffffffll - kNormThreads)
+    return fail(PKV_E_UNSUPPORTED, "%s: %d tokens of %lld heads; at most 2^31 heads a call", fn, n_tokens, heads);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (vec && lanes == 4) launch_lanes<T, 4>(a, s);
   else if (vec && lanes == 8) launch_lanes<T, 8>(a, s);

@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const float sl2 = a.scale * kLog2e;
     // the two warps of a row's threads
     auto meet = [&] { asm volatile("bar.sync %0, 64;\n" ::"r"(1 + g * 4 + (warp & 3)) : "memory"); };
-    uint32_t e0 = 0, done = 0, finished = 0;                     // ring entries before this item; the group's key tiles; its commits to O_FULL awaited
+    uint32_t e0 = 0, done = 0, items = 0;                        // ring entries before this item; the group's key tiles and items
     for (int r = 0; r < n_items && !dead; ++r) {
       int pair, n, rows, kv_len;
       {
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           // arrived, were issued behind it; so is P's place.
           if constexpr (S::kLead > 1) {
             if (!opening) {
-              WAIT(BAR(O_FULL + g), finished & 1);
+              WAIT(BAR(O_FULL + g), (done & 1) ^ 1);
               tc::fence_after();
             }
           }
@@ -486,9 +486,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         } else if constexpr (S::kLead > 1) {
           // no row of this warp is the item's: it keeps step only
-          if (!opening) WAIT(BAR(O_FULL + g), finished & 1);
+          if (!opening) WAIT(BAR(O_FULL + g), (done & 1) ^ 1);
         }
-        if (S::kLead > 1 && !opening) ++finished;
         if (t + step >= n && valid < kTileKeys && (g == 0 || pair)) {
           // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring held.  Cleared
           // before the group's threads report the tile's P, so that 0 * x stays 0.
@@ -529,8 +528,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           to = reinterpret_cast<unsigned long long>(static_cast<T*>(a.out) + (static_cast<size_t>(token) * a.q_heads + head) * D + half * (D / 2));
         }
       }
-      WAIT(BAR(O_FULL + g), finished & 1);
-      ++finished;
+      WAIT(BAR(O_FULL + g), S::kLead > 1 ? (done & 1) ^ 1 : items & 1);
+      ++items;
       tc::fence_after();
       if (!working) continue;
       const float inv = 1.f / sum;

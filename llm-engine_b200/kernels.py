@@ -85,40 +85,52 @@ def launch_rope_store_kv(q, k, v, positions, cos_table, sin_table, slots, k_cach
     _lib.check(fn, st)
 
 
-def _rows(t, cols: int, what: str):
+# The checks below run once per call and layer: a few tenths of a microsecond per tensor, attributes looked up once.
+def _wrong(tensors, dtype, device: int, what: str):
+    """Raises the error of the first of `tensors` that is not a contiguous `dtype` tensor of CUDA device `device`."""
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError("paged-KV operators take CUDA tensors; there is no CPU path")
+        if t.dtype is not dtype:
+            raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+        if t.get_device() != device:
+            raise ValueError(f"{what} lie on different devices: {t.get_device()} and {device}")
+        if not t.is_contiguous():
+            raise ValueError("paged-KV operators take contiguous tensors")
+
+
+def _check(tensors, dtype, device: int, what: str) -> None:
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+            _wrong(tensors, dtype, device, what)
+
+
+def _rows(t, cols: int, dtype, device: int, n_rows: int, what: str):
     """(pointer, elements from one row to the next) of a [rows][cols] tensor whose rows may lie apart."""
-    if not t.is_cuda:
-        raise ValueError("paged-KV operators take CUDA tensors; there is no CPU path")
-    if t.dim() != 2 or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what} must be [rows][{cols}] with contiguous rows, not {tuple(t.shape)} with strides {tuple(t.stride())}")
+    if t.dtype is not dtype or t.get_device() != device:
+        _wrong((t,), dtype, device, what)
+    if t.dim() != 2 or t.size(1) != cols or t.size(0) < n_rows or (t.stride(1) != 1 and cols > 1):
+        raise ValueError(f"{what} must be [at least {n_rows}][{cols}] with contiguous rows, not {tuple(t.shape)} with strides {t.stride()}")
     return t.data_ptr(), t.stride(0)
 
 
-def _same(ref, *tensors):
-    """Every tensor has the element type of `ref` and lies on its device."""
-    for t in tensors:
-        if t.dtype != ref.dtype:
-            raise TypeError(f"element types differ: {t.dtype} and {ref.dtype}")
-    _on_device(ref, *tensors)
+_torch = None
+_one_device = False
 
 
-def _on_device(ref, *tensors):
-    for t in tensors:
-        if t.device != ref.device:
-            raise ValueError(f"tensors on different devices: {t.device} and {ref.device}")
+def _this_device(device: int):
+    """None if `device` is current, else a context in which it is (launches follow the current one)."""
+    global _torch, _one_device
+    if _torch is None:
+        import torch
+        _torch, _one_device = torch, torch.cuda.device_count() == 1
+        _stream(None)
+    return None if _one_device or _torch.cuda.current_device() == device else _torch.cuda.device(device)
 
 
-def _ints(*tensors):
-    import torch
-    for t in tensors:
-        if t.dtype != torch.int32:
-            raise TypeError(f"index arrays are int32, not {t.dtype}")
-
-
-def _device_of(t):
-    """A context in which t's device is the current one (launches and their streams follow it)."""
-    import torch
-    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+def _stream_of(stream, device: int):
+    """_stream for a device that is the current one."""
+    return _raw_stream(device) if stream is None else getattr(stream, "cuda_stream", stream)
 
 
 def launch_qk_norm_rope_store_kv(q, k, v, q_weight, k_weight, eps: float, positions, cos_table, sin_table, slots, q_out, k_cache,
@@ -128,27 +140,33 @@ def launch_qk_norm_rope_store_kv(q, k, v, q_weight, k_weight, eps: float, positi
     projection's output; q_out (contiguous) receives the rotated q.  Rows whose position is outside the tables are
     left alone, rows whose slot is outside the pools bring no K/V (padded steps)."""
     fn, call = _fn("pkv_qk_norm_rope_append_", k_cache)
+    device, dtype = k_cache.get_device(), k_cache.dtype
+    other = _this_device(device)
+    if other is not None:
+        with other:
+            return launch_qk_norm_rope_store_kv(q, k, v, q_weight, k_weight, eps, positions, cos_table, sin_table, slots, q_out, k_cache,
+                                                v_cache, n_tokens, q_heads, kv_heads, head_dim, stream)
     q_dim, kv_dim = q_heads * head_dim, kv_heads * head_dim
-    _same(k_cache, q, k, v, q_weight, k_weight, q_out, v_cache)
-    _on_device(k_cache, positions, cos_table, sin_table, slots)
-    _ints(positions, slots)
-    if cos_table.dtype != sin_table.dtype or "float32" not in str(cos_table.dtype):
-        raise TypeError("cos and sin tables are float32")
-    if cos_table.shape != sin_table.shape or cos_table.dim() != 2 or cos_table.shape[1] != head_dim // 2:
+    _check((q_weight, k_weight, q_out, k_cache, v_cache), dtype, device, "weights, q_out and pools")
+    _check((positions, slots), _torch.int32, device, "positions and slots")
+    _check((cos_table, sin_table), _torch.float32, device, "cos and sin tables")
+    max_positions, n_pool = cos_table.size(0), k_cache.numel()
+    if 2 * cos_table.numel() != max_positions * head_dim or sin_table.size(0) != max_positions or sin_table.numel() != cos_table.numel():
         raise ValueError(f"cos and sin tables must both be [positions][{head_dim // 2}]")
     if q_weight.numel() != head_dim or k_weight.numel() != head_dim:
         raise ValueError(f"norm weights must have head_dim = {head_dim} elements")
-    if min(q.shape[0], k.shape[0], v.shape[0], positions.numel(), slots.numel()) < n_tokens or q_out.numel() < n_tokens * q_dim:
+    if positions.numel() < n_tokens or slots.numel() < n_tokens or q_out.numel() < n_tokens * q_dim:
         raise ValueError(f"fewer rows than n_tokens = {n_tokens}")
-    n_slots = k_cache.numel() // max(kv_dim, 1)
-    if v_cache.numel() != k_cache.numel():
+    if v_cache.numel() != n_pool:
         raise ValueError("K and V pools differ in size")
-    (qp, qs), (kp, ks), (vp, vs) = _rows(q, q_dim, "q"), _rows(k, kv_dim, "k"), _rows(v, kv_dim, "v")
-    with _device_of(k_cache):
-        st = call(qp, kp, vp, qs, ks, vs, _ptr(q_weight), _ptr(k_weight), C.c_float(eps), _ptr(positions), _ptr(cos_table),
-                  _ptr(sin_table), cos_table.shape[0], _ptr(slots), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), n_slots, n_tokens,
-                  q_heads, kv_heads, head_dim, _stream(stream))
-    _lib.check(fn, st)
+    qp, qs = _rows(q, q_dim, dtype, device, n_tokens, "q")
+    kp, ks = _rows(k, kv_dim, dtype, device, n_tokens, "k")
+    vp, vs = _rows(v, kv_dim, dtype, device, n_tokens, "v")
+    st = call(qp, kp, vp, qs, ks, vs, q_weight.data_ptr(), k_weight.data_ptr(), eps, positions.data_ptr(), cos_table.data_ptr(),
+              sin_table.data_ptr(), max_positions, slots.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+              n_pool // max(kv_dim, 1), n_tokens, q_heads, kv_heads, head_dim, _stream_of(stream, device))
+    if st:
+        _lib.check(fn, st)
 
 
 def decode_workspace_bytes(n_tokens: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
@@ -314,6 +332,8 @@ class _SegmentPlan:
         n = max(int(L.pkv_segment_staging_bytes(n_tokens, q_heads, kv_heads)), 256)
         self.staging = torch.empty(n, dtype=torch.uint8, pin_memory=torch.cuda.is_available())
         self.plan = _lib.SegmentPlan()
+        self._plan_ref = C.byref(self.plan)
+        self._device, self._ws = workspace.get_device(), (_ptr(workspace), workspace.numel())
         self._out_elems = n_tokens * q_heads * head_dim
 
     def _geometry(self):
@@ -325,19 +345,27 @@ class _SegmentPlan:
         if image:
             st = getattr(L, name + "_image")(*args, *where, self.workspace.numel(), C.byref(self.plan))
         else:
-            with _device_of(self.workspace):
+            with _this_device(self.workspace.get_device()) or contextlib.nullcontext():
                 st = getattr(L, name)(*args, *where, _ptr(self.workspace), self.workspace.numel(), _stream(stream), C.byref(self.plan))
         _lib.check(name, st)
         self.plan.num_blocks = self.num_blocks
 
-    def _check(self, q, k_cache, v_cache, out, *ints):
-        for t in (q, k_cache, v_cache, out):
-            if t.dtype != self.dtype:
-                raise TypeError(f"the plan is for {self.dtype}, not {t.dtype}")
+    def _run(self, op, q, k_cache, v_cache, out, ints, scale, stream):
+        """One attention call: pointers of q, the pools, the index arrays and out, in the order of the C signatures."""
+        device = self._device
+        other = _this_device(device)
+        if other is not None:
+            with other:
+                return self._run(op, q, k_cache, v_cache, out, ints, scale, stream)
+        _check((q, k_cache, v_cache, out), self.dtype, device, "q, out and pools")
+        _check(ints, _torch.int32, device, "index arrays")
         if q.numel() < self._out_elems or out.numel() < self._out_elems:
             raise ValueError(f"q and out must have {self.n_tokens} rows of {self.q_heads} heads")
-        _on_device(self.workspace, q, k_cache, v_cache, out, *ints)
-        _ints(*ints)
+        fn, call = _fn(op, k_cache)
+        st = call(self._plan_ref, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *[t.data_ptr() for t in ints], out.data_ptr(), scale,
+                  *self._ws, _stream_of(stream, device))
+        if st:
+            _lib.check(fn, st)
 
 
 class CrossPlan(_SegmentPlan):
@@ -375,12 +403,7 @@ class CrossPlan(_SegmentPlan):
     def attention(self, q, k_cache, v_cache, block_tables, table_offset, out, scale: float, stream=None) -> None:
         """out[t] = softmax(q[t] K^T scale) V over all keys of t's sequence; zero where it has none.  table_offset[s] is the
         start of sequence s's table."""
-        self._check(q, k_cache, v_cache, out, block_tables, table_offset)
-        fn, call = _fn("pkv_cross_attn_", k_cache)
-        with _device_of(k_cache):
-            st = call(C.byref(self.plan), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), _ptr(table_offset), _ptr(out),
-                      scale, _ptr(self.workspace), self.workspace.numel(), _stream(stream))
-        _lib.check(fn, st)
+        self._run("pkv_cross_attn_", q, k_cache, v_cache, out, (block_tables, table_offset), scale, stream)
 
 
 class PrefixPlan(_SegmentPlan):
@@ -413,12 +436,7 @@ class PrefixPlan(_SegmentPlan):
 
     def attention(self, q, k_cache, v_cache, block_tables, table_offset, token_seq, out, scale: float, stream=None) -> None:
         """As launch_attention_decode with the step's whole tables."""
-        self._check(q, k_cache, v_cache, out, block_tables, table_offset, token_seq)
-        fn, call = _fn("pkv_prefix_attn_", k_cache)
-        with _device_of(k_cache):
-            st = call(C.byref(self.plan), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), _ptr(table_offset), _ptr(token_seq),
-                      _ptr(out), scale, _ptr(self.workspace), self.workspace.numel(), _stream(stream))
-        _lib.check(fn, st)
+        self._run("pkv_prefix_attn_", q, k_cache, v_cache, out, (block_tables, table_offset, token_seq), scale, stream)
 
 
 def launch_attention_prefill(q, k_cache, v_cache, block_tables, table_offset, q_start, q_len, ctx_len, out,

@@ -91,7 +91,8 @@ def check(torch, pkv, d, n, qh, kvh, hd, eps, dtype, **kw):
     # q_heads, kv_heads, head_dim, tokens
     (14, 2, 64, 1), (14, 2, 64, 33), (32, 8, 128, 257), (4, 1, 256, 9),
     (32, 4, 64, 4400),            # several heads a lane
-    (5, 3, 128, 5000),            # heads that do not divide by them
+    (5, 4, 128, 5000),            # heads that do not divide by them
+    (31, 9, 128, 6700),           # more rows than fit L2
     (3, 2, 32, 20), (6, 3, 40, 17), (4, 4, 6, 5), (1, 1, 2, 3), (2, 1, 96, 40),
 ])
 def test_against_formula(pkv, torch_cuda, dtype, packed, geom):

@@ -395,21 +395,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // the two warps of a row's threads
     auto meet = [&] { asm volatile("bar.sync %0, 64;\n" ::"r"(1 + g * 4 + (warp & 3)) : "memory"); };
     uint32_t e0 = 0, done = 0, items = 0;                        // ring entries before this item; the group's key tiles and items
-    for (int r = 0; r < n_items && !dead; ++r) {
-      int pair, n, rows, kv_len;
+    // (A thread whose wait has run out goes on to the end without waiting: its partner meets it at every tile.)
+    for (int r = 0; r < n_items; ++r) {
+      int pair, n, kv_len;
+      bool working;                                              // some row of this warp is the item's
       {
         const TileItem it = load_tile(tiles + r);
         pair = it.flags & kPair ? 1 : 0;
         n = (it.kv_len + kTileKeys - 1) / kTileKeys << pair;
-        rows = it.n_tok * a.group;
         kv_len = it.kv_len;
+        const int rows = it.n_tok * a.group;
+        e0 += 2 * n;
+        if (g == 1 && !pair && rows <= 128) continue;
+        working = (pair ? 0 : g * 128) + (warp & 3) * 32 < rows;
       }
       const int step = 1 + pair;
-      e0 += 2 * n;
-      const uint32_t last_v = e0 - 1 - pair + (pair & g);        // ring entry of the group's last V tile
-      const int row = pair ? r_in : g * 128 + r_in;   // row of the item
-      if (g == 1 && !pair && rows <= 128) continue;
-      const bool working = (row & ~31) < rows;                   // some row of this warp is the item's
       float m_used = -INFINITY;
       float2 l = both(0.f);
       for (int t = pair & g; t < n; t += step, ++done) {
@@ -491,6 +491,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (t + step >= n && valid < kTileKeys && (g == 0 || pair)) {
           // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring held.  Cleared
           // before the group's threads report the tile's P, so that 0 * x stays 0.
+          const uint32_t last_v = e0 - 1 - pair + (pair & g);  // ring entry of the group's last V tile
           WAIT(BAR(KV_FULL + last_v % NS), (last_v / NS) & 1);
           if (r_in >= valid && half < S::kHalves) {
             unsigned char* v = base_ptr + S::kRing + (last_v % NS) * S::kTile + half * kBlockBytes + r_in * 128;
@@ -517,6 +518,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       asm volatile("" : "+l"(again));
       const TileItem it = load_tile(again);
       const bool partial = it.part >= 0;
+      const int rows = it.n_tok * a.group, row = pair ? r_in : g * 128 + r_in;
       unsigned long long to = 0;
       if (row < rows) {
         if (partial) {
@@ -533,27 +535,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::fence_after();
       if (!working) continue;
       const float inv = 1.f / sum;
+      if (partial) {
 #pragma unroll 1
-      for (int c = 0; c < D / 2; c += 32) {
-        uint32_t v[32];
-        tc::ld32(t_o + c, v);
-        tc::wait_ld();
-        if (partial) {                                         // 128 bytes of every lane's row: whole lines
-          transpose<8>(v, lane);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const unsigned long long row_to = __shfl_sync(0xffffffffu, to, (lane & 24) + i);
-            if (row_to) *reinterpret_cast<uint4*>(row_to + c * 4 + (lane & 7) * 16) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          }
-        } else {                                               // 64 bytes
-          uint32_t x[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = pack2<T>(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
-          transpose<4>(x, lane);
+        for (int c = 0; c < D / 2; c += 16) {
+          uint32_t v[16];
+          tc::ld16(t_o + c, v);
+          tc::wait_ld();
+          transpose<4>(v, lane);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const unsigned long long row_to = __shfl_sync(0xffffffffu, to, (lane & 28) + i);
-            if (row_to) *reinterpret_cast<uint4*>(row_to + c * 2 + (lane & 3) * 16) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            if (row_to) *reinterpret_cast<uint4*>(row_to + c * 4 + (lane & 3) * 16) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < D / 2; c += 16) {
+          uint32_t v[16], x[8];
+          tc::ld16(t_o + c, v);
+          tc::wait_ld();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = pack2<T>(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
+          transpose<2>(x, lane);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const unsigned long long row_to = __shfl_sync(0xffffffffu, to, (lane & 30) + i);
+            if (row_to) *reinterpret_cast<uint4*>(row_to + c * 2 + (lane & 1) * 16) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
           }
         }
       }

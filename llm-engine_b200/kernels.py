@@ -109,9 +109,10 @@ def _rows(t, cols: int, dtype, device: int, n_rows: int, what: str):
     """(pointer, elements from one row to the next) of a [rows][cols] tensor whose rows may lie apart."""
     if t.dtype is not dtype or t.get_device() != device:
         _wrong((t,), dtype, device, what)
-    if t.dim() != 2 or t.size(1) != cols or t.size(0) < n_rows or (t.stride(1) != 1 and cols > 1):
-        raise ValueError(f"{what} must be [at least {n_rows}][{cols}] with contiguous rows, not {tuple(t.shape)} with strides {t.stride()}")
-    return t.data_ptr(), t.stride(0)
+    shape, stride = t.shape, t.stride()      # (size(0) and stride(0) take twice as long)
+    if len(shape) != 2 or shape[1] != cols or shape[0] < n_rows or (stride[1] != 1 and cols > 1):
+        raise ValueError(f"{what} must be [at least {n_rows}][{cols}] with contiguous rows, not {tuple(shape)} with strides {stride}")
+    return t.data_ptr(), stride[0]
 
 
 _torch = None
@@ -150,8 +151,8 @@ def launch_qk_norm_rope_store_kv(q, k, v, q_weight, k_weight, eps: float, positi
     _check((q_weight, k_weight, q_out, k_cache, v_cache), dtype, device, "weights, q_out and pools")
     _check((positions, slots), _torch.int32, device, "positions and slots")
     _check((cos_table, sin_table), _torch.float32, device, "cos and sin tables")
-    max_positions, n_pool = cos_table.size(0), k_cache.numel()
-    if 2 * cos_table.numel() != max_positions * head_dim or sin_table.size(0) != max_positions or sin_table.numel() != cos_table.numel():
+    tables, n_pool = cos_table.shape, k_cache.numel()
+    if tables != sin_table.shape or len(tables) != 2 or 2 * tables[1] != head_dim:
         raise ValueError(f"cos and sin tables must both be [positions][{head_dim // 2}]")
     if q_weight.numel() != head_dim or k_weight.numel() != head_dim:
         raise ValueError(f"norm weights must have head_dim = {head_dim} elements")
@@ -163,7 +164,7 @@ def launch_qk_norm_rope_store_kv(q, k, v, q_weight, k_weight, eps: float, positi
     kp, ks = _rows(k, kv_dim, dtype, device, n_tokens, "k")
     vp, vs = _rows(v, kv_dim, dtype, device, n_tokens, "v")
     st = call(qp, kp, vp, qs, ks, vs, q_weight.data_ptr(), k_weight.data_ptr(), eps, positions.data_ptr(), cos_table.data_ptr(),
-              sin_table.data_ptr(), max_positions, slots.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+              sin_table.data_ptr(), tables[0], slots.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
               n_pool // max(kv_dim, 1), n_tokens, q_heads, kv_heads, head_dim, _stream_of(stream, device))
     if st:
         _lib.check(fn, st)

@@ -299,85 +299,84 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       __syncwarp();
     } else if (warp == kIssuer) {
       after_previous();
-      if (lane == 0) {
-        uint32_t e = 0, done = 0, read = 0;                        // ring entries; bit g: parity of group g's P and S taken
-        for (int r = 0; r < n_items && !dead; ++r) {
-          const TileItem it = load_tile(tiles + r);
-          const int pair = it.flags & kPair ? 1 : 0, n = (it.kv_len + kTileKeys - 1) / kTileKeys << pair;
-          const int last = it.n_tok * a.group > 128 ? 1 : 0, qb = r % S::kQBufs;   // last group, if both take every tile; buffer of Q
-          // waits for the ring entry and returns where it lies
-          auto full = [&](uint32_t entry) {
-            WAIT(BAR(KV_FULL + entry % NS), (entry / NS) & 1);
-            tc::fence_after();
-            return ring + (entry % NS) * S::kTile;
-          };
-          // Descriptors differ in their low word only.  It is made opaque at every call: the compiler would otherwise keep two
-          // dozen of them per group at hand, spilled, and a product waited 200 cycles for its own.
-          auto scores = [&](int g, uint32_t k_addr, bool read_first) {
-            if (S::kLead > 1) {
-              if (read_first) {
-                WAIT(BAR(S_READ + g), (read >> g) & 1);
-                tc::fence_after();
-              }
-              // counted by tiles: the phase of an item's last tile, which nobody waits for, is over when its P is there
-              if (read_first) read ^= 1u << g;
-            }
-            uint32_t q_lo = (base + qb * S::kQ + g * kBlockBytes) >> 4, k_lo = k_addr >> 4;
-            const uint32_t d = tmem + g * kGroupCols;
-            asm volatile("" : "+r"(q_lo), "+r"(k_lo));
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-              tc::mma_ss(d, tc::operand_at(q_lo + (ks >> 2) * (S::kQHalf >> 4) + (ks & 3) * 2),
-                         tc::operand_at(k_lo + (ks >> 2) * (kBlockBytes >> 4) + (ks & 3) * 2), kInstrQK, ks > 0);
-            }
-            tc::commit(BAR(S_FULL + g));
-          };
-          // Products of one thread run in order: where P lies over S, the group's next scores overwrite it behind these.
-          auto values = [&](int g, uint32_t v_addr, bool first, bool final) {
-            WAIT(BAR(P_FULL + g), (done >> g) & 1);
-            tc::fence_after();
-            uint32_t v_lo = v_addr >> 4, t = tmem + g * kGroupCols;
-            asm volatile("" : "+r"(v_lo), "+r"(t));
-#pragma unroll
-            for (int kk = 0; kk < kTileKeys / 16; ++kk)
-              tc::mma_ts(t + kColO, t + S::kColP + kk * 8, tc::operand_at(v_lo + kk * (2048 >> 4), kBlockBytes), kInstrPV, !(first && kk == 0));
-            done ^= 1u << g;
-            if (final && S::kLead > 1) read ^= 1u << g;              // see scores()
-            if (final || S::kLead > 1) tc::commit(BAR(O_FULL + g));
-          };
-          auto free_entry = [&](uint32_t entry) { tc::commit(BAR(KV_EMPTY + entry % NS)); };
-          WAIT(BAR(Q_FULL + qb), (r / S::kQBufs) & 1);
+      const uint32_t one = lane == 0 ? 1u : 0u;
+      uint32_t e = 0, done = 0, read = 0;                        // ring entries; bit g: parity of group g's P and S taken
+      for (int r = 0; r < n_items && !dead; ++r) {
+        const TileItem it = load_tile(tiles + r);
+        const int pair = it.flags & kPair ? 1 : 0, n = (it.kv_len + kTileKeys - 1) / kTileKeys << pair;
+        const int last = it.n_tok * a.group > 128 ? 1 : 0, qb = r % S::kQBufs;   // last group, if both take every tile; buffer of Q
+        // waits for the ring entry and returns where it lies
+        auto full = [&](uint32_t entry) {
+          WAIT(BAR(KV_FULL + entry % NS), (entry / NS) & 1);
           tc::fence_after();
-          const int lead = min(n, S::kLead << pair);
-          for (int t = 0; t < lead; ++t, ++e) {
-            const uint32_t k_addr = full(e);
-            if (pair) {
-              scores(t & 1, k_addr, t >= 2);
-            } else {
-              for (int g = 0; g <= last; ++g) scores(g, k_addr, t >= 1);
+          return ring + (entry % NS) * S::kTile;
+        };
+        // Descriptors differ in their low word only.  It is made opaque at every call: the compiler would otherwise keep two
+        // dozen of them per group at hand, spilled, and a product waited 200 cycles for its own.
+        auto scores = [&](int g, uint32_t k_addr, bool read_first) {
+          if (S::kLead > 1) {
+            if (read_first) {
+              WAIT(BAR(S_READ + g), (read >> g) & 1);
+              tc::fence_after();
             }
-            free_entry(e);
-            if (t == n - 1) tc::commit(BAR(Q_EMPTY + qb));
+            // counted by tiles: the phase of an item's last tile, which nobody waits for, is over when its P is there
+            if (read_first) read ^= 1u << g;
           }
-          for (int t = 0; t < n && !dead; ++t) {
-            const int kt = t + lead;
-            const bool more = kt < n;
-            const uint32_t v_addr = full(e);
-            uint32_t k_addr = 0;
-            const int g0 = pair ? t & 1 : 0, g1 = pair ? t & 1 : last;
-            for (int g = g0; g <= g1; ++g) {
-              values(g, v_addr, t <= pair, t + 1 + pair >= n);
-              if (g == g1) free_entry(e);
-              if (!more) continue;
-              if (g == g0) k_addr = full(e + 1);
-              scores(g, k_addr, true);
-              if (g == g1) {
-                free_entry(e + 1);
-                if (kt == n - 1) tc::commit(BAR(Q_EMPTY + qb));
-              }
+          uint32_t q_lo = (base + qb * S::kQ + g * kBlockBytes) >> 4, k_lo = k_addr >> 4;
+          const uint32_t d = tmem + g * kGroupCols;
+          asm volatile("" : "+r"(q_lo), "+r"(k_lo));
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            tc::mma_ss(d, tc::operand_at(q_lo + (ks >> 2) * (S::kQHalf >> 4) + (ks & 3) * 2),
+                       tc::operand_at(k_lo + (ks >> 2) * (kBlockBytes >> 4) + (ks & 3) * 2), kInstrQK, ks > 0, one);
+          }
+          tc::commit(BAR(S_FULL + g), one);
+        };
+        // Products of one thread run in order: where P lies over S, the group's next scores overwrite it behind these.
+        auto values = [&](int g, uint32_t v_addr, bool first, bool final) {
+          WAIT(BAR(P_FULL + g), (done >> g) & 1);
+          tc::fence_after();
+          uint32_t v_lo = v_addr >> 4, t = tmem + g * kGroupCols;
+          asm volatile("" : "+r"(v_lo), "+r"(t));
+#pragma unroll
+          for (int kk = 0; kk < kTileKeys / 16; ++kk)
+            tc::mma_ts(t + kColO, t + S::kColP + kk * 8, tc::operand_at(v_lo + kk * (2048 >> 4), kBlockBytes), kInstrPV, !(first && kk == 0), one);
+          done ^= 1u << g;
+          if (final && S::kLead > 1) read ^= 1u << g;              // see scores()
+          if (final || S::kLead > 1) tc::commit(BAR(O_FULL + g), one);
+        };
+        auto free_entry = [&](uint32_t entry) { tc::commit(BAR(KV_EMPTY + entry % NS), one); };
+        WAIT(BAR(Q_FULL + qb), (r / S::kQBufs) & 1);
+        tc::fence_after();
+        const int lead = min(n, S::kLead << pair);
+        for (int t = 0; t < lead; ++t, ++e) {
+          const uint32_t k_addr = full(e);
+          if (pair) {
+            scores(t & 1, k_addr, t >= 2);
+          } else {
+            for (int g = 0; g <= last; ++g) scores(g, k_addr, t >= 1);
+          }
+          free_entry(e);
+          if (t == n - 1) tc::commit(BAR(Q_EMPTY + qb), one);
+        }
+        for (int t = 0; t < n && !dead; ++t) {
+          const int kt = t + lead;
+          const bool more = kt < n;
+          const uint32_t v_addr = full(e);
+          uint32_t k_addr = 0;
+          const int g0 = pair ? t & 1 : 0, g1 = pair ? t & 1 : last;
+          for (int g = g0; g <= g1; ++g) {
+            values(g, v_addr, t <= pair, t + 1 + pair >= n);
+            if (g == g1) free_entry(e);
+            if (!more) continue;
+            if (g == g0) k_addr = full(e + 1);
+            scores(g, k_addr, true);
+            if (g == g1) {
+              free_entry(e + 1);
+              if (kt == n - 1) tc::commit(BAR(Q_EMPTY + qb), one);
             }
-            e += more ? 2 : 1;
           }
+          e += more ? 2 : 1;
         }
       }
       __syncwarp();

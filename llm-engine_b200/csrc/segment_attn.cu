@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&vmap) : "memory");
       }
-      const int box_rows = 1 << a.box_log2, boxes = kTileKeys >> a.box_log2;
+      const int box_rows = 1 << a.box_log2, boxes = kTileKeys >> a.box_log2, per_batch_log2 = 5 - (7 - a.box_log2);   // key tiles of a batch
       for (int r = 0; r < n_items && !dead; ++r) {
         const TileItem it = load_tile(tiles + r);
         const int pair = it.flags & kPair ? 1 : 0, n = (it.kv_len + kTileKeys - 1) / kTileKeys << pair, end = it.kv_begin + it.kv_len;
@@ -228,17 +228,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int lead = min(n, S::kLead << pair), turns = 2 * (n - lead);
         auto is_v = [&](int i) { return i >= lead && !(i - lead < turns && ((i - lead) & 1)); };
         auto tile_of = [&](int i) { return i < lead ? i : i - lead >= turns ? i - n : ((i - lead) & 1) ? lead + ((i - lead) >> 1) : (i - lead) >> 1; };
-        auto row_of = [&](int i) {           // pool row of this lane's box
-          const int pos = it.kv_begin + (tile_of(i) >> pair) * kTileKeys + (lane << a.box_log2);
-          if (lane >= boxes || pos >= end) return 0;
+        // Pool rows of the item's boxes, a batch of 32 at a time, a lane each: the look-up through the block table takes longer
+        // than a tile, and its batches are asked for one ahead.  V follows K by fewer tiles than a batch has.
+        auto batch = [&](int b) {
+          const int pos = it.kv_begin + ((b * 32 + lane) << a.box_log2);
+          if (pos >= end) return 0;
           return (__ldg(tbl + (pos >> a.bs_log2)) << a.bs_log2) + (pos & (a.block_size - 1));
         };
-        int y = row_of(0);
+        int at = 0, before = 0, here = batch(0), ahead = batch(1);
+        auto row_of = [&](int kt) {          // pool row of this lane's box of a key tile
+          const int b = kt >> per_batch_log2;
+          if (b > at) {
+            before = here;
+            here = ahead;
+            ahead = batch(++at + 1);
+          }
+          return __shfl_sync(0xffffffffu, b == at ? here : before, ((kt << (5 - per_batch_log2)) + (lane & (boxes - 1))) & 31);
+        };
         if (first) after_previous();
         first = false;
         for (int i = 0; i < 2 * n; ++i, ++e) {
-          const int y_next = i + 1 < 2 * n ? row_of(i + 1) : 0;
-          const int t = tile_of(i), st = static_cast<int>(e % NS), left = it.kv_len - (t >> pair) * kTileKeys;
+          const int t = tile_of(i), y = row_of(t >> pair), st = static_cast<int>(e % NS), left = it.kv_len - (t >> pair) * kTileKeys;
           const int x = (it.kvh + (t & pair)) * D;
           const int valid = min(boxes, (left + box_rows - 1) >> a.box_log2);
           if (lane == 0) {
@@ -254,7 +264,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (int h = 0; h < S::kHalves; ++h) tma_load_2d(dst + h * kBlockBytes, map, x + h * 64, y, BAR(KV_FULL + st));
           }
           __syncwarp();
-          y = y_next;
         }
       }
       // whatever this warp has sent for has arrived before the block leaves

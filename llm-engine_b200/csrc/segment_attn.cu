@@ -14,7 +14,8 @@
 //                   tile of both groups at head_dim 128, 3,300 at 64.)  P goes back to tensor memory as 16-bit pairs, the A
 //                   operand of the second product.  O stays there and is rescaled only when a row's maximum has grown by
 //                   more than 2^8.
-//   warp 16         TMA: K and V tiles through the block table into a ring (boxes of up to 128 slots x 128 bytes).
+//   warps 16, 19    TMA: K, V tiles through the block table into one ring (boxes of up to 128 slots x 128 bytes).  Two, because a warp
+//                   sends a 16-slot box every 170 cycles, half as fast as two heads of 64 dims eat them.
 //   warp 17         issues the products, one thread: S = Q K^T and O += P V of both groups in turns.
 //   warp 18         TMA: the next item's rows of Q, a box for each token's heads, or for several consecutive tokens'.
 //
@@ -55,7 +56,7 @@ namespace {
 constexpr int kTileThreads = 640;
 // Registers a thread of the softmax warps and of the others; launched with 96 each (4 x 104 + 64 <= 5 x 96).
 constexpr int kSoftmaxRegs = 104, kOtherRegs = 64;
-constexpr int kProducer = 16, kIssuer = 17, kRowsLoader = 18;   // the 20th warp idles: registers are split by fours
+constexpr int kProducer = 16, kIssuer = 17, kRowsLoader = 18, kProducerV = 19;
 constexpr int kBlockBytes = 128 * 128;                   // 128 rows x 64 16-bit elements: one operand block
 constexpr uint32_t kGroupCols = 256, kColO = 128;        // tensor memory of a group: S, then O ...
 constexpr float kRescale = 8.f;                          // in log2 units: P stays below 2^8
@@ -211,15 +212,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   if (warp >= kProducer) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
-    if (warp == kProducer) {
+    if (warp == kProducer || warp == kProducerV) {
       // The entries of the ring for an item of n key tiles, in the order the products use them: K of the first `lead` tiles,
       // then V0 K(lead) V1 K(lead + 1) ..., and the last V.
-      uint32_t e = 0;
+      const bool for_v = warp == kProducerV;
+      const CUtensorMap* map = for_v ? &vmap : &kmap;
+      uint32_t e = 0, mine = 0, parity = 0;                        // ring entries; stages this warp filled last, and in which phase
       bool first = true;
-      if (lane == 0) {
-        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&kmap) : "memory");
-        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&vmap) : "memory");
-      }
+      if (lane == 0) asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
       const int box_rows = 1 << a.box_log2, boxes = kTileKeys >> a.box_log2, per_batch_log2 = 5 - (7 - a.box_log2);   // key tiles of a batch
       for (int r = 0; r < n_items && !dead; ++r) {
         const TileItem it = load_tile(tiles + r);
@@ -229,26 +229,30 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         auto is_v = [&](int i) { return i >= lead && !(i - lead < turns && ((i - lead) & 1)); };
         auto tile_of = [&](int i) { return i < lead ? i : i - lead >= turns ? i - n : ((i - lead) & 1) ? lead + ((i - lead) >> 1) : (i - lead) >> 1; };
         // Pool rows of the item's boxes, a batch of 32 at a time, a lane each: the look-up through the block table takes longer
-        // than a tile, and its batches are asked for one ahead.  V follows K by fewer tiles than a batch has.
+        // than a tile, and its batches are asked for one ahead.
         auto batch = [&](int b) {
           const int pos = it.kv_begin + ((b * 32 + lane) << a.box_log2);
           if (pos >= end) return 0;
           return (__ldg(tbl + (pos >> a.bs_log2)) << a.bs_log2) + (pos & (a.block_size - 1));
         };
-        int at = 0, before = 0, here = batch(0), ahead = batch(1);
+        int at = 0, here = batch(0), ahead = batch(1);
         auto row_of = [&](int kt) {          // pool row of this lane's box of a key tile
           const int b = kt >> per_batch_log2;
           if (b > at) {
-            before = here;
             here = ahead;
             ahead = batch(++at + 1);
           }
-          return __shfl_sync(0xffffffffu, b == at ? here : before, ((kt << (5 - per_batch_log2)) + (lane & (boxes - 1))) & 31);
+          return __shfl_sync(0xffffffffu, here, ((kt << (5 - per_batch_log2)) + (lane & (boxes - 1))) & 31);
         };
         if (first) after_previous();
         first = false;
         for (int i = 0; i < 2 * n; ++i, ++e) {
-          const int t = tile_of(i), y = row_of(t >> pair), st = static_cast<int>(e % NS), left = it.kv_len - (t >> pair) * kTileKeys;
+          const int st = static_cast<int>(e % NS);
+          if (is_v(i) != for_v) {
+            mine &= ~(1u << st);
+            continue;
+          }
+          const int t = tile_of(i), y = row_of(t >> pair), left = it.kv_len - (t >> pair) * kTileKeys;
           const int x = (it.kvh + (t & pair)) * D;
           const int valid = min(boxes, (left + box_rows - 1) >> a.box_log2);
           if (lane == 0) {
@@ -257,9 +261,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           dead = __shfl_sync(0xffffffffu, dead ? 1 : 0, 0) != 0;
           if (dead) break;
+          mine |= 1u << st;
+          parity = (parity & ~(1u << st)) | ((e / NS) & 1) << st;
           if (lane < valid) {
             const uint32_t dst = ring + st * S::kTile + (lane << a.box_log2) * 128;
-            const CUtensorMap* map = is_v(i) ? &vmap : &kmap;
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h) tma_load_2d(dst + h * kBlockBytes, map, x + h * 64, y, BAR(KV_FULL + st));
           }
@@ -268,7 +273,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       // whatever this warp has sent for has arrived before the block leaves
       if (lane == 0) {
-        for (uint32_t i = e > NS ? e - NS : 0; i < e; ++i) mbar_wait(BAR(KV_FULL + i % NS), (i / NS) & 1);
+        for (int st = 0; st < NS; ++st)
+          if (mine >> st & 1) mbar_wait(BAR(KV_FULL + st), parity >> st & 1);
       }
       __syncwarp();
     } else if (warp == kRowsLoader) {
@@ -389,8 +395,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
       __syncwarp();
-    } else {
-      after_previous();
     }
   } else {
     after_previous();

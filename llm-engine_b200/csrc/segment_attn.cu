@@ -31,6 +31,7 @@
 // Blocks are persistent, one on an SM, each with a list of items of its own.  Every wait is bounded: one that runs
 // out sets bit 32 of the error word and the block winds down.
 #include <algorithm>
+#include <cstdlib>
 #include <new>
 #include <type_traits>
 #include <vector>
@@ -61,8 +62,7 @@ constexpr int kBlockBytes = 128 * 128;                   // 128 rows x 64 16-bit
 constexpr uint32_t kGroupCols = 256, kColO = 128;        // tensor memory of a group: S, then O ...
 constexpr float kRescale = 8.f;                          // in log2 units: P stays below 2^8
 constexpr int kBoxRows = 64;                             // rows of Q, at most, that a box of several tokens brings
-constexpr int kMinTileTokens = 4;                        // sequences with fewer tokens go to the decode kernels
-constexpr int kMinPrefixTokens = 2;                      // batches of fewer tokens behind the prefix, too
+constexpr int kMinTileTokens = 2, kManyTileTokens = 32;  // sequences with fewer tokens always go to the decode kernels, with as many never
 
 template <int D> struct TileSmem {
   static constexpr int kHalves = D / 64;
@@ -751,6 +751,13 @@ int check_geometry(const char* fn, const SegmentGeometry& g) {
 
 enum Kind { kCross = 1, kPrefix = 2 };
 
+// PKV_SEGMENT_TILES=1: whatever the tile kernel can take goes to it, =0: nothing does; else what is reckoned to take least.
+// Read at every planning call (a measurement and testing aid).
+int tiles_asked() {
+  const char* e = std::getenv("PKV_SEGMENT_TILES");
+  return e && (*e == '0' || *e == '1') ? *e - '0' : -1;
+}
+
 int write_image(const char* fn, Kind kind, const SegmentGeometry& g, const SegmentLists& l, const std::vector<int>& seq, const std::vector<int>& pos,
                 bool cluster, void* h_staging, size_t staging_bytes, size_t workspace_bytes, pkv_segment_plan* plan) {
   const SegmentOffsets o = segment_offsets(g, SegmentCounts{l.row_token.size(), l.items.size(), l.first.size(), l.list_first.size(), l.tiles.size(),
@@ -805,30 +812,55 @@ int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* 
   if (!q_len || !kv_len || !h_staging) return fail(PKV_E_ARG, "%s: null pointer", fn);
   int st = check_geometry(fn, g);
   if (st != PKV_OK) return st;
-  std::vector<int> seq(g.n_tokens, -1), pos(g.n_tokens, -1), empty;
-  std::vector<Segment> segs;
-  std::vector<OwnRange> own;
-  SegmentLists l;
+  std::vector<int> seq(g.n_tokens, -1), pos(g.n_tokens, -1), empty, start(n_seqs);
   long long next = 0;
-  int listed = 0;
+  int listed = 0, most = 0;
   for (int s = 0; s < n_seqs; ++s) {
-    const long long start = q_start ? q_start[s] : next;
-    if (q_len[s] < 0 || kv_len[s] < 0 || start < 0 || start + q_len[s] > g.n_tokens)
-      return fail(PKV_E_ARG, "%s: sequence %d has rows %lld .. + %d of %d and %d keys", fn, s, start, q_len[s], g.n_tokens, kv_len[s]);
-    next = start + q_len[s];
+    const long long at = q_start ? q_start[s] : next;
+    if (q_len[s] < 0 || kv_len[s] < 0 || at < 0 || at + q_len[s] > g.n_tokens)
+      return fail(PKV_E_ARG, "%s: sequence %d has rows %lld .. + %d of %d and %d keys", fn, s, at, q_len[s], g.n_tokens, kv_len[s]);
+    next = at + q_len[s];
+    start[s] = static_cast<int>(at);
     listed += q_len[s];
-    const bool tiled = kv_len[s] > 0 && g.tiles() && q_len[s] >= kMinTileTokens;
-    if (tiled) segs.push_back(Segment{static_cast<int>(l.row_token.size()), q_len[s], kv_len[s], ~s});
-    for (int i = 0; i < q_len[s]; ++i) {
-      const int t = static_cast<int>(start) + i;
+    if (kv_len[s] > 0) most = std::max(most, q_len[s]);
+    for (int t = start[s]; t < next; ++t) {
       if (seq[t] >= 0) return fail(PKV_E_ARG, "%s: row %d belongs to sequences %d and %d", fn, t, seq[t], s);
       seq[t] = s;
       pos[t] = kv_len[s] - 1;
       if (kv_len[s] == 0) empty.push_back(t);
-      else if (tiled) l.row_token.push_back(t);
-      else own.push_back(OwnRange{t, 0, kv_len[s]});
     }
   }
+  // Sequences of at least `fewest` tokens go to the tile kernel, the others to the decode kernels, which fetch the keys anew for
+  // every token.  The number for which the step is reckoned to take least.
+  std::vector<Segment> segs;
+  std::vector<OwnRange> own;
+  SegmentLists l;
+  auto split = [&](int fewest) {
+    segs.clear();
+    own.clear();
+    l.row_token.clear();
+    for (int s = 0; s < n_seqs; ++s) {
+      if (q_len[s] == 0 || kv_len[s] == 0) continue;
+      const bool tiled = g.tiles() && q_len[s] >= fewest;
+      if (tiled) segs.push_back(Segment{static_cast<int>(l.row_token.size()), q_len[s], kv_len[s], ~s});
+      for (int t = start[s]; t < start[s] + q_len[s]; ++t) {
+        if (tiled) l.row_token.push_back(t);
+        else own.push_back(OwnRange{t, 0, kv_len[s]});
+      }
+    }
+  };
+  const int asked = tiles_asked();
+  int fewest = asked == 1 ? 1 : asked == 0 ? 0x7fffffff : kMinTileTokens;
+  if (g.tiles() && asked < 0) {
+    long long least = -1;
+    for (int f = kMinTileTokens; f <= kManyTileTokens; f = f < 4 ? f + 1 : f * 2) {
+      split(f);
+      const long long c = step_cycles(segs, own, l.row_token, g, decode_sms(), false);
+      if (least < 0 || c < least) { least = c; fewest = f; }
+      if (segs.empty()) break;
+    }
+  }
+  split(fewest);
   list_segments(segs, own, empty, g, decode_sms(), false, l);
   return write_image(fn, kCross, g, l, seq, pos, segs.empty() && empty.empty() && listed == g.n_tokens, h_staging, staging_bytes, workspace_bytes, plan);
 }
@@ -852,13 +884,26 @@ int plan_prefix(const char* fn, const int* token_pos, int prefix_len, const Segm
     if (token_pos[t] < 0 || token_pos[t] == 0x7fffffff) return fail(PKV_E_ARG, "%s: token %d has position %d", fn, t, token_pos[t]);
     if (shared > 0 && token_pos[t] >= shared - 1) l.row_token.push_back(t);
   }
-  const bool together = static_cast<int>(l.row_token.size()) >= kMinPrefixTokens;
-  if (!together) l.row_token.clear();
-  for (int t = 0; t < g.n_tokens; ++t) {
-    const int begin = together && token_pos[t] >= shared - 1 ? shared : 0, len = token_pos[t] + 1 - begin;
-    if (len > 0) own.push_back(OwnRange{t, begin, len});
+  // worth while where every token's own way through the prefix, on the decode kernels, is reckoned to take longer
+  auto ranges = [&](bool together) {
+    own.clear();
+    for (int t = 0; t < g.n_tokens; ++t) {
+      const int begin = together && token_pos[t] >= shared - 1 ? shared : 0, len = token_pos[t] + 1 - begin;
+      if (len > 0) own.push_back(OwnRange{t, begin, len});
+    }
+  };
+  const int asked = tiles_asked();
+  if (asked == 1 && !l.row_token.empty()) {
+    segs.push_back(Segment{0, static_cast<int>(l.row_token.size()), shared, l.row_token[0]});
+  } else if (asked < 0 && l.row_token.size() >= 2) {
+    ranges(false);
+    const long long apart = step_cycles(segs, own, l.row_token, g, decode_sms(), true);
+    ranges(true);
+    segs.push_back(Segment{0, static_cast<int>(l.row_token.size()), shared, l.row_token[0]});
+    if (step_cycles(segs, own, l.row_token, g, decode_sms(), true) >= apart) segs.clear();
   }
-  if (together) segs.push_back(Segment{0, static_cast<int>(l.row_token.size()), shared, l.row_token[0]});
+  if (segs.empty()) l.row_token.clear();
+  ranges(!segs.empty());
   list_segments(segs, own, empty, g, decode_sms(), true, l);
   return write_image(fn, kPrefix, g, l, none, pos, segs.empty(), h_staging, staging_bytes, workspace_bytes, plan);
 }

@@ -84,16 +84,24 @@ inline long long most_tile_rows(const SegmentGeometry& g, int sms, bool prefix) 
 }
 inline long long most_parts(const SegmentGeometry& g, bool prefix) { return (prefix ? g.n_tokens : 0ll) + 2ll * own_extra(g); }
 
-// What a block needs for an item, in cycles (measured on B200, head_dim 64 and 128 alike within a tenth): start and end, and a
-// key tile of two groups, of one alone, of a pair of heads.
-constexpr int kItemCycles = 4500, kTwoGroupCycles = 3500, kOneGroupCycles = 2600, kPairCycles = 3600;
+// What the planner reckons with, in cycles of 1/1.75 ns (measured on B200; head_dim 64 and 128 alike within a tenth).
+// A block of the tile kernel: an item's start and end, and a key tile of two groups, of one alone, of a pair of heads.
+constexpr int kItemCycles = 5000, kTwoGroupCycles = 3700, kOneGroupCycles = 3500, kPairCycles = 4200;
 constexpr int kLeastTiles = 2;      // key tiles of a piece, at least
-// Partials cost a merge launch, and their way to L2 and back (rows of head_dim, cycles each for the whole GPU).
+// Partials of tiles are written and read at about 2,000 bytes a cycle, and the merge is a launch more.
 constexpr int kMergeCycles = 5000;
-inline long long partial_cycles(long long rows, int head_dim) { return rows * head_dim / 1024; }
+inline long long partial_cycles(long long rows, int head_dim) { return rows * head_dim * 8 / 2000; }
+// The decode kernels: a launch, and the K/V of every token's keys, mostly from L2.  (64 tokens of 1,084 keys on 8 kv heads of
+// 128 dims 31 us by this account and measured; 6 of 560 on 2 of 64 4.7 and 3.7.)
+constexpr int kOwnCycles = 7900, kOwnBytesPerCycle = 6300;
+inline long long own_cycles(const std::vector<OwnRange>& own, const SegmentGeometry& g) {
+  long long keys = 0;
+  for (const OwnRange& o : own) keys += o.len;
+  return own.empty() ? 0 : kOwnCycles + keys * g.kv_heads * g.head_dim * 2 * g.elem_bytes / kOwnBytesPerCycle;
+}
 
 struct TileUnit { TileItem item; int n_kt, per_tile; long long cycles() const { return kItemCycles + static_cast<long long>(n_kt) * per_tile; } };
-struct TileDeal { std::vector<std::vector<TileItem>> lists; long long cycles = 0, part_rows = 0; };
+struct TileDeal { std::vector<std::vector<TileItem>> lists; long long cycles = 0, part_rows = 0, cost = 0; };   // of the longest list; with the partials' way
 
 inline long long item_rows(const TileItem& t, const SegmentGeometry& g) { return static_cast<long long>(t.n_tok) * g.group() * (t.flags & kPair ? 2 : 1); }
 
@@ -117,7 +125,7 @@ inline TileDeal deal_whole(std::vector<TileUnit> units, int sms) {
 }
 
 // End to end, cut into equal shares.  `part` numbers the pieces' partial rows; pieces of a unit lie one behind the other.
-inline TileDeal deal_shares(const std::vector<TileUnit>& units, int sms, const SegmentGeometry& g, bool prefix) {
+inline TileDeal deal_shares(const std::vector<TileUnit>& units, int sms, int least, const SegmentGeometry& g, bool prefix) {
   TileDeal d;
   long long total = 0, longest = 0;
   for (const TileUnit& u : units) {
@@ -125,7 +133,7 @@ inline TileDeal deal_shares(const std::vector<TileUnit>& units, int sms, const S
     longest = std::max<long long>(longest, u.per_tile);
   }
   // every cut costs an item's start and end again
-  const long long share = std::max<long long>((total + static_cast<long long>(sms) * kItemCycles) / sms, kItemCycles + kLeastTiles * longest);
+  const long long share = std::max<long long>((total + static_cast<long long>(sms) * kItemCycles) / sms, kItemCycles + least * longest);
   long long room = 0, done = 0;
   for (const TileUnit& u : units) {
     int at = 0;
@@ -203,11 +211,26 @@ inline void cut_own(const std::vector<OwnRange>& own, const SegmentGeometry& g, 
   std::stable_sort(out.items.begin(), out.items.end(), [](const WorkItem& x, const WorkItem& y) { return x.kv_len > y.kv_len; });
 }
 
-// Puts everything together.  out.row_token holds the segments' tokens already; `empty`: tokens without keys.
-inline void list_segments(const std::vector<Segment>& segs, const std::vector<OwnRange>& own, const std::vector<int>& empty, const SegmentGeometry& g,
-                          int sms, bool prefix, SegmentLists& out) {
-  std::vector<int> pieces;
-  cut_own(own, g, own_extra(g), out, pieces);
+// The cheapest of: whole, and shares of pieces of at least 2, 4, 8 ... key tiles (fewer pieces leave fewer partials).
+inline TileDeal deal_tiles(const std::vector<TileUnit>& units, int sms, const SegmentGeometry& g, bool prefix) {
+  TileDeal best;
+  if (units.empty()) return best;
+  if (!prefix) {
+    best = deal_whole(units, sms);
+    best.cost = best.cycles;
+  }
+  int longest = 0;
+  for (const TileUnit& u : units) longest = std::max(longest, u.n_kt);
+  for (int least = kLeastTiles;; least *= 2) {
+    TileDeal d = deal_shares(units, sms, least, g, prefix);
+    d.cost = d.cycles + (d.part_rows > 0 ? (prefix ? 0 : kMergeCycles) + partial_cycles(d.part_rows, g.head_dim) : 0);
+    if ((best.lists.empty() || d.cost < best.cost) && d.part_rows <= most_tile_rows(g, sms, prefix)) best = std::move(d);
+    if (least >= longest) break;
+  }
+  return best;
+}
+
+inline std::vector<TileUnit> tile_units(const std::vector<Segment>& segs, const SegmentGeometry& g, const std::vector<int>& row_token) {
   const int group = g.group();
   std::vector<TileUnit> units;
   for (const Segment& s : segs) {
@@ -217,19 +240,29 @@ inline void list_segments(const std::vector<Segment>& segs, const std::vector<Ow
         const int n = std::min(g.tile_tokens(), s.n_tok - t), tok0 = s.tok0 + t;
         const bool small = n * group <= kTileRows / 2, pair = small && (kvh ^ 1) < g.kv_heads;
         if (pair && (kvh & 1)) continue;
-        const bool row = out.row_token[tok0 + n - 1] - out.row_token[tok0] == n - 1;      // (they ascend)
+        const bool row = row_token[tok0 + n - 1] - row_token[tok0] == n - 1;              // (they ascend)
         units.push_back(TileUnit{TileItem{tok0, n, kvh, 0, s.kv_len, -1, (row ? kConsecutive : 0) | (pair ? kPair : 0), s.source}, n_kt,
                                  pair ? kPairCycles : small ? kOneGroupCycles : kTwoGroupCycles});
       }
   }
+  return units;
+}
+
+// What a step would take with these tiles and own ranges.
+inline long long step_cycles(const std::vector<Segment>& segs, const std::vector<OwnRange>& own, const std::vector<int>& row_token, const SegmentGeometry& g,
+                             int sms, bool prefix) {
+  return deal_tiles(tile_units(segs, g, row_token), sms, g, prefix).cost + own_cycles(own, g) + (prefix && !segs.empty() ? kMergeCycles - kOwnCycles + 2000 : 0);
+}
+
+// Puts everything together.  out.row_token holds the segments' tokens already; `empty`: tokens without keys.
+inline void list_segments(const std::vector<Segment>& segs, const std::vector<OwnRange>& own, const std::vector<int>& empty, const SegmentGeometry& g,
+                          int sms, bool prefix, SegmentLists& out) {
+  std::vector<int> pieces;
+  cut_own(own, g, own_extra(g), out, pieces);
+  const int group = g.group();
+  const std::vector<TileUnit> units = tile_units(segs, g, out.row_token);
   if (!units.empty()) {
-    TileDeal deal = deal_shares(units, sms, g, prefix);
-    if (!prefix) {
-      TileDeal whole = deal_whole(units, sms);
-      if (whole.cycles <= deal.cycles + (deal.part_rows > 0 ? kMergeCycles + partial_cycles(deal.part_rows, g.head_dim) : 0) ||
-          deal.part_rows > most_tile_rows(g, sms, false))
-        deal = std::move(whole);
-    }
+    const TileDeal deal = deal_tiles(units, sms, g, prefix);
     out.n_tile_rows = deal.part_rows;
     for (const auto& list : deal.lists) {
       out.list_first.push_back(static_cast<int>(out.tiles.size()));

@@ -18,9 +18,10 @@ def run(pkv, step, **kw):
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("geom", [PAIRED, WIDE, QWEN, (48, 1, 64), (20, 1, 128)])
 @pytest.mark.parametrize("q_len,kv_len", [
-    ([4], [1]), ([130], [128]), ([5], [127]), ([300], [129]), ([9, 4, 33], [1500, 64, 16]), ([17], [5000]),
+    ([1], [200]), ([4], [1]), ([130], [128]), ([5], [127]), ([300], [129]), ([9, 4, 33], [1500, 64, 16]), ([17], [5000]),
 ])
-def test_tiles(pkv, torch_cuda, dtype, geom, q_len, kv_len):
+def test_tiles(pkv, torch_cuda, monkeypatch, dtype, geom, q_len, kv_len):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
     step = Step(torch_cuda, dtype, geom, q_len, kv_len, 16, seed=len(q_len) * 100 + q_len[0])
     plan = run(pkv, step)
     assert plan.plan.n_tiles > 0
@@ -33,7 +34,9 @@ def test_tiles(pkv, torch_cuda, dtype, geom, q_len, kv_len):
     ([1], [1]), ([1] * 40, [1 + 37 * i for i in range(40)]), ([1, 2, 3, 1], [700, 0, 65, 3000]),
     ([0, 60, 1, 0, 7, 200, 2], [100, 333, 1000, 0, 0, 1, 2049]),
 ])
-def test_ragged(pkv, torch_cuda, dtype, geom, q_len, kv_len):
+@pytest.mark.parametrize("tiles", ["", "1"])
+def test_ragged(pkv, torch_cuda, monkeypatch, tiles, dtype, geom, q_len, kv_len):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
     step = Step(torch_cuda, dtype, geom, q_len, kv_len, 16, seed=len(q_len))
     run(pkv, step)
     step.check(pkv)
@@ -41,7 +44,8 @@ def test_ragged(pkv, torch_cuda, dtype, geom, q_len, kv_len):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("bs", [1, 8, 24, 32, 64, 128, 512])
-def test_block_sizes(pkv, torch_cuda, dtype, bs):
+def test_block_sizes(pkv, torch_cuda, monkeypatch, dtype, bs):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
     for geom in (QWEN, WIDE):
         step = Step(torch_cuda, dtype, geom, [40, 1, 6, 150], [700, 901, 33, 128], bs, seed=bs)
         run(pkv, step)
@@ -54,9 +58,10 @@ def test_rows_of_no_sequence_stay(pkv, torch_cuda):
     step.check(pkv)
 
 
-def test_large_scores_and_rising_maxima(pkv, torch_cuda):
+def test_large_scores_and_rising_maxima(pkv, torch_cuda, monkeypatch):
     """Rows whose maximum grows tile by tile, so that the accumulator is rescaled again and again."""
     torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
     for geom in (PAIRED, WIDE):
         step = Step(torch, "bf16", geom, [140, 12], [1500, 900], 16, seed=4, sharp=6.0)
         for s in range(2):

@@ -29,15 +29,18 @@ def run(pkv, step, shared, pos=None, **kw):
 @pytest.mark.parametrize("n,shared,tails", [
     (2, 16, [1]), (3, 128, [5, 1, 300]), (9, 1024, [16, 1, 77]), (40, 2000, [3, 500, 64, 1]), (130, 640, [20, 9]), (4, 9008, [40]),
 ])
-def test_against_definition(pkv, torch_cuda, dtype, geom, n, shared, tails):
+@pytest.mark.parametrize("tiles", ["", "1"])
+def test_against_definition(pkv, torch_cuda, monkeypatch, tiles, dtype, geom, n, shared, tails):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
     step = make(torch_cuda, dtype, geom, n, shared, tails, 16, seed=n)
     plan = run(pkv, step, shared)
-    assert plan.plan.n_tiles > 0 or n < 4
+    assert plan.plan.n_tiles > 0 or tiles == ""
     step.check(pkv)
 
 
 @pytest.mark.parametrize("bs", [32, 64, 256])
-def test_block_sizes(pkv, torch_cuda, bs):
+def test_block_sizes(pkv, torch_cuda, monkeypatch, bs):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
     for geom in (TINY, WIDE):
         step = make(torch_cuda, "bf16", geom, 20, 1024, [1, 40, 333], bs, seed=bs)
         run(pkv, step, 1024)
@@ -59,9 +62,11 @@ def test_no_prefix_and_one_token(pkv, torch_cuda):
         step.check(pkv)
 
 
-def test_tokens_inside_the_prefix(pkv, torch_cuda):
+@pytest.mark.parametrize("tiles", ["", "1"])
+def test_tokens_inside_the_prefix(pkv, torch_cuda, monkeypatch, tiles):
     """A fully cached prompt computes its last token again: its position is the prefix's last, or any before."""
     torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
     shared = 512
     for geom in (TINY, WIDE):
         step = make(torch, "bf16", geom, 8, shared, [0, 30, 0, 1, 0, 0, 16, 200], 16, seed=2)
@@ -71,8 +76,9 @@ def test_tokens_inside_the_prefix(pkv, torch_cuda):
         step.check(pkv, limits=[p + 1 for p in pos])
 
 
-def test_prefix_that_ends_inside_a_block(pkv, torch_cuda):
+def test_prefix_that_ends_inside_a_block(pkv, torch_cuda, monkeypatch):
     """Keys the sequences agree on need not fill whole blocks or boxes."""
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
     step = make(torch_cuda, "f16", TINY, 10, 1024, [30, 5, 100], 32, seed=3)
     for shared in (1001, 1023, 1024, 1008):
         step.out.copy_(step.mark)
@@ -80,7 +86,8 @@ def test_prefix_that_ends_inside_a_block(pkv, torch_cuda):
         step.check(pkv)
 
 
-def test_against_the_ordinary_path_and_captured(pkv, torch_cuda):
+def test_against_the_ordinary_path_and_captured(pkv, torch_cuda, monkeypatch):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
     torch = torch_cuda
     step = make(torch, "bf16", WIDE, 70, 3000 // 16 * 16, [64, 1, 500], 16, seed=4)
     side = torch.cuda.Stream()
@@ -108,7 +115,8 @@ def test_against_the_ordinary_path_and_captured(pkv, torch_cuda):
         assert torch.equal(step.out, first)
 
 
-def test_two_plans_on_two_streams(pkv, torch_cuda):
+def test_two_plans_on_two_streams(pkv, torch_cuda, monkeypatch):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
     torch = torch_cuda
     steps = [make(torch, "bf16", TINY, 33 + i, 1600, [30, 5], 16, seed=5 + i) for i in range(2)]
     streams = [torch.cuda.Stream() for _ in steps]
@@ -126,10 +134,12 @@ def test_two_plans_on_two_streams(pkv, torch_cuda):
         step.check(pkv)
 
 
-def test_layer_with_norms_prefix_and_encoder(pkv, torch_cuda):
+@pytest.mark.parametrize("tiles", ["", "1"])
+def test_layer_with_norms_prefix_and_encoder(pkv, torch_cuda, monkeypatch, tiles):
     """One layer's run as a model makes it: norms + rotation + append of the step's tokens, attention over the shared
     prompt and their own keys, then attention to an encoder's states, every layer through the same two plans."""
     torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
     qh, kvh, hd = TINY
     n, shared, bs = 24, 320, 16
     step = make(torch, "bf16", TINY, n, shared, [40, 7, 90], bs, seed=6)

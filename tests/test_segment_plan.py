@@ -43,8 +43,10 @@ def log_int(r, lo, hi):
     return int(round(lo * (hi / lo) ** r.random()))
 
 
+@pytest.mark.parametrize("tiles", ["", "1", "0"])
 @pytest.mark.parametrize("seed", range(60))
-def test_cross_covers_every_pair(pkv, seed):
+def test_cross_covers_every_pair(pkv, monkeypatch, seed, tiles):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
     r = random.Random(seed)
     geom = r.choice(GEOMS)
     n_seqs = log_int(r, 1, 60)
@@ -69,8 +71,10 @@ def test_cross_covers_every_pair(pkv, seed):
     assert (np.delete(image.seq, list(want)) == -1).all()
 
 
+@pytest.mark.parametrize("tiles", ["", "1", "0"])
 @pytest.mark.parametrize("seed", range(60))
-def test_prefix_covers_every_pair(pkv, seed):
+def test_prefix_covers_every_pair(pkv, monkeypatch, seed, tiles):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
     r = random.Random(1000 + seed)
     geom = r.choice(GEOMS)
     n = log_int(r, 1, 700)

@@ -853,8 +853,11 @@ int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* 
   int fewest = asked == 1 ? 1 : asked == 0 ? 0x7fffffff : kMinTileTokens;
   if (g.tiles() && asked < 0) {
     long long least = -1;
+    size_t tiled = 0;
     for (int f = kMinTileTokens; f <= kManyTileTokens; f = f < 4 ? f + 1 : f * 2) {
       split(f);
+      if (least >= 0 && segs.size() == tiled) continue;          // the same sequences as before
+      tiled = segs.size();
       const long long c = step_cycles(segs, own, l.row_token, g, decode_sms(), false);
       if (least < 0 || c < least) { least = c; fewest = f; }
       if (segs.empty()) break;

@@ -105,27 +105,31 @@ struct TileDeal { std::vector<std::vector<TileItem>> lists; long long cycles = 0
 
 inline long long item_rows(const TileItem& t, const SegmentGeometry& g) { return static_cast<long long>(t.n_tok) * g.group() * (t.flags & kPair ? 2 : 1); }
 
-// Whole, longest first, each to the block with the least to do so far.
-inline TileDeal deal_whole(std::vector<TileUnit> units, int sms) {
-  std::stable_sort(units.begin(), units.end(), [](const TileUnit& x, const TileUnit& y) { return x.cycles() > y.cycles(); });
+// Whole, longest first, each to the block with the least to do so far.  `keep`: the lists, not only what they would cost.
+inline TileDeal deal_whole(const std::vector<TileUnit>& units, int sms, bool keep) {
+  std::vector<int> order(units.size());
+  for (size_t i = 0; i < order.size(); ++i) order[i] = static_cast<int>(i);
+  std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return units[x].cycles() > units[y].cycles(); });
   TileDeal d;
-  d.lists.resize(std::min<size_t>(units.size(), sms));
+  const size_t blocks = std::min<size_t>(units.size(), sms);
+  if (keep) d.lists.resize(blocks);
   using Load = std::pair<long long, int>;
   std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least;
-  for (size_t b = 0; b < d.lists.size(); ++b) least.push({0, static_cast<int>(b)});
-  for (const TileUnit& u : units) {
+  for (size_t b = 0; b < blocks; ++b) least.push({0, static_cast<int>(b)});
+  for (int u : order) {
     Load l = least.top();
     least.pop();
-    d.lists[l.second].push_back(u.item);
-    l.first += u.cycles();
+    if (keep) d.lists[l.second].push_back(units[u].item);
+    l.first += units[u].cycles();
     d.cycles = std::max(d.cycles, l.first);
     least.push(l);
   }
+  d.cost = d.cycles;
   return d;
 }
 
 // End to end, cut into equal shares.  `part` numbers the pieces' partial rows; pieces of a unit lie one behind the other.
-inline TileDeal deal_shares(const std::vector<TileUnit>& units, int sms, int least, const SegmentGeometry& g, bool prefix) {
+inline TileDeal deal_shares(const std::vector<TileUnit>& units, int sms, int least, const SegmentGeometry& g, bool prefix, bool keep) {
   TileDeal d;
   long long total = 0, longest = 0;
   for (const TileUnit& u : units) {
@@ -135,36 +139,44 @@ inline TileDeal deal_shares(const std::vector<TileUnit>& units, int sms, int lea
   // every cut costs an item's start and end again
   const long long share = std::max<long long>((total + static_cast<long long>(sms) * kItemCycles) / sms, kItemCycles + least * longest);
   long long room = 0, done = 0;
+  int lists = 0, in_list = 0;                                              // so far; items of the last one
+  std::vector<std::pair<size_t, size_t>> pieces;                           // of a unit: (list, place)
   for (const TileUnit& u : units) {
-    int at = 0;
-    std::vector<std::pair<size_t, size_t>> pieces;                       // (list, place)
-    while (at < u.n_kt) {
-      const bool last = static_cast<int>(d.lists.size()) >= sms;
-      if (d.lists.empty() || (!last && !d.lists.back().empty() && room < kItemCycles + std::min(kLeastTiles, u.n_kt - at) * static_cast<long long>(u.per_tile))) {
-        d.lists.emplace_back();
-        room += share;                                                   // (what a list leaves, the next one gets)
-        done = 0;
+    int n_pieces = 0;
+    pieces.clear();
+    for (int at = 0; at < u.n_kt;) {
+      const bool last = lists >= sms;
+      if (lists == 0 || (!last && in_list > 0 && room < kItemCycles + std::min(kLeastTiles, u.n_kt - at) * static_cast<long long>(u.per_tile))) {
+        ++lists;
+        if (keep) d.lists.emplace_back();
+        room += share;                                                     // (what a list leaves, the next one gets)
+        done = in_list = 0;
         continue;
       }
       int n = last ? u.n_kt - at : static_cast<int>(std::min<long long>(u.n_kt - at, std::max<long long>(kLeastTiles, (room - kItemCycles) / u.per_tile)));
-      if (u.n_kt - at - n < kLeastTiles) n = u.n_kt - at;                // nothing worth a piece would be left
-      TileItem t = u.item;
-      t.kv_begin = at * kTileKeys;
-      t.kv_len = std::min(n * kTileKeys, u.item.kv_len - t.kv_begin);
-      pieces.push_back({d.lists.size() - 1, d.lists.back().size()});
-      d.lists.back().push_back(t);
+      if (u.n_kt - at - n < kLeastTiles) n = u.n_kt - at;                  // nothing worth a piece would be left
+      if (keep) {
+        TileItem t = u.item;
+        t.kv_begin = at * kTileKeys;
+        t.kv_len = std::min(n * kTileKeys, u.item.kv_len - t.kv_begin);
+        pieces.push_back({d.lists.size() - 1, d.lists.back().size()});
+        d.lists.back().push_back(t);
+      }
+      ++n_pieces;
+      ++in_list;
       const long long took = kItemCycles + static_cast<long long>(n) * u.per_tile;
       room -= took;
       done += took;
       d.cycles = std::max(d.cycles, done);
       at += n;
     }
-    if (prefix || pieces.size() > 1)
-      for (const auto& p : pieces) {
-        d.lists[p.first][p.second].part = static_cast<int>(d.part_rows);
-        d.part_rows += item_rows(u.item, g);
-      }
+    if (prefix || n_pieces > 1) {
+      const long long rows = item_rows(u.item, g);
+      for (size_t p = 0; p < pieces.size(); ++p) d.lists[pieces[p].first][pieces[p].second].part = static_cast<int>(d.part_rows + static_cast<long long>(p) * rows);
+      d.part_rows += n_pieces * rows;
+    }
   }
+  d.cost = d.cycles + (d.part_rows > 0 ? (prefix ? 0 : kMergeCycles) + partial_cycles(d.part_rows, g.head_dim) : 0);
   return d;
 }
 
@@ -212,22 +224,18 @@ inline void cut_own(const std::vector<OwnRange>& own, const SegmentGeometry& g, 
 }
 
 // The cheapest of: whole, and shares of pieces of at least 2, 4, 8 ... key tiles (fewer pieces leave fewer partials).
-inline TileDeal deal_tiles(const std::vector<TileUnit>& units, int sms, const SegmentGeometry& g, bool prefix) {
-  TileDeal best;
-  if (units.empty()) return best;
-  if (!prefix) {
-    best = deal_whole(units, sms);
-    best.cost = best.cycles;
-  }
-  int longest = 0;
+inline TileDeal deal_tiles(const std::vector<TileUnit>& units, int sms, const SegmentGeometry& g, bool prefix, bool keep) {
+  if (units.empty()) return TileDeal();
+  long long cost = prefix ? -1 : deal_whole(units, sms, false).cost;
+  int pick = 0, longest = 0;                                               // least tiles of a piece; 0: whole
   for (const TileUnit& u : units) longest = std::max(longest, u.n_kt);
   for (int least = kLeastTiles;; least *= 2) {
-    TileDeal d = deal_shares(units, sms, least, g, prefix);
-    d.cost = d.cycles + (d.part_rows > 0 ? (prefix ? 0 : kMergeCycles) + partial_cycles(d.part_rows, g.head_dim) : 0);
-    if ((best.lists.empty() || d.cost < best.cost) && d.part_rows <= most_tile_rows(g, sms, prefix)) best = std::move(d);
+    const TileDeal d = deal_shares(units, sms, least, g, prefix, false);
+    if ((cost < 0 || d.cost < cost) && d.part_rows <= most_tile_rows(g, sms, prefix)) { cost = d.cost; pick = least; }
     if (least >= longest) break;
   }
-  return best;
+  TileDeal d = pick ? deal_shares(units, sms, pick, g, prefix, keep) : deal_whole(units, sms, keep);
+  return d;
 }
 
 inline std::vector<TileUnit> tile_units(const std::vector<Segment>& segs, const SegmentGeometry& g, const std::vector<int>& row_token) {
@@ -251,7 +259,7 @@ inline std::vector<TileUnit> tile_units(const std::vector<Segment>& segs, const 
 // What a step would take with these tiles and own ranges.
 inline long long step_cycles(const std::vector<Segment>& segs, const std::vector<OwnRange>& own, const std::vector<int>& row_token, const SegmentGeometry& g,
                              int sms, bool prefix) {
-  return deal_tiles(tile_units(segs, g, row_token), sms, g, prefix).cost + own_cycles(own, g) + (prefix && !segs.empty() ? kMergeCycles - kOwnCycles + 2000 : 0);
+  return deal_tiles(tile_units(segs, g, row_token), sms, g, prefix, false).cost + own_cycles(own, g) + (prefix && !segs.empty() ? kMergeCycles - kOwnCycles + 2000 : 0);
 }
 
 // Puts everything together.  out.row_token holds the segments' tokens already; `empty`: tokens without keys.
@@ -262,7 +270,7 @@ inline void list_segments(const std::vector<Segment>& segs, const std::vector<Ow
   const int group = g.group();
   const std::vector<TileUnit> units = tile_units(segs, g, out.row_token);
   if (!units.empty()) {
-    const TileDeal deal = deal_tiles(units, sms, g, prefix);
+    const TileDeal deal = deal_tiles(units, sms, g, prefix, true);
     out.n_tile_rows = deal.part_rows;
     for (const auto& list : deal.lists) {
       out.list_first.push_back(static_cast<int>(out.tiles.size()));

@@ -287,14 +287,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const TileItem it = load_tile(tiles + r);
         const int heads = it.flags & kPair ? 2 : 1, qb = r % S::kQBufs;
         const uint32_t bar = BAR(Q_FULL + qb), dst = base + qb * S::kQ;
-        const int many = (it.flags & kConsecutive) ? it.n_tok / a.box_tokens : 0, boxes = many + it.n_tok - many * a.box_tokens;
+        // A lane a box: boxes of several tokens where the tokens are consecutive, the last one with rows past the item's that
+        // nobody looks at if there is room for them, else boxes of one.
+        const int up = (it.n_tok + a.box_tokens - 1) / a.box_tokens;
+        const int many = !(it.flags & kConsecutive) ? 0 : up * a.box_tokens * a.group <= 256 / heads ? up : it.n_tok / a.box_tokens;
+        const int boxes = many + max(it.n_tok - many * a.box_tokens, 0);
         int token = 0;
         auto first_of = [&](int b) { return b < many ? b * a.box_tokens : b + many * (a.box_tokens - 1); };   // first token of a box
         if (lane < boxes) token = __ldg(a.row_token + it.tok0 + first_of(lane));
         if (r == 0) after_previous();
         if (lane == 0) {
           WAIT(BAR(Q_EMPTY + qb), ((r / S::kQBufs) & 1) ^ 1);
-          if (!dead) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(heads * it.n_tok * a.group) * 128u * S::kHalves);
+          if (!dead) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(heads * (many * a.box_tokens + boxes - many) * a.group) * 128u * S::kHalves);
         }
         dead = __shfl_sync(0xffffffffu, dead ? 1 : 0, 0) != 0;
         if (dead) break;

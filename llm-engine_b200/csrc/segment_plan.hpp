@@ -88,6 +88,7 @@ inline long long most_parts(const SegmentGeometry& g, bool prefix) { return (pre
 // A block of the tile kernel: an item's start and end, and a key tile of two groups, of one alone, of a pair of heads.
 constexpr int kItemCycles = 5000, kTwoGroupCycles = 3700, kOneGroupCycles = 3500, kPairCycles = 4200;
 constexpr int kLeastTiles = 2;      // key tiles of a piece, at least
+constexpr int kManyUnits = 32;      // units a block, from which on a step's time is their average
 // Partials of tiles are written and read at about 2,000 bytes a cycle, and the merge is a launch more.
 constexpr int kMergeCycles = 5000;
 inline long long partial_cycles(long long rows, int head_dim) { return rows * head_dim * 8 / 2000; }
@@ -226,10 +227,24 @@ inline void cut_own(const std::vector<OwnRange>& own, const SegmentGeometry& g, 
 // The cheapest of: whole, and shares of pieces of at least 2, 4, 8 ... key tiles (fewer pieces leave fewer partials).
 inline TileDeal deal_tiles(const std::vector<TileUnit>& units, int sms, const SegmentGeometry& g, bool prefix, bool keep) {
   if (units.empty()) return TileDeal();
-  long long cost = prefix ? -1 : deal_whole(units, sms, false).cost;
   int pick = 0, longest = 0;                                               // least tiles of a piece; 0: whole
-  for (const TileUnit& u : units) longest = std::max(longest, u.n_kt);
-  for (int least = kLeastTiles;; least *= 2) {
+  long long total = 0;
+  for (const TileUnit& u : units) {
+    longest = std::max(longest, u.n_kt);
+    total += u.cycles();
+  }
+  if (!keep && units.size() > static_cast<size_t>(kManyUnits) * sms) {     // dealt out as good as evenly, whatever the order
+    TileDeal d;
+    if (prefix)
+      for (const TileUnit& u : units) d.part_rows += item_rows(u.item, g);
+    d.cycles = total / sms;
+    d.cost = d.cycles + partial_cycles(d.part_rows, g.head_dim);
+    return d;
+  }
+  long long cost = prefix ? -1 : deal_whole(units, sms, false).cost;
+  // Cuts could gain a fiftieth and their merge's cost at most: whole without reckoning them.  (Many units are level by themselves.)
+  const bool level = cost >= 0 && cost <= total / sms + total / sms / 50 + kMergeCycles;
+  for (int least = kLeastTiles; !level; least *= 2) {
     const TileDeal d = deal_shares(units, sms, least, g, prefix, false);
     if ((cost < 0 || d.cost < cost) && d.part_rows <= most_tile_rows(g, sms, prefix)) { cost = d.cost; pick = least; }
     if (least >= longest) break;

@@ -139,7 +139,8 @@ int pkv_rope_append_f32(void* q, const void* k, const void* v, const int* positi
  * may be q itself if q's rows are contiguous (no other overlap is allowed).
  * Padded steps: a row whose position is outside [0, max_positions) (rows of the tables)
  * is neither read nor written; a row whose slot is outside [0, n_slots) (pool rows)
- * gets its q_out, but no K/V.  Slots of a call are distinct.  head_dim must be even.
+ * gets its q_out, but no K/V.  Slots of a call are distinct (rows of one slot would race:
+ * whichever comes last stays).  head_dim must be even.
  * No llm-engine counterpart (its models have no such norms); the rotation is
  * include/engine/ops.h:56-68, the append src/kernels/store_kv.cu:20-36. */
 int pkv_qk_norm_rope_append_f16(const void* q, const void* k, const void* v, long long q_stride, long long k_stride,
@@ -466,9 +467,17 @@ int pkv_prefill_attn_f16(const void* q, const void* k_cache, const void* v_cache
  * to its own position only.  (pkv_decode_plan_host_shared finds common prefixes by itself and
  * reads them once per four tokens.)
  *
+ * out may not overlap q or the pools.  kv_len and token_pos + 1 are 2^30 at most.
+ *
+ * Ahead of a call: the plan, block_tables, table_offset and token_seq are read while the
+ * launch directly before it may still be running (q, K and V are not), so they must have been
+ * complete when that launch BEGAN.  Copies and kernels that do not release their dependents
+ * early (griddepcontrol.launch_dependents) may stand directly before the call whatever they write.
+ *
  * A plan belongs to the host lengths it was made from and to the workspace it was uploaded
  * to (256-byte aligned; pkv_cross_workspace_bytes / pkv_prefix_workspace_bytes are enough for
- * any lengths); it serves any number of calls on one stream, captured ones included.  Calls
+ * any lengths); it serves any number of calls on one stream, captured ones included: a replay
+ * repeats the captured step's work list, other lengths want another plan and capture.  Calls
  * that may overlap need a workspace each.  h_staging (at least pkv_segment_staging_bytes, pinned
  * for a truly asynchronous copy) must stay untouched until the upload has run; the _image forms
  * write it and leave the copy of plan->image_bytes to the start of the workspace to the caller.

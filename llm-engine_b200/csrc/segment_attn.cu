@@ -487,7 +487,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               tc::st16(t_o + c, v);
             }
           }
-          const float2 neg = both(-m_used * sl2), by = both(sl2);
+          // (no finite score yet: the weights are zero, not inf - inf)
+          const float2 neg = both(m_used == -INFINITY ? 0.f : -m_used * sl2), by = both(sl2);
 #pragma unroll
           for (int c = 0; c < 64; c += 32) {
             uint32_t pk[16];
@@ -754,6 +755,7 @@ int check_geometry(const char* fn, const SegmentGeometry& g) {
 }
 
 enum Kind { kCross = 1, kPrefix = 2 };
+constexpr int kMostKeys = 1 << 30;       // of a token: lengths rounded up to tiles stay below 2^31
 
 // PKV_SEGMENT_TILES=1: whatever the tile kernel can take goes to it, =0: nothing does; else what is reckoned to take least.
 // Read at every planning call (a measurement and testing aid).
@@ -811,8 +813,11 @@ int write_image(const char* fn, Kind kind, const SegmentGeometry& g, const Segme
 int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* kv_len, int n_seqs, const SegmentGeometry& g, void* h_staging,
                size_t staging_bytes, size_t workspace_bytes, pkv_segment_plan* plan) {
   if (!plan) return fail(PKV_E_ARG, "%s: null plan", fn);
-  std::memset(plan, 0, sizeof(*plan));
-  if (g.n_tokens <= 0 || n_seqs <= 0) return PKV_OK;
+  std::memset(plan, 0, sizeof(*plan));                           // (kind 0: a refused plan is refused again where it is used)
+  if (g.n_tokens <= 0 || n_seqs <= 0) {
+    plan->kind = kCross;
+    return PKV_OK;
+  }
   if (!q_len || !kv_len || !h_staging) return fail(PKV_E_ARG, "%s: null pointer", fn);
   int st = check_geometry(fn, g);
   if (st != PKV_OK) return st;
@@ -821,6 +826,7 @@ int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* 
   int listed = 0, most = 0;
   for (int s = 0; s < n_seqs; ++s) {
     const long long at = q_start ? q_start[s] : next;
+    if (kv_len[s] > kMostKeys) return fail(PKV_E_UNSUPPORTED, "%s: sequence %d has %d keys; at most 2^30", fn, s, kv_len[s]);
     if (q_len[s] < 0 || kv_len[s] < 0 || at < 0 || at + q_len[s] > g.n_tokens)
       return fail(PKV_E_ARG, "%s: sequence %d has rows %lld .. + %d of %d and %d keys", fn, s, at, q_len[s], g.n_tokens, kv_len[s]);
     next = at + q_len[s];
@@ -876,7 +882,10 @@ int plan_prefix(const char* fn, const int* token_pos, int prefix_len, const Segm
                 size_t workspace_bytes, pkv_segment_plan* plan) {
   if (!plan) return fail(PKV_E_ARG, "%s: null plan", fn);
   std::memset(plan, 0, sizeof(*plan));
-  if (g.n_tokens <= 0) return PKV_OK;
+  if (g.n_tokens <= 0) {
+    plan->kind = kPrefix;
+    return PKV_OK;
+  }
   if (!token_pos || !h_staging) return fail(PKV_E_ARG, "%s: null pointer", fn);
   if (prefix_len < 0) return fail(PKV_E_ARG, "%s: prefix_len %d must not be negative", fn, prefix_len);
   int st = check_geometry(fn, g);
@@ -888,7 +897,8 @@ int plan_prefix(const char* fn, const int* token_pos, int prefix_len, const Segm
   std::vector<OwnRange> own;
   SegmentLists l;
   for (int t = 0; t < g.n_tokens; ++t) {
-    if (token_pos[t] < 0 || token_pos[t] == 0x7fffffff) return fail(PKV_E_ARG, "%s: token %d has position %d", fn, t, token_pos[t]);
+    if (token_pos[t] < 0) return fail(PKV_E_ARG, "%s: token %d has negative position %d", fn, t, token_pos[t]);
+    if (token_pos[t] >= kMostKeys) return fail(PKV_E_UNSUPPORTED, "%s: token %d has position %d; below 2^30", fn, t, token_pos[t]);
     if (shared > 0 && token_pos[t] >= shared - 1) l.row_token.push_back(t);
   }
   // worth while where every token's own way through the prefix, on the decode kernels, is reckoned to take longer
@@ -927,12 +937,14 @@ int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const v
                  const int* table_offset, const int* token_seq, void* out, float scale, void* workspace, size_t workspace_bytes, pkv_stream stream) {
   const char* fn = kind == kCross ? "pkv_cross_attn" : "pkv_prefix_attn";
   if (!plan) return fail(PKV_E_ARG, "%s: null plan", fn);
+  if (plan->kind != kind) return fail(PKV_E_ARG, "%s: a plan of the other kind, or one that was never made", fn);
   if (plan->n_tokens <= 0 || (plan->n_tiles == 0 && plan->n_items == 0 && plan->n_merged == 0)) return PKV_OK;
   int st = check_error_mirror(fn);
   if (st != PKV_OK) return st;
-  if (plan->kind != kind) return fail(PKV_E_ARG, "%s: a plan of the other kind", fn);
   if (plan->elem_bytes != static_cast<int>(sizeof(T))) return fail(PKV_E_ARG, "%s: the plan is for elements of %d bytes", fn, plan->elem_bytes);
-  if (!q || !k_cache || !v_cache || !block_tables || !table_offset || !out || (kind == kPrefix && !token_seq)) return fail(PKV_E_ARG, "%s: null device pointer", fn);
+  const bool keys = plan->n_tiles > 0 || plan->n_items > 0;      // else every row's output is zero
+  if (!out || (keys && (!q || !k_cache || !v_cache || !block_tables || !table_offset || (kind == kPrefix && !token_seq))))
+    return fail(PKV_E_ARG, "%s: null device pointer", fn);
   if (!(scale > 0.f)) return fail(PKV_E_ARG, "%s: scale must be positive", fn);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255)) return fail(PKV_E_ARG, "%s: workspace null or not 256-byte aligned", fn);
   if (workspace_bytes < plan->workspace_bytes) return fail(PKV_E_WORKSPACE, "%s: workspace of %zu bytes; the plan takes %zu", fn, workspace_bytes, plan->workspace_bytes);

@@ -404,6 +404,8 @@ class CrossPlan(_SegmentPlan):
     def attention(self, q, k_cache, v_cache, block_tables, table_offset, out, scale: float, stream=None) -> None:
         """out[t] = softmax(q[t] K^T scale) V over all keys of t's sequence; zero where it has none.  table_offset[s] is the
         start of sequence s's table."""
+        if table_offset.numel() < self.n_seqs:
+            raise ValueError(f"table_offset must name the tables of {self.n_seqs} sequences")
         self._run("pkv_cross_attn_", q, k_cache, v_cache, out, (block_tables, table_offset), scale, stream)
 
 
@@ -437,6 +439,8 @@ class PrefixPlan(_SegmentPlan):
 
     def attention(self, q, k_cache, v_cache, block_tables, table_offset, token_seq, out, scale: float, stream=None) -> None:
         """As launch_attention_decode with the step's whole tables."""
+        if token_seq.numel() < self.n_tokens:
+            raise ValueError(f"token_seq must name the sequences of {self.n_tokens} tokens")
         self._run("pkv_prefix_attn_", q, k_cache, v_cache, out, (block_tables, table_offset, token_seq), scale, stream)
 
 

@@ -73,6 +73,22 @@ def test_large_scores_and_rising_maxima(pkv, torch_cuda, monkeypatch):
         step.check(pkv)
 
 
+def test_scores_of_minus_infinity(pkv, torch_cuda, monkeypatch):
+    """Keys that the values of K themselves shut out (weight zero), the whole first key tile of them and more."""
+    torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
+    for geom in (PAIRED, WIDE):
+        for shut in (64, 128, 300):
+            step = Step(torch, "bf16", geom, [150, 9], [1500, 700], 16, seed=shut)
+            step.q.view(step.n, step.qh, step.hd)[:, :, 0] = 1.0
+            for s in range(2):
+                step.kc.view(-1, step.kvh, step.hd)[step.slots[s][:shut], :, 0] = -float("inf")
+            run(pkv, step)
+            for s in range(2):
+                step.slots[s] = step.slots[s][shut:]             # the definition over the other keys: these add exact zeros
+            step.check(pkv)
+
+
 def test_many_items_on_every_block(pkv, torch_cuda):
     """More items than blocks: queues of several items each, of both kinds, with odd and even numbers of key tiles."""
     lens = [300 + 61 * (i % 7) for i in range(30)]
@@ -135,5 +151,10 @@ def test_python_refusals(pkv, torch_cuda):
         plan.attention(*args[:3], step.block_tables.long(), *args[4:], step.scale)
     with pytest.raises(ValueError):
         plan.build_host([5, 1], [60, 3])
+    with pytest.raises(ValueError):
+        plan.attention(*args[:4], step.table_offset[:0], step.out, step.scale)
+    fresh = pkv.CrossPlan(5, 1, *TINY, 16, step.q.dtype)
+    with pytest.raises(pkv.PkvError):
+        fresh.attention(*args, step.scale)                       # never built
     with pytest.raises(pkv.PkvError):
         plan.attention(*args, 0.0)

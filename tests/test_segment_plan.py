@@ -104,6 +104,17 @@ def test_packed_rows_without_starts_and_empty_steps(pkv):
         assert pkv.lib().pkv_cross_attn_bf16(C.byref(plan), *[None] * 6, 1.0, None, 0, None) == 0
 
 
+def test_plans_that_were_never_made_are_refused(pkv):
+    L, E = pkv.lib(), pkv._lib
+    plan = E.SegmentPlan()
+    cross_args, prefix_args = (C.byref(plan), *[None] * 6, 1.0, None, 0, None), (C.byref(plan), *[None] * 7, 1.0, None, 0, None)
+    assert L.pkv_cross_attn_bf16(*cross_args) == L.pkv_prefix_attn_bf16(*prefix_args) == E.PKV_E_ARG
+    st, plan, b = cross(pkv, [1, -1], [5, 5], 4, GEOMS[0])
+    assert st == E.PKV_E_ARG and L.pkv_cross_attn_bf16(C.byref(plan), *[None] * 6, 1.0, None, 0, None) == E.PKV_E_ARG
+    st, plan, b = cross(pkv, [1], [5], 0, GEOMS[0], b=Buffers(pkv, 1, 14, 2, 64, False))
+    assert st == 0 and L.pkv_prefix_attn_bf16(C.byref(plan), *[None] * 7, 1.0, None, 0, None) == E.PKV_E_ARG
+
+
 def test_refusals(pkv):
     L, E = pkv.lib(), pkv._lib
     g = GEOMS[0]
@@ -116,7 +127,8 @@ def test_refusals(pkv):
     assert cross(pkv, [2], [5], 9, (14, 4, 64), b=Buffers(pkv, 9, 14, 2, 64, False))[0] == E.PKV_E_UNSUPPORTED
     assert cross(pkv, [2], [5], 9, (2, 1, 512))[0] == E.PKV_E_UNSUPPORTED
     assert prefix(pkv, [5, -1], 0, g)[0] == E.PKV_E_ARG
-    assert prefix(pkv, [5, 2 ** 31 - 1], 0, g)[0] == E.PKV_E_ARG
+    assert prefix(pkv, [5, 2 ** 31 - 1], 0, g)[0] == E.PKV_E_UNSUPPORTED and prefix(pkv, [5, 2 ** 30], 0, g)[0] == E.PKV_E_UNSUPPORTED
+    assert cross(pkv, [2], [2 ** 30 + 1], 9, g)[0] == E.PKV_E_UNSUPPORTED and cross(pkv, [2], [2 ** 31 - 1], 9, g)[0] == E.PKV_E_UNSUPPORTED
     assert prefix(pkv, [5], -16, g)[0] == E.PKV_E_ARG
     small = Buffers(pkv, 64, 14, 2, 64, True)
     small.ws = 4096
@@ -165,3 +177,28 @@ def test_norm_refusals(pkv):
     assert call(maxp=0) == E.PKV_E_ARG and call(n_slots=0) == E.PKV_E_ARG and call(qh=-1) == E.PKV_E_ARG
     assert call(qo=one, qs=1024) == E.PKV_E_ARG                    # in place needs contiguous rows
     assert call(n=0, q=None) == 0 and call(qh=0, kvh=0, q=None) == 0
+
+
+def test_longest_allowed_keys_are_planned(pkv):
+    """2^30 keys, whose lengths in tiles and slabs stay within 32 bits."""
+    for geom in (GEOMS[0], GEOMS[2]):
+        st, plan, b = cross(pkv, [40, 1], [2 ** 30, 2 ** 30], 41, geom)
+        assert st == 0, pkv._lib.last_error()
+        check_cover(Image(b.staging, plan), plan, {t: 2 ** 30 for t in range(41)})
+        st, plan, b = prefix(pkv, [2 ** 30 - 1] * 3, 2 ** 30 - 16, geom)
+        assert st == 0, pkv._lib.last_error()
+        check_cover(Image(b.staging, plan), plan, {t: 2 ** 30 for t in range(3)})
+
+
+def test_plans_do_not_depend_on_what_was_planned_before(pkv):
+    """The same lengths give the same image, whatever the staging buffer held."""
+    b = Buffers(pkv, 100, 32, 8, 128, True)
+    pos = [4096 + 7 * i for i in range(100)]
+    st, plan, _ = prefix(pkv, pos, 4096, GEOMS[2], b=b)
+    first = b.staging[:plan.image_bytes].copy()
+    prefix(pkv, [50] * 100, 0, GEOMS[2], b=b)
+    st, again, _ = prefix(pkv, pos, 4096, GEOMS[2], b=b)
+    assert st == 0 and again.image_bytes == plan.image_bytes
+    a, c = Image(first, plan), Image(b.staging, again)
+    for name in ("items", "tiles", "merge", "pos"):
+        assert np.array_equal(getattr(a, name), getattr(c, name)), name

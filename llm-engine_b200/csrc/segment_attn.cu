@@ -28,6 +28,11 @@
 // P is rounded to 16 bits for the second product (the sums are of the unrounded ones), as the operands of the
 // tensor cores are; scores, sums and accumulators are fp32.
 //
+// Measured on B200: a key tile of both groups takes about 3,600 cycles at head_dim 128 (products 2,048, exponentials 2,048, the rest a
+// group's chain of load, maximum, exponentials, store that one other group does not cover) and 3,350 at 64 (products 1,024; the issuing
+// warp's waits); an item's start and end 5,000.  4 sequences of 1,000 - 2,048 tokens and 4,000 - 6,500 keys, 32/8 heads of 128 dims: 593 us,
+// 1,155 TFLOP/s.  24 of 3 - 448 tokens and 100 - 1,500 keys, 16/16 heads of 64: 52 us.
+//
 // Blocks are persistent, one on an SM, each with a list of items of its own.  Every wait is bounded: one that runs
 // out sets bit 32 of the error word and the block winds down.
 #include <algorithm>

@@ -89,20 +89,35 @@ inline long long most_parts(const SegmentGeometry& g, bool prefix) { return (pre
 constexpr int kItemCycles = 5000, kTwoGroupCycles = 3700, kOneGroupCycles = 3500, kPairCycles = 4200;
 constexpr int kLeastTiles = 2;      // key tiles of a piece, at least
 constexpr int kManyUnits = 32;      // units a block, from which on a step's time is their average
+constexpr int kFewUnits = 2;        // and up to which it is worth while to look for fewer blocks
 // Partials of tiles are written and read at about 2,000 bytes a cycle, and the merge is a launch more.
 constexpr int kMergeCycles = 5000;
 inline long long partial_cycles(long long rows, int head_dim) { return rows * head_dim * 8 / 2000; }
 // The decode kernels: a launch, and the K/V of every token's keys, mostly from L2.  (64 tokens of 1,084 keys on 8 kv heads of
 // 128 dims 31 us by this account and measured; 6 of 560 on 2 of 64 4.7 and 3.7.)
 constexpr int kOwnCycles = 7900, kOwnBytesPerCycle = 6300;
-inline long long own_cycles(const std::vector<OwnRange>& own, const SegmentGeometry& g) {
+inline long long own_fetch(const std::vector<OwnRange>& own, const SegmentGeometry& g) {
   long long keys = 0;
   for (const OwnRange& o : own) keys += o.len;
-  return own.empty() ? 0 : kOwnCycles + keys * g.kv_heads * g.head_dim * 2 * g.elem_bytes / kOwnBytesPerCycle;
+  return keys * g.kv_heads * g.head_dim * 2 * g.elem_bytes / kOwnBytesPerCycle;
 }
+inline long long own_cycles(const std::vector<OwnRange>& own, const SegmentGeometry& g) { return own.empty() ? 0 : kOwnCycles + own_fetch(own, g); }
+// Behind a tile kernel: their blocks start on the SMs that it leaves free, kOwnStart cycles after it, and what is left when it ends takes
+// the whole GPU and kOwnTail more.  (128 tokens behind 2,048 keys, 32/4 heads of 64: 128 blocks of tiles 20.6 us, 64 blocks of
+// twice as many 15.9.  200 behind 16,384, 32/8 of 128: 148 blocks 87.3 us, 132 84.8, 139 84.0, 112 85.4, 96 95.4.)
+constexpr int kOwnStart = 6000, kOwnTail = 4000;
 
 struct TileUnit { TileItem item; int n_kt, per_tile; long long cycles() const { return kItemCycles + static_cast<long long>(n_kt) * per_tile; } };
-struct TileDeal { std::vector<std::vector<TileItem>> lists; long long cycles = 0, part_rows = 0, cost = 0; };   // of the longest list; with the partials' way
+struct TileDeal {
+  std::vector<std::vector<TileItem>> lists;
+  int blocks = 0;                                                          // lists
+  long long cycles = 0, part_rows = 0, cost = 0;                           // of the longest list; with the partials' way
+};
+// With the decode kernels' part behind it, `fetch` cycles on the whole GPU.
+inline long long joint_cost(const TileDeal& d, long long fetch, int sms) {
+  const long long hidden = std::max<long long>(d.cycles - kOwnStart, 0) * (sms - d.blocks) / sms;
+  return d.cost + (fetch > hidden ? fetch - hidden + kOwnTail : 0);
+}
 
 inline long long item_rows(const TileItem& t, const SegmentGeometry& g) { return static_cast<long long>(t.n_tok) * g.group() * (t.flags & kPair ? 2 : 1); }
 
@@ -113,6 +128,7 @@ inline TileDeal deal_whole(const std::vector<TileUnit>& units, int sms, bool kee
   std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return units[x].cycles() > units[y].cycles(); });
   TileDeal d;
   const size_t blocks = std::min<size_t>(units.size(), sms);
+  d.blocks = static_cast<int>(blocks);
   if (keep) d.lists.resize(blocks);
   using Load = std::pair<long long, int>;
   std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least;
@@ -177,6 +193,7 @@ inline TileDeal deal_shares(const std::vector<TileUnit>& units, int sms, int lea
       d.part_rows += n_pieces * rows;
     }
   }
+  d.blocks = lists;
   d.cost = d.cycles + (d.part_rows > 0 ? (prefix ? 0 : kMergeCycles) + partial_cycles(d.part_rows, g.head_dim) : 0);
   return d;
 }
@@ -224,10 +241,11 @@ inline void cut_own(const std::vector<OwnRange>& own, const SegmentGeometry& g, 
   std::stable_sort(out.items.begin(), out.items.end(), [](const WorkItem& x, const WorkItem& y) { return x.kv_len > y.kv_len; });
 }
 
-// The cheapest of: whole, and shares of pieces of at least 2, 4, 8 ... key tiles (fewer pieces leave fewer partials).
-inline TileDeal deal_tiles(const std::vector<TileUnit>& units, int sms, const SegmentGeometry& g, bool prefix, bool keep) {
+// The cheapest of: whole, and shares of pieces of at least 2, 4, 8 ... key tiles (fewer pieces leave fewer partials), and with work
+// for the decode kernels (`fetch`) each of them on fewer blocks too.
+inline TileDeal deal_tiles(const std::vector<TileUnit>& units, long long fetch, int sms, const SegmentGeometry& g, bool prefix, bool keep) {
   if (units.empty()) return TileDeal();
-  int pick = 0, longest = 0;                                               // least tiles of a piece; 0: whole
+  int pick = 0, on = sms, longest = 0;                                     // least tiles of a piece, 0: whole; blocks
   long long total = 0;
   for (const TileUnit& u : units) {
     longest = std::max(longest, u.n_kt);
@@ -237,20 +255,34 @@ inline TileDeal deal_tiles(const std::vector<TileUnit>& units, int sms, const Se
     TileDeal d;
     if (prefix)
       for (const TileUnit& u : units) d.part_rows += item_rows(u.item, g);
+    d.blocks = sms;
     d.cycles = total / sms;
     d.cost = d.cycles + partial_cycles(d.part_rows, g.head_dim);
     return d;
   }
-  long long cost = prefix ? -1 : deal_whole(units, sms, false).cost;
-  // Cuts could gain a fiftieth and their merge's cost at most: whole without reckoning them.  (Many units are level by themselves.)
-  const bool level = cost >= 0 && cost <= total / sms + total / sms / 50 + kMergeCycles;
-  for (int least = kLeastTiles; !level; least *= 2) {
-    const TileDeal d = deal_shares(units, sms, least, g, prefix, false);
-    if ((cost < 0 || d.cost < cost) && d.part_rows <= most_tile_rows(g, sms, prefix)) { cost = d.cost; pick = least; }
-    if (least >= longest) break;
+  const bool narrow = fetch > 0 && units.size() <= static_cast<size_t>(kFewUnits) * sms;
+  long long best = -1;
+  for (int blocks = sms; blocks >= sms / 4; blocks -= std::max(sms / 16, 1)) {
+    if (best >= 0 && total / blocks >= best) break;
+    auto offer = [&](const TileDeal& d, int least) {
+      const long long c = joint_cost(d, fetch, sms);
+      if (best < 0 || c < best) { best = c; pick = least; on = blocks; }
+    };
+    bool level = false;
+    if (!prefix) {
+      const TileDeal d = deal_whole(units, blocks, false);
+      offer(d, 0);
+      // Cuts could gain a fiftieth and their merge's cost at most: whole without reckoning them.  (Many units are level by themselves.)
+      level = d.cost <= total / blocks + total / blocks / 50 + kMergeCycles;
+    }
+    for (int least = kLeastTiles; !level; least *= 2) {
+      const TileDeal d = deal_shares(units, blocks, least, g, prefix, false);
+      if (d.part_rows <= most_tile_rows(g, sms, prefix)) offer(d, least);
+      if (least >= longest) break;
+    }
+    if (!narrow) break;
   }
-  TileDeal d = pick ? deal_shares(units, sms, pick, g, prefix, keep) : deal_whole(units, sms, keep);
-  return d;
+  return pick ? deal_shares(units, on, pick, g, prefix, keep) : deal_whole(units, on, keep);
 }
 
 inline std::vector<TileUnit> tile_units(const std::vector<Segment>& segs, const SegmentGeometry& g, const std::vector<int>& row_token) {
@@ -274,7 +306,9 @@ inline std::vector<TileUnit> tile_units(const std::vector<Segment>& segs, const 
 // What a step would take with these tiles and own ranges.
 inline long long step_cycles(const std::vector<Segment>& segs, const std::vector<OwnRange>& own, const std::vector<int>& row_token, const SegmentGeometry& g,
                              int sms, bool prefix) {
-  return deal_tiles(tile_units(segs, g, row_token), sms, g, prefix, false).cost + own_cycles(own, g) + (prefix && !segs.empty() ? kMergeCycles - kOwnCycles + 2000 : 0);
+  if (segs.empty()) return own_cycles(own, g);
+  const long long fetch = own_fetch(own, g);
+  return joint_cost(deal_tiles(tile_units(segs, g, row_token), fetch, sms, g, prefix, false), fetch, sms) + (prefix ? kMergeCycles : 0);
 }
 
 // Puts everything together.  out.row_token holds the segments' tokens already; `empty`: tokens without keys.
@@ -285,7 +319,7 @@ inline void list_segments(const std::vector<Segment>& segs, const std::vector<Ow
   const int group = g.group();
   const std::vector<TileUnit> units = tile_units(segs, g, out.row_token);
   if (!units.empty()) {
-    const TileDeal deal = deal_tiles(units, sms, g, prefix, true);
+    const TileDeal deal = deal_tiles(units, own_fetch(own, g), sms, g, prefix, true);
     out.n_tile_rows = deal.part_rows;
     for (const auto& list : deal.lists) {
       out.list_first.push_back(static_cast<int>(out.tiles.size()));

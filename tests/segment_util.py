@@ -184,3 +184,14 @@ class Step:
         rest = torch.ones(self.n, dtype=torch.bool, device="cuda")
         rest[rows] = False
         assert torch.equal(out[rest], self.mark[rest]), "rows of no sequence were written"
+
+    def move_behind(self, blocks):
+        """The same step in pools that begin with `blocks` blocks of nobody's."""
+        for name in ("kc", "vc"):
+            small = getattr(self, name)
+            pool = self.torch.empty((blocks * self.bs + small.shape[0], small.shape[1]), device="cuda", dtype=small.dtype)
+            pool[blocks * self.bs:] = small
+            setattr(self, name, pool)
+        self.block_tables += blocks
+        self.slots = [s + blocks * self.bs for s in self.slots]
+        self.num_blocks += blocks

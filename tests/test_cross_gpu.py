@@ -158,3 +158,27 @@ def test_python_refusals(pkv, torch_cuda):
         fresh.attention(*args, step.scale)                       # never built
     with pytest.raises(pkv.PkvError):
         plan.attention(*args, 0.0)
+
+
+@pytest.mark.parametrize("dtype,tiles", [("bf16", "1"), ("bf16", "0"), ("f32", "")])
+def test_pools_of_more_than_four_billion_elements(pkv, torch_cuda, monkeypatch, dtype, tiles):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
+    step = Step(torch_cuda, dtype, WIDE, [70, 1, 3], [500, 900, 129], 16, seed=20)
+    step.move_behind(2 ** 32 // (8 * 128 * 16))
+    run(pkv, step)
+    step.check(pkv)
+
+
+def test_q_of_more_than_two_billion_elements(pkv, torch_cuda):
+    """First and last rows of one long sequence."""
+    torch = torch_cuda
+    qh, kvh, hd = WIDE
+    n, keys = 530001, 200
+    small = Step(torch, "bf16", WIDE, [200], [keys], 16, seed=21)
+    q, out = torch.empty((n, qh * hd), device="cuda", dtype=torch.bfloat16), torch.empty((n, qh * hd), device="cuda", dtype=torch.bfloat16)
+    q.normal_()
+    q[:100], q[-100:] = small.q[:100], small.q[100:]
+    plan = pkv.CrossPlan(n, 1, qh, kvh, hd, 16, q.dtype, num_blocks=small.num_blocks).build_host([n], [keys])
+    plan.attention(q, small.kc, small.vc, small.block_tables, small.table_offset, out, small.scale)
+    small.out = torch.cat([out[:100], out[-100:]])
+    small.check(pkv)

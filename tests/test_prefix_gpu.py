@@ -172,3 +172,12 @@ def test_layer_with_norms_prefix_and_encoder(pkv, torch_cuda, monkeypatch, tiles
         size = torch.cat([(a * c).abs() + (b * s).abs()] * 2, -1).flatten(1) + torch.cat([(b * c).abs() + (a * s).abs()] * 2, -1).flatten(1)
         assert bool(((step.q.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * size).all())
         assert torch.equal(step.vc[slots.long()], v)
+
+
+@pytest.mark.parametrize("tiles", ["1", "0"])
+def test_pools_of_more_than_four_billion_elements(pkv, torch_cuda, monkeypatch, tiles):
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
+    step = make(torch_cuda, "bf16", WIDE, 12, 512, [1 + 30 * i for i in range(12)], 16, 20)
+    step.move_behind(2 ** 32 // (8 * 128 * 16))
+    run(pkv, step, 512)
+    step.check(pkv)

@@ -168,3 +168,26 @@ def test_not_a_number_stays_in_its_head(pkv, torch_cuda):
     assert bad.nonzero().tolist() == [[2, 1]]
     kept = d["kc"][d["slots"].long()].view(5, 2, 64)
     assert torch.isnan(kept).any(-1).nonzero().tolist() == [[3, 0]]
+
+
+@pytest.mark.parametrize("hd", [64, 40])
+@pytest.mark.parametrize("qh,kvh", [(0, 3), (5, 0)])
+def test_only_q_or_only_kv(pkv, torch_cuda, qh, kvh, hd):
+    d = make(torch_cuda, "bf16", qh, kvh, hd, 21, True, seed=12)
+    check(torch_cuda, pkv, d, 21, qh, kvh, hd, 1e-6, "bf16")
+
+
+@pytest.mark.parametrize("hd", [128, 120])
+def test_pools_of_more_than_four_billion_elements(pkv, torch_cuda, hd):
+    torch = torch_cuda
+    qh, kvh, n = 8, 8, 300
+    d = make(torch, "bf16", qh, kvh, hd, n, True, seed=13)
+    k_want, k_size = formula(torch, d, kvh, hd, "k", 1e-6)
+    far = -(-2 ** 32 // (kvh * hd))
+    d["kc"], d["vc"] = (torch.zeros((far + n + 37, kvh * hd), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    d["slots"] += far
+    launch(pkv, d, n, qh, kvh, hd, 1e-6)
+    at = d["slots"].long()
+    near(torch, d["kc"][at], k_want, k_size, "bf16")
+    assert torch.equal(d["vc"][at], d["v"])
+    assert not bool(d["kc"][:far].any()) and not bool(d["vc"][:far].any())

@@ -86,8 +86,8 @@ def launch_rope_store_kv(q, k, v, positions, cos_table, sin_table, slots, k_cach
 
 
 # The checks below run once per call and layer: a few tenths of a microsecond per tensor, attributes looked up once.
-def _wrong(tensors, dtype, device: int, what: str):
-    """Raises the error of the first of `tensors` that is not a contiguous `dtype` tensor of CUDA device `device`."""
+def _wrong(tensors, dtype, device: int, what: str, rows: bool = False):
+    """Raises the error of the first of `tensors` that is not a contiguous (or `rows`) `dtype` tensor of CUDA device `device`."""
     for t in tensors:
         if not t.is_cuda:
             raise ValueError("paged-KV operators take CUDA tensors; there is no CPU path")
@@ -95,7 +95,7 @@ def _wrong(tensors, dtype, device: int, what: str):
             raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
         if t.get_device() != device:
             raise ValueError(f"{what} lie on different devices: {t.get_device()} and {device}")
-        if not t.is_contiguous():
+        if not rows and not t.is_contiguous():
             raise ValueError("paged-KV operators take contiguous tensors")
 
 
@@ -105,10 +105,8 @@ def _check(tensors, dtype, device: int, what: str) -> None:
             _wrong(tensors, dtype, device, what)
 
 
-def _rows(t, cols: int, dtype, device: int, n_rows: int, what: str):
+def _rows(t, cols: int, n_rows: int, what: str):
     """(pointer, elements from one row to the next) of a [rows][cols] tensor whose rows may lie apart."""
-    if t.dtype is not dtype or t.get_device() != device:
-        _wrong((t,), dtype, device, what)
     shape, stride = t.shape, t.stride()      # (size(0) and stride(0) take twice as long)
     if len(shape) != 2 or shape[1] != cols or shape[0] < n_rows or (stride[1] != 1 and cols > 1):
         raise ValueError(f"{what} must be [at least {n_rows}][{cols}] with contiguous rows, not {tuple(shape)} with strides {stride}")
@@ -140,17 +138,29 @@ def launch_qk_norm_rope_store_kv(q, k, v, q_weight, k_weight, eps: float, positi
     rotation, append, in one pass.  q, k and v are [rows][heads*head_dim] and may be column ranges of one
     projection's output; q_out (contiguous) receives the rotated q.  Rows whose position is outside the tables are
     left alone, rows whose slot is outside the pools bring no K/V (padded steps)."""
-    fn, call = _fn("pkv_qk_norm_rope_append_", k_cache)
     device, dtype = k_cache.get_device(), k_cache.dtype
+    if device < 0:
+        _wrong((k_cache,), dtype, device, "pools")
     other = _this_device(device)
     if other is not None:
         with other:
             return launch_qk_norm_rope_store_kv(q, k, v, q_weight, k_weight, eps, positions, cos_table, sin_table, slots, q_out, k_cache,
                                                 v_cache, n_tokens, q_heads, kv_heads, head_dim, stream)
     q_dim, kv_dim = q_heads * head_dim, kv_heads * head_dim
-    _check((q_weight, k_weight, q_out, k_cache, v_cache), dtype, device, "weights, q_out and pools")
-    _check((positions, slots), _torch.int32, device, "positions and slots")
-    _check((cos_table, sin_table), _torch.float32, device, "cos and sin tables")
+    i32, f32 = _torch.int32, _torch.float32
+    if not (q.dtype is dtype and k.dtype is dtype and v.dtype is dtype and q_weight.dtype is dtype and k_weight.dtype is dtype
+            and q_out.dtype is dtype and v_cache.dtype is dtype and positions.dtype is i32 and slots.dtype is i32
+            and cos_table.dtype is f32 and sin_table.dtype is f32
+            and device == q.get_device() == k.get_device() == v.get_device() == q_weight.get_device() == k_weight.get_device()
+            == positions.get_device() == cos_table.get_device() == sin_table.get_device() == slots.get_device()
+            == q_out.get_device() == v_cache.get_device()
+            and q_weight.is_contiguous() and k_weight.is_contiguous() and positions.is_contiguous() and cos_table.is_contiguous()
+            and sin_table.is_contiguous() and slots.is_contiguous() and q_out.is_contiguous() and k_cache.is_contiguous()
+            and v_cache.is_contiguous()):
+        _wrong((q_weight, k_weight, q_out, k_cache, v_cache), dtype, device, "weights, q_out and pools")
+        _wrong((positions, slots), i32, device, "positions and slots")
+        _wrong((cos_table, sin_table), f32, device, "cos and sin tables")
+        _wrong((q, k, v), dtype, device, "q, k and v", rows=True)
     tables, n_pool = cos_table.shape, k_cache.numel()
     if tables != sin_table.shape or len(tables) != 2 or 2 * tables[1] != head_dim:
         raise ValueError(f"cos and sin tables must both be [positions][{head_dim // 2}]")
@@ -160,9 +170,10 @@ def launch_qk_norm_rope_store_kv(q, k, v, q_weight, k_weight, eps: float, positi
         raise ValueError(f"fewer rows than n_tokens = {n_tokens}")
     if v_cache.numel() != n_pool:
         raise ValueError("K and V pools differ in size")
-    qp, qs = _rows(q, q_dim, dtype, device, n_tokens, "q")
-    kp, ks = _rows(k, kv_dim, dtype, device, n_tokens, "k")
-    vp, vs = _rows(v, kv_dim, dtype, device, n_tokens, "v")
+    fn, call = _fn("pkv_qk_norm_rope_append_", k_cache)
+    qp, qs = _rows(q, q_dim, n_tokens, "q")
+    kp, ks = _rows(k, kv_dim, n_tokens, "k")
+    vp, vs = _rows(v, kv_dim, n_tokens, "v")
     st = call(qp, kp, vp, qs, ks, vs, q_weight.data_ptr(), k_weight.data_ptr(), eps, positions.data_ptr(), cos_table.data_ptr(),
               sin_table.data_ptr(), tables[0], slots.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
               n_pool // max(kv_dim, 1), n_tokens, q_heads, kv_heads, head_dim, _stream_of(stream, device))

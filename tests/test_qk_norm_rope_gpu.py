@@ -191,3 +191,23 @@ def test_pools_of_more_than_four_billion_elements(pkv, torch_cuda, hd):
     near(torch, d["kc"][at], k_want, k_size, "bf16")
     assert torch.equal(d["vc"][at], d["v"])
     assert not bool(d["kc"][:far].any()) and not bool(d["vc"][:far].any())
+
+
+def test_python_refusals(pkv, torch_cuda):
+    torch = torch_cuda
+    qh, kvh, hd, n = 4, 2, 64, 9
+    good = make(torch, "bf16", qh, kvh, hd, n, True, seed=14)
+    for name in good:
+        bad = dict(good, **{name: good[name].cpu()})
+        with pytest.raises(ValueError):
+            launch(pkv, bad, n, qh, kvh, hd, 1e-6)
+        with pytest.raises(TypeError):
+            launch(pkv, dict(good, **{name: good[name].to(torch.float64)}), n, qh, kvh, hd, 1e-6)
+    with pytest.raises(ValueError):
+        launch(pkv, {k: v.cpu() for k, v in good.items()}, n, qh, kvh, hd, 1e-6)
+    for name, bad in (("q", good["q"][:, :-1]), ("k", good["k"][:5]), ("v", good["v"][:, ::2]), ("qw", good["qw"][:32]), ("pos", good["pos"][:8]),
+                      ("slots", good["slots"][::2]), ("cos", good["cos"][:, :16]), ("sin", good["sin"][:600]), ("qo", good["qo"][:8]),
+                      ("vc", good["vc"][:-1]), ("kc", good["kc"][:, :64])):
+        with pytest.raises(ValueError):
+            launch(pkv, dict(good, **{name: bad}), n, qh, kvh, hd, 1e-6)
+    check(torch, pkv, good, n, qh, kvh, hd, 1e-6, "bf16")

@@ -202,3 +202,14 @@ def test_plans_do_not_depend_on_what_was_planned_before(pkv):
     a, c = Image(first, plan), Image(b.staging, again)
     for name in ("items", "tiles", "merge", "pos"):
         assert np.array_equal(getattr(a, name), getattr(c, name)), name
+
+
+def test_tensors_without_a_device_are_refused(pkv):
+    """No CPU path: the Python calls say so before anything is launched."""
+    torch = pytest.importorskip("torch")
+    x = torch.zeros(2, 128, dtype=torch.bfloat16)
+    i, table = torch.zeros(2, dtype=torch.int32), torch.zeros(4, 32)
+    with pytest.raises(ValueError, match="no CPU path"):
+        pkv.launch_qk_norm_rope_store_kv(x, x, x, x[0, :64], x[0, :64], 1e-6, i, table, table, i, x, x, x, 2, 2, 2, 64)
+    with pytest.raises(ValueError, match="no CPU path"):
+        pkv.CrossPlan(2, 1, 2, 2, 64, 16, torch.bfloat16, workspace=torch.zeros(1 << 20, dtype=torch.uint8))

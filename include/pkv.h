@@ -467,7 +467,8 @@ int pkv_prefill_attn_f16(const void* q, const void* k_cache, const void* v_cache
  * to its own position only.  (pkv_decode_plan_host_shared finds common prefixes by itself and
  * reads them once per four tokens.)
  *
- * out may not overlap q or the pools.  kv_len and token_pos + 1 are 2^30 at most.
+ * out may not overlap q or the pools.  kv_len and token_pos + 1 are 2^30 at most; a step of more
+ * than about a second's work on the tensor cores is refused.
  *
  * Ahead of a call: the plan, block_tables, table_offset and token_seq are read while the
  * launch directly before it may still be running (q, K and V are not), so they must have been

@@ -66,6 +66,8 @@ constexpr int kProducer = 16, kIssuer = 17, kRowsLoader = 18, kProducerV = 19;
 constexpr int kBlockBytes = 128 * 128;                   // 128 rows x 64 16-bit elements: one operand block
 constexpr uint32_t kGroupCols = 256, kColO = 128;        // tensor memory of a group: S, then O ...
 constexpr float kRescale = 8.f;                          // in log2 units: P stays below 2^8
+// A blocking poll takes 2 us.  Waits for a tile: 0.27 s; waits that may span whole items, or a block's list of them (kMostListCycles): 2.1 s.
+constexpr uint32_t kItemPolls = 1u << 20;
 constexpr int kBoxRows = 64;                             // rows of Q, at most, that a box of several tokens brings
 constexpr int kMinTileTokens = 2, kManyTileTokens = 32;  // sequences with fewer tokens always go to the decode kernels, with as many never
 
@@ -203,9 +205,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int n_items = __ldg(a.list_first + blockIdx.x + 1) - __ldg(a.list_first + blockIdx.x);
 
   bool dead = false;
-  auto WAIT = [&](uint32_t bar, uint32_t parity) {
+  auto WAIT = [&](uint32_t bar, uint32_t parity, uint32_t polls = 1u << 17) {
     if (dead) return;
-    if (!mbar_wait(bar, parity)) {
+    if (!mbar_wait(bar, parity, polls)) {
       dead = true;
       atomicOr(&g_pkv_tile_error, kErrTileWait);
       if (a.host_err) {
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (lane < boxes) token = __ldg(a.row_token + it.tok0 + first_of(lane));
         if (r == 0) after_previous();
         if (lane == 0) {
-          WAIT(BAR(Q_EMPTY + qb), ((r / S::kQBufs) & 1) ^ 1);
+          WAIT(BAR(Q_EMPTY + qb), ((r / S::kQBufs) & 1) ^ 1, kItemPolls);
           if (!dead) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(heads * (many * a.box_tokens + boxes - many) * a.group) * 128u * S::kHalves);
         }
         dead = __shfl_sync(0xffffffffu, dead ? 1 : 0, 0) != 0;
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       float m_used = -INFINITY;
       float2 l = both(0.f);
       for (int t = pair & g; t < n; t += step, ++done) {
-        WAIT(BAR(S_FULL + g), done & 1);
+        WAIT(BAR(S_FULL + g), done & 1, kItemPolls);            // (the second group lets items of one group pass)
         tc::fence_after();
         const int valid = kv_len - (t >> pair) * kTileKeys;   // keys of this tile, if fewer than kTileKeys
         const bool opening = t < step;
@@ -775,6 +777,8 @@ int write_image(const char* fn, Kind kind, const SegmentGeometry& g, const Segme
                                                             l.merge.size(), static_cast<size_t>(l.n_tile_rows), static_cast<size_t>(l.n_parts)});
   if (o.total > workspace_bytes) return fail(PKV_E_WORKSPACE, "%s: workspace of %zu bytes; this step takes %zu", fn, workspace_bytes, o.total);
   if (o.image > staging_bytes) return fail(PKV_E_WORKSPACE, "%s: staging buffer of %zu bytes; this step's plan takes %zu", fn, staging_bytes, o.image);
+  if (l.list_cycles > kMostListCycles)
+    return fail(PKV_E_UNSUPPORTED, "%s: more than a second's work (%.3g cycles) for one call; split the step", fn, static_cast<double>(l.list_cycles));
   if (l.n_tile_rows > 0x7fffffffll || static_cast<long long>(l.items.size()) * g.kv_heads > 0x7fffffffll)
     return fail(PKV_E_UNSUPPORTED, "%s: more than 2^31 - 1 work items or partial rows", fn);
   char* img = static_cast<char*>(h_staging);
@@ -856,7 +860,7 @@ int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* 
     l.row_token.clear();
     for (int s = 0; s < n_seqs; ++s) {
       if (q_len[s] == 0 || kv_len[s] == 0) continue;
-      const bool tiled = g.tiles() && q_len[s] >= fewest;
+      const bool tiled = g.tiles() && q_len[s] >= fewest && kv_len[s] <= kMostTileKeys;
       if (tiled) segs.push_back(Segment{static_cast<int>(l.row_token.size()), q_len[s], kv_len[s], ~s});
       for (int t = start[s]; t < start[s] + q_len[s]; ++t) {
         if (tiled) l.row_token.push_back(t);
@@ -896,7 +900,7 @@ int plan_prefix(const char* fn, const int* token_pos, int prefix_len, const Segm
   int st = check_geometry(fn, g);
   if (st != PKV_OK) return st;
   // the decode kernels fetch boxes of 16 slots: a token's own keys begin on a multiple of 16
-  const int shared = g.tiles() ? prefix_len & ~15 : 0;
+  const int shared = g.tiles() && prefix_len <= kMostTileKeys ? prefix_len & ~15 : 0;
   std::vector<int> none, pos(token_pos, token_pos + g.n_tokens), empty;
   std::vector<Segment> segs;
   std::vector<OwnRange> own;

@@ -35,6 +35,9 @@ namespace pkv {
 
 constexpr int kTileRows = 256;      // rows of a tile item: two groups of 128
 constexpr int kTileKeys = 128;      // keys per step of the tile kernel
+// What its waits for whole items allow (2.1 s): keys of an item, walked in 0.6 s, and a block's list, in cycles (1.1 s).
+constexpr int kMostTileKeys = 1 << 25;
+constexpr long long kMostListCycles = 2000000000ll;
 
 // Tokens row_token[tok0 .. tok0 + n_tok - 1] of a segment: row r of the item is token r / group, head r % group.
 struct TileItem {
@@ -73,6 +76,7 @@ struct SegmentLists {
   std::vector<TileItem> tiles;
   std::vector<MergeRow> merge;
   long long n_tile_rows = 0;
+  long long list_cycles = 0;        // of the longest list
   int n_parts = 0, chunk = 0, longest = 0;
 };
 
@@ -321,6 +325,7 @@ inline void list_segments(const std::vector<Segment>& segs, const std::vector<Ow
   if (!units.empty()) {
     const TileDeal deal = deal_tiles(units, own_fetch(own, g), sms, g, prefix, true);
     out.n_tile_rows = deal.part_rows;
+    out.list_cycles = deal.cycles;
     for (const auto& list : deal.lists) {
       out.list_first.push_back(static_cast<int>(out.tiles.size()));
       out.tiles.insert(out.tiles.end(), list.begin(), list.end());

@@ -213,3 +213,17 @@ def test_tensors_without_a_device_are_refused(pkv):
         pkv.launch_qk_norm_rope_store_kv(x, x, x, x[0, :64], x[0, :64], 1e-6, i, table, table, i, x, x, x, 2, 2, 2, 64)
     with pytest.raises(ValueError, match="no CPU path"):
         pkv.CrossPlan(2, 1, 2, 2, 64, 16, torch.bfloat16, workspace=torch.zeros(1 << 20, dtype=torch.uint8))
+
+
+def test_waits_are_long_enough_for_what_is_planned(pkv):
+    """Items that a bounded wait could take for a lost one are not planned: very long ones go to the decode kernels, a call of seconds
+    is refused."""
+    E = pkv._lib
+    st, plan, _ = cross(pkv, [300], [2 ** 25], 300, GEOMS[2])
+    assert st == 0 and plan.n_tiles > 0
+    st, plan, _ = cross(pkv, [300], [2 ** 25 + 1], 300, GEOMS[2])
+    assert st == 0 and plan.n_tiles == 0 and plan.n_items >= 300
+    st, plan, _ = prefix(pkv, [2 ** 25 + 40] * 5, 2 ** 25 + 16, GEOMS[2])
+    assert st == 0 and plan.n_tiles == 0
+    st, plan, _ = cross(pkv, [2 ** 15], [2 ** 25], 2 ** 15, GEOMS[2])
+    assert st == E.PKV_E_UNSUPPORTED and "split the step" in pkv._lib.last_error()

@@ -206,15 +206,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   bool dead = false;
   auto WAIT = [&](uint32_t bar, uint32_t parity, uint32_t polls = 1u << 17) {
-    if (dead) return;
-    if (!mbar_wait(bar, parity, polls)) {
-      dead = true;
-      atomicOr(&g_pkv_tile_error, kErrTileWait);
-      if (a.host_err) {
-        *reinterpret_cast<volatile unsigned int*>(a.host_err) = kErrTileWait;
-        __threadfence_system();
-      }
-    }
+    if (!dead) dead = !mbar_wait(bar, parity, polls);
   };
 
   if (warp >= kProducer) {
@@ -589,6 +581,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
       tc::fence_before();
+    }
+  }
+  if (dead) {
+    atomicOr(&g_pkv_tile_error, kErrTileWait);
+    if (a.host_err) {
+      *reinterpret_cast<volatile unsigned int*>(a.host_err) = kErrTileWait;
+      __threadfence_system();
     }
   }
   tc::fence_before();

@@ -28,10 +28,10 @@
 // P is rounded to 16 bits for the second product (the sums are of the unrounded ones), as the operands of the
 // tensor cores are; scores, sums and accumulators are fp32.
 //
-// Measured on B200: a key tile of both groups takes about 3,600 cycles at head_dim 128 (products 2,048, exponentials 2,048, the rest a
-// group's chain of load, maximum, exponentials, store that one other group does not cover) and 3,350 at 64 (products 1,024; the issuing
+// Measured on B200: a key tile of both groups takes about 3,500 cycles at head_dim 128 (products 2,048, exponentials 2,048, the rest a
+// group's chain of load, maximum, exponentials, store that one other group does not cover) and 3,200 at 64 (products 1,024; the issuing
 // warp's waits); an item's start and end 5,000.  4 sequences of 1,000 - 2,048 tokens and 4,000 - 6,500 keys, 32/8 heads of 128 dims: 593 us,
-// 1,155 TFLOP/s.  24 of 3 - 448 tokens and 100 - 1,500 keys, 16/16 heads of 64: 52 us.
+// 1,155 TFLOP/s, in a burst (650 under the power cap).  24 of 3 - 448 tokens and 100 - 1,500 keys, 16/16 heads of 64: 50 us.
 //
 // Blocks are persistent, one on an SM, each with a list of items of its own.  Every wait is bounded: one that runs
 // out sets bit 32 of the error word and the block winds down.
@@ -208,6 +208,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   auto WAIT = [&](uint32_t bar, uint32_t parity, uint32_t polls = 1u << 17) {
     if (!dead) dead = !mbar_wait(bar, parity, polls);
   };
+  // Without the first look, for waits that are waits nearly always: it only takes the others' cycles and power.
+  auto BLOCK = [&](uint32_t bar, uint32_t parity, uint32_t polls = 1u << 17) {
+    if (dead) return;
+    bool there = false;
+    for (uint32_t i = 0; i < polls && !there; ++i) there = mbar_try_wait(bar, parity);
+    dead = !there;
+  };
 
   if (warp >= kProducer) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
@@ -352,7 +359,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         };
         // Products of one thread run in order: where P lies over S, the group's next scores overwrite it behind these.
         auto values = [&](int g, uint32_t v_addr, bool first, bool final) {
-          WAIT(BAR(P_FULL + g), (done >> g) & 1);
+          // (a look first: 242 us against 247 for full tiles at 64 dims, 660 against 647 for the largest case at 128)
+          if constexpr (D == 64) WAIT(BAR(P_FULL + g), (done >> g) & 1);
+          else BLOCK(BAR(P_FULL + g), (done >> g) & 1);
           tc::fence_after();
           uint32_t v_lo = v_addr >> 4, t = tmem + g * kGroupCols;
           asm volatile("" : "+r"(v_lo), "+r"(t));
@@ -428,7 +437,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       float m_used = -INFINITY;
       float2 l = both(0.f);
       for (int t = pair & g; t < n; t += step, ++done) {
-        WAIT(BAR(S_FULL + g), done & 1, kItemPolls);            // (the second group lets items of one group pass)
+        BLOCK(BAR(S_FULL + g), done & 1, kItemPolls);            // (the second group lets items of one group pass)
         tc::fence_after();
         const int valid = kv_len - (t >> pair) * kTileKeys;   // keys of this tile, if fewer than kTileKeys
         const bool opening = t < step;
@@ -464,7 +473,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           // arrived, were issued behind it; so is P's place.
           if constexpr (S::kLead > 1) {
             if (!opening) {
-              WAIT(BAR(O_FULL + g), (done & 1) ^ 1);
+              BLOCK(BAR(O_FULL + g), (done & 1) ^ 1);
               tc::fence_after();
             }
           }
@@ -502,13 +511,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         } else if constexpr (S::kLead > 1) {
           // no row of this warp is the item's: it keeps step only
-          if (!opening) WAIT(BAR(O_FULL + g), (done & 1) ^ 1);
+          if (!opening) BLOCK(BAR(O_FULL + g), (done & 1) ^ 1);
         }
         if (t + step >= n && valid < kTileKeys && (g == 0 || pair)) {
           // Keys past the end: their P is zero, but the V rows behind them are whatever the pool or the ring held.  Cleared
           // before the group's threads report the tile's P, so that 0 * x stays 0.
           const uint32_t last_v = e0 - 1 - pair + (pair & g);  // ring entry of the group's last V tile
-          WAIT(BAR(KV_FULL + last_v % NS), (last_v / NS) & 1);
+          BLOCK(BAR(KV_FULL + last_v % NS), (last_v / NS) & 1);
           if (r_in >= valid && half < S::kHalves) {
             unsigned char* v = base_ptr + S::kRing + (last_v % NS) * S::kTile + half * kBlockBytes + r_in * 128;
 #pragma unroll
@@ -546,7 +555,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           to = reinterpret_cast<unsigned long long>(static_cast<T*>(a.out) + (static_cast<size_t>(token) * a.q_heads + head) * D + half * (D / 2));
         }
       }
-      WAIT(BAR(O_FULL + g), S::kLead > 1 ? (done & 1) ^ 1 : items & 1);
+      BLOCK(BAR(O_FULL + g), S::kLead > 1 ? (done & 1) ^ 1 : items & 1);
       ++items;
       tc::fence_after();
       if (!working) continue;

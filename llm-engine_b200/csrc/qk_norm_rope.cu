@@ -12,7 +12,7 @@
 // one token, which share the token's cos / sin: 8,191 tokens of 32/8 heads of 128, bf16 (206 MB), 48 us with one head a
 // lane, 43 with two, 71 with four (94 registers).  Steps whose rows do not fit L2 read and write them as data that is
 // not used again: 36.5 us, 5.6 TB/s; 1,024 tokens lose a tenth that way (6.2 and 6.9), and the launch behind them finds
-// its q, K and V in L2.
+// its q, K and V in L2.  Sending for the rows before the position is known: 36.2 -> 38.2 us.
 #include "common.cuh"
 #include "launch_util.hpp"
 #include "status.hpp"

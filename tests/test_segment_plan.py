@@ -227,3 +227,19 @@ def test_waits_are_long_enough_for_what_is_planned(pkv):
     assert st == 0 and plan.n_tiles == 0
     st, plan, _ = cross(pkv, [2 ** 15], [2 ** 25], 2 ** 15, GEOMS[2])
     assert st == E.PKV_E_UNSUPPORTED and "split the step" in pkv._lib.last_error()
+
+
+def test_recorded_give_up_is_reported_once(pkv):
+    """What a kernel recorded is told by the next call of either form, which enqueues nothing; empty steps never look."""
+    L, E = pkv.lib(), pkv._lib
+    _, plan, _ = cross(pkv, [3, 40], [50, 700], 43, GEOMS[0])
+    nothing = (C.byref(plan), *[None] * 6, 1.0, None, 0, None)
+    _, other, _ = prefix(pkv, [600] * 9, 512, GEOMS[0])
+    _, empty, _ = cross(pkv, [0], [5], 2, GEOMS[0])
+    assert L.pkv_debug_set_reported_flags(32) == 0
+    assert L.pkv_cross_attn_bf16(C.byref(empty), *[None] * 6, 1.0, None, 0, None) == 0
+    assert L.pkv_cross_attn_bf16(*nothing) == E.PKV_E_CUDA and "0x20" in E.last_error()
+    assert L.pkv_cross_attn_bf16(*nothing) == E.PKV_E_ARG            # cleared by the report: as far as the pointers
+    assert L.pkv_debug_set_reported_flags(32) == 0
+    assert L.pkv_prefix_attn_f16(C.byref(other), *[None] * 7, 1.0, None, 0, None) == E.PKV_E_CUDA
+    assert L.pkv_prefix_attn_f16(C.byref(other), *[None] * 7, 1.0, None, 0, None) == E.PKV_E_ARG

@@ -467,6 +467,9 @@ int pkv_prefill_attn_f16(const void* q, const void* k_cache, const void* v_cache
  * to its own position only.  (pkv_decode_plan_host_shared finds common prefixes by itself and
  * reads them once per four tokens.)
  *
+ * Scores are finite where a row sees the key (slots that none sees may hold anything, NaN too);
+ * with infinite ones a row may come out as NaN, as in pkv_decode_attn_*.
+ *
  * out may not overlap q or the pools.  kv_len and token_pos + 1 are 2^30 at most; a step of more
  * than about a second's work on the tensor cores is refused.
  *

@@ -481,7 +481,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             m_used = mx;
           } else if (__any_sync(0xffffffffu, (mx - m_used) * sl2 > kRescale)) {
             const float m_new = (mx - m_used) * sl2 > kRescale ? mx : m_used;
-            const float f = ex2((m_used - m_new) * sl2);
+            // (one row's growth rescales the warp's 32: the others keep theirs, which may still be -inf, by a factor of exactly one)
+            const float f = m_new == m_used ? 1.f : ex2((m_used - m_new) * sl2);
             m_used = m_new;
             l.x *= f;
             l.y *= f;

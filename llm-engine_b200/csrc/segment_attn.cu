@@ -1018,7 +1018,8 @@ int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const v
   }
   if (plan->n_merged > 0) {
     MergeArgs m{reinterpret_cast<const MergeRow*>(ws + plan->off_merge), plan->n_merged, plan->q_heads, group, D, tile_ml, tile_acc, ml, acc, out};
-    const int vec = D % 4 == 0 ? 4 : 1;
+    // four values in one store where every row of out begins on a multiple of them (rows of other than 16-byte multiples may begin anywhere)
+    const int vec = D % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0 ? 4 : 1;
     const long long blocks = (static_cast<long long>(plan->n_merged) * group * (D / vec) + kMergeThreads - 1) / kMergeThreads;
     if (blocks > 0x7fffffffll) return fail(PKV_E_UNSUPPORTED, "%s: %lld blocks to merge", fn, blocks);
     auto kern = vec == 4 ? (log2_domain ? segment_merge_kernel<T, true, 4> : segment_merge_kernel<T, false, 4>)

@@ -46,3 +46,36 @@ def test_rows_of_a_warp_without_a_finite_score_yet(pkv, torch_cuda, monkeypatch,
     bad = ~((step.out.double() - want).abs() <= bound)
     assert not bool(bad.any()), f"{int(bad.any(1)[late].sum())} late rows and {int(bad.any(1)[~late].sum())} others of {step.n}"
     assert pkv.debug_device_flags() == 0
+
+
+def off_by(torch, t, elements):
+    """The same values, `elements` past a 16-byte boundary."""
+    store = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)
+    at = store[elements:elements + t.numel()].view(t.shape)
+    at.copy_(t)
+    return at
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("geom", [(6, 2, 36), (4, 4, 20), (3, 1, 100)])
+@pytest.mark.parametrize("elements", [1, 2, 3, 4])
+def test_rows_of_other_than_16_byte_multiples_may_begin_anywhere(pkv, torch_cuda, dtype, geom, elements):
+    """Heads of 8-byte multiples in tensors that are aligned to an element only; tokens cut in pieces and tokens without keys, which the
+    merge writes."""
+    torch = torch_cuda
+    step = Step(torch, dtype, geom, [1, 2, 1], [3000, 0, 900], 16, seed=elements)
+    for name in ("q", "kc", "vc", "out", "mark"):
+        setattr(step, name, off_by(torch, getattr(step, name), elements))
+    plan = cross(pkv, step)
+    assert plan.plan.n_parts > 0 and plan.plan.n_merged > 2 * step.kvh
+    attend(plan, step)
+    step.check(pkv)
+
+    step = Step(torch, dtype, geom, [1] * 3, [2500, 2401, 2900], 16, seed=elements, shared=2400)
+    for name in ("q", "kc", "vc", "out", "mark"):
+        setattr(step, name, off_by(torch, getattr(step, name), elements))
+    plan = pkv.PrefixPlan(step.n, *geom, 16, step.q.dtype, num_blocks=step.num_blocks).build_host([k - 1 for k in step.kv_len], 2400)
+    assert plan.plan.n_merged > 0
+    plan.attention(step.q, step.kc, step.vc, step.block_tables, step.table_offset, torch.arange(3, device="cuda", dtype=torch.int32), step.out,
+                   step.scale)
+    step.check(pkv)

@@ -85,6 +85,12 @@ int pkv_debug_set_reported_flags(unsigned int flags);
  * ordinary form, and this counter is how a test tells the two apart.  No llm-engine counterpart. */
 unsigned long long pkv_debug_cluster_launches(void);
 
+/* Whether the device has come past a CUDA event (a cudaEvent_t): 1 or 0, or a negative status; with `wait`
+ * the call returns 1 once it has.  For callers that record one behind a plan's upload and write the staging
+ * buffer anew: unlike the runtime's own query it may run while a stream is being captured, by this thread
+ * or another (the event must have been recorded outside the capture).  No llm-engine counterpart. */
+int pkv_event_passed(void* event, int wait);
+
 /* ----------------------------------------------------------- K/V append ----
  * K/V append.  Replaces engine::launch_store_kv (include/engine/cuda_kernels.h:43-45,
  * src/kernels/store_kv.cu:20-36) and the CPU memcpy pair

@@ -74,3 +74,15 @@ extern "C" int pkv_debug_set_reported_flags(unsigned int flags) {
   pkv::g_plain |= flags;
   return PKV_OK;
 }
+
+extern "C" int pkv_event_passed(void* event, int wait) {
+  if (!event) return pkv::fail(PKV_E_ARG, "pkv_event_passed: null event");
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;     // (else a capture under way would end with an error)
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  const cudaError_t e = wait ? cudaEventSynchronize(static_cast<cudaEvent_t>(event)) : cudaEventQuery(static_cast<cudaEvent_t>(event));
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e == cudaSuccess) return 1;
+  cudaGetLastError();
+  if (e == cudaErrorNotReady) return 0;
+  return pkv::fail(PKV_E_CUDA, "pkv_event_passed: %s", cudaGetErrorString(e));
+}

@@ -325,10 +325,61 @@ class DecodePlan:
         _lib.check(fn, st)
 
 
+def _passed(event, wait: bool) -> bool:
+    """Whether the GPU has come past `event`, inside a stream capture too (torch's own query ends one)."""
+    return bool(_lib.check("pkv_event_passed", _lib.lib().pkv_event_passed(event.cuda_event, wait)))
+
+
+def _mark(event, stream, device: int):
+    """`event`, recorded behind what `stream` (None, a stream or its handle) of the current device holds so far; what a stream that is being
+    captured holds runs with the graph only, and the event stays where it was."""
+    import torch
+    if stream is not None and not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+        if not torch.cuda.is_current_stream_capturing():
+            event = event or torch.cuda.Event()
+            event.record()
+    return event
+
+
+class _Staging:
+    """Pinned memory that a plan is written to on the host and uploaded from.  A stream runs the upload when it gets there, perhaps
+    after the next step's lengths are known or the plan object is gone, and torch's allocator does not know of it: until then the bytes
+    are neither written again (writable) nor given back (the owner may drop them at any time)."""
+    _left = []      # (event, bytes) whose owners are gone
+
+    def __init__(self, n: int):
+        import torch
+        pending = []
+        while _Staging._left:
+            try:
+                left = _Staging._left.pop()          # (one thread's at a time)
+            except IndexError:
+                break
+            if not _passed(left[0], False):
+                pending.append(left)
+        _Staging._left.extend(pending)
+        self.bytes = torch.empty(max(n, 256), dtype=torch.uint8, pin_memory=torch.cuda.is_available())
+        self._sent = None
+
+    def writable(self) -> None:
+        if self._sent is not None:
+            _passed(self._sent, True)
+
+    def sent(self, stream, device: int) -> None:
+        self._sent = _mark(self._sent, stream, device)
+
+    def __del__(self, left=_left):
+        if getattr(self, "_sent", None) is not None:
+            left.append((self._sent, self.bytes))
+
+
 class _SegmentPlan:
     """Work list of attention in which many rows see the same keys, built once per step on the host and used by
     every layer's call (include/pkv.h, pkv_segment_plan).  Its calls share one workspace: those that may
-    overlap on the GPU need a plan each."""
+    overlap on the GPU need a plan each.  A plan may be made anew, or dropped, while the GPU still works on earlier calls; a graph
+    that captured its calls needs it for as long as it is replayed."""
 
     def __init__(self, workspace_bytes, n_tokens: int, q_heads: int, kv_heads: int, head_dim: int, block_size: int, dtype,
                  num_blocks: int, workspace, device):
@@ -338,11 +389,13 @@ class _SegmentPlan:
         self.n_tokens, self.q_heads, self.kv_heads, self.head_dim = n_tokens, q_heads, kv_heads, head_dim
         self.block_size, self.dtype, self.num_blocks = block_size, dtype, num_blocks
         L = _lib.lib()
+        self._streams = None        # handles of the streams that torch's allocator knows to use the workspace; the caller's own is the caller's
         if workspace is None:
             workspace = torch.empty(max(int(getattr(L, workspace_bytes)(n_tokens, q_heads, kv_heads, head_dim)), 256), dtype=torch.uint8, device=device)
+            self._streams = {torch.cuda.current_stream(workspace.device).cuda_stream}
         self.workspace = workspace
-        n = max(int(L.pkv_segment_staging_bytes(n_tokens, q_heads, kv_heads)), 256)
-        self.staging = torch.empty(n, dtype=torch.uint8, pin_memory=torch.cuda.is_available())
+        self._staging = _Staging(int(L.pkv_segment_staging_bytes(n_tokens, q_heads, kv_heads)))
+        self.staging = self._staging.bytes
         self.plan = _lib.SegmentPlan()
         self._plan_ref = C.byref(self.plan)
         self._device, self._ws = workspace.get_device(), (_ptr(workspace), workspace.numel())
@@ -352,15 +405,27 @@ class _SegmentPlan:
         return self.q_heads, self.kv_heads, self.head_dim, self.block_size, self.dtype.itemsize
 
     def _build(self, name, image: bool, *args, stream=None):
+        self._staging.writable()
         where = (self.staging.data_ptr(), self.staging.numel())
         L = _lib.lib()
         if image:
             st = getattr(L, name + "_image")(*args, *where, self.workspace.numel(), C.byref(self.plan))
         else:
-            with _this_device(self.workspace.get_device()) or contextlib.nullcontext():
+            device = self.workspace.get_device()
+            with _this_device(device) or contextlib.nullcontext():
                 st = getattr(L, name)(*args, *where, _ptr(self.workspace), self.workspace.numel(), _stream(stream), C.byref(self.plan))
+                self._staging.sent(stream, device)
+                self._used_on(stream, device)
         _lib.check(name, st)
         self.plan.num_blocks = self.num_blocks
+
+    def _used_on(self, stream, device: int) -> None:
+        """Dropped, the workspace is not handed out again before `stream` is done with it.  (Of a bare handle nobody knows how long its
+        stream lives: there the plan has to outlive the calls.)"""
+        handle = _stream_of(stream, device)
+        if self._streams is not None and handle not in self._streams and (stream is None or hasattr(stream, "cuda_stream")):
+            self._streams.add(handle)
+            self.workspace.record_stream(_torch.cuda.current_stream(device) if stream is None else stream)
 
     def _run(self, op, q, k_cache, v_cache, out, ints, scale, stream):
         """One attention call: pointers of q, the pools, the index arrays and out, in the order of the C signatures."""
@@ -374,8 +439,11 @@ class _SegmentPlan:
         if q.numel() < self._out_elems or out.numel() < self._out_elems:
             raise ValueError(f"q and out must have {self.n_tokens} rows of {self.q_heads} heads")
         fn, call = _fn(op, k_cache)
+        handle = _stream_of(stream, device)
+        if self._streams is not None and handle not in self._streams:
+            self._used_on(stream, device)
         st = call(self._plan_ref, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *[t.data_ptr() for t in ints], out.data_ptr(), scale,
-                  *self._ws, _stream_of(stream, device))
+                  *self._ws, handle)
         if st:
             _lib.check(fn, st)
 
@@ -399,14 +467,15 @@ class CrossPlan(_SegmentPlan):
 
     def build_host(self, q_len, kv_len, q_start=None, stream=None) -> "CrossPlan":
         """q_len, kv_len, q_start: per sequence, on the host; without q_start the rows are packed one sequence behind
-        the other.  The staging buffer belongs to the upload until it has run."""
+        the other.  Waits, if need be, until the plan's last upload has run."""
         arrays = self._lengths(q_len, kv_len, q_start)
         self._build("pkv_cross_plan_host", False, *[None if a is None else a.ctypes.data for a in arrays], self.n_seqs, self.n_tokens,
                     *self._geometry(), stream=stream)
         return self
 
     def build_host_image(self, q_len, kv_len, q_start=None) -> int:
-        """The plan without the upload: bytes of self.staging that must reach the start of self.workspace."""
+        """The plan without the upload: bytes of self.staging that must reach the start of self.workspace, before the plan
+        is made anew."""
         arrays = self._lengths(q_len, kv_len, q_start)
         self._build("pkv_cross_plan_host", True, *[None if a is None else a.ctypes.data for a in arrays], self.n_seqs, self.n_tokens,
                     *self._geometry())
@@ -437,13 +506,14 @@ class PrefixPlan(_SegmentPlan):
 
     def build_host(self, token_pos, prefix_len: int, stream=None) -> "PrefixPlan":
         """token_pos: every token's position, on the host; its sequence's first prefix_len positions lie in the same
-        blocks as everyone's.  The staging buffer belongs to the upload until it has run."""
+        blocks as everyone's.  Waits, if need be, until the plan's last upload has run."""
         pos = self._positions(token_pos)
         self._build("pkv_prefix_plan_host", False, pos.ctypes.data, self.n_tokens, prefix_len, *self._geometry(), stream=stream)
         return self
 
     def build_host_image(self, token_pos, prefix_len: int) -> int:
-        """The plan without the upload: bytes of self.staging that must reach the start of self.workspace."""
+        """The plan without the upload: bytes of self.staging that must reach the start of self.workspace, before the plan
+        is made anew."""
         pos = self._positions(token_pos)
         self._build("pkv_prefix_plan_host", True, pos.ctypes.data, self.n_tokens, prefix_len, *self._geometry())
         return int(self.plan.image_bytes)

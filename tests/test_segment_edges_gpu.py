@@ -79,3 +79,92 @@ def test_rows_of_other_than_16_byte_multiples_may_begin_anywhere(pkv, torch_cuda
     plan.attention(step.q, step.kc, step.vc, step.block_tables, step.table_offset, torch.arange(3, device="cuda", dtype=torch.int32), step.out,
                    step.scale)
     step.check(pkv)
+
+
+def prefix_step(torch, geom, n, shared, tail, seed):
+    step = Step(torch, "bf16", geom, [1] * n, [shared + tail + 3 * (i % 5) for i in range(n)], 16, seed=seed, shared=shared)
+    step.token_seq = torch.arange(n, device="cuda", dtype=torch.int32)
+    return step
+
+
+def prefix_plan(pkv, step):
+    return pkv.PrefixPlan(step.n, step.qh, step.kvh, step.hd, 16, step.q.dtype, num_blocks=step.num_blocks)
+
+
+def attend_prefix(plan, step, **kw):
+    plan.attention(step.q, step.kc, step.vc, step.block_tables, step.table_offset, step.token_seq, step.out, step.scale, **kw)
+
+
+BUSY = 100_000_000      # cycles, 50 ms and more: time for the host to plan the steps behind
+
+
+@pytest.mark.parametrize("tiles", ["", "1"])
+@pytest.mark.parametrize("drop", [False, True])
+def test_plans_of_steps_that_the_gpu_has_not_reached(pkv, torch_cuda, monkeypatch, tiles, drop):
+    """The host plans three steps ahead, through one object or through objects it drops."""
+    torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
+    steps = [prefix_step(torch, TINY, 60, 640, 20 + 150 * i, seed=30 + i) for i in range(3)]
+    sources = [Step(torch, "bf16", TINY, [1 + (j + i) % 4 for j in range(20)], [50 + 300 * i + 7 * j for j in range(20)], 16, seed=40 + i)
+               for i in range(3)]
+    rows = max(s.n for s in sources)
+    plan, other = prefix_plan(pkv, steps[0]), pkv.CrossPlan(rows, 20, *TINY, 16, torch.bfloat16)
+    for s in sources:                                            # every step as many rows: the last ones of no sequence
+        extra = rows - s.n
+        s.q, s.mark = (torch.cat([t, t[:extra]]) for t in (s.q, s.mark))
+        s.out, s.n = s.mark.clone(), rows
+    torch.cuda.synchronize()
+    torch.cuda._sleep(BUSY)
+    for step, source in zip(steps, sources):
+        if drop:
+            plan, other = prefix_plan(pkv, step), pkv.CrossPlan(rows, 20, *TINY, 16, torch.bfloat16)
+        plan.num_blocks = step.num_blocks
+        plan.build_host([k - 1 for k in step.kv_len], 640)
+        other.build_host(source.q_len, source.kv_len)
+        attend_prefix(plan, step)
+        attend(other, source)
+    for x in steps + sources:
+        x.check(pkv)
+
+
+def test_workspace_of_a_plan_dropped_on_another_stream(pkv, torch_cuda, monkeypatch):
+    """Its memory is not handed out again while that stream's calls are to come."""
+    torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
+    step = prefix_step(torch, TINY, 60, 640, 50, seed=50)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for named in (False, True):
+        step.out.copy_(step.mark)
+        plan = prefix_plan(pkv, step).build_host([k - 1 for k in step.kv_len], 640)
+        size = plan.workspace.numel()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(BUSY)
+            if not named:
+                attend_prefix(plan, step)
+        if named:
+            attend_prefix(plan, step, stream=side)
+        del plan
+        others = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(3)]
+        step.check(pkv)
+        del others
+
+
+def test_plans_around_a_capture(pkv, torch_cuda):
+    """Made anew, made and dropped while a stream is being captured: nothing of it ends the capture."""
+    torch = torch_cuda
+    step = prefix_step(torch, TINY, 60, 640, 50, seed=60)
+    pos = [k - 1 for k in step.kv_len]
+    plan = prefix_plan(pkv, step).build_host(pos, 640)
+    attend_prefix(plan, step)
+    dropped = prefix_plan(pkv, step).build_host(pos, 640)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        del dropped
+        plan.build_host(pos, 640)                                # its copy is a node of the graph
+        attend_prefix(plan, step)
+    for _ in range(2):
+        step.out.copy_(step.mark)
+        graph.replay()
+        step.check(pkv)

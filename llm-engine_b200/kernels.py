@@ -229,102 +229,6 @@ def launch_attention_mixed(q, k_cache, v_cache, block_tables, table_offset, toke
 launch_attention_decode_gqa = launch_attention_decode
 
 
-class DecodePlan:
-    """Split-K work list built once per step and shared by every layer's attention call."""
-
-    def __init__(self, n_tokens: int, q_heads: int, kv_heads: int, head_dim: int, workspace=None, device="cuda",
-                 num_blocks: int = 0):
-        """num_blocks: blocks per K/V pool, if known: the kernels' tensor maps then end at the pool
-        (a wrong block id reads zeros); 0 = unknown, as through llm-engine's own launcher signature."""
-        import torch
-        self.n_tokens, self.q_heads, self.kv_heads, self.head_dim = n_tokens, q_heads, kv_heads, head_dim
-        self.num_blocks = num_blocks
-        self.workspace = workspace if workspace is not None else alloc_decode_workspace(
-            n_tokens, q_heads, kv_heads, head_dim, device)
-        nstage = int(_lib.lib().pkv_decode_plan_staging_bytes(n_tokens, kv_heads))
-        self.staging = torch.empty(max(nstage, 256), dtype=torch.uint8).pin_memory()
-        self.plan = _lib.DecodePlan()
-
-    def _ws(self):
-        return self.workspace.data_ptr(), self.workspace.numel()
-
-    def build_host(self, token_pos_host, stream=None) -> "DecodePlan":
-        """token_pos_host: int32 numpy array or CPU tensor of the packed tokens' positions."""
-        import numpy as np
-        pos = np.ascontiguousarray(token_pos_host, dtype=np.int32)
-        p, n = self._ws()
-        st = _lib.lib().pkv_decode_plan_host(pos.ctypes.data, self.n_tokens, self.q_heads, self.kv_heads,
-                                             self.head_dim, self.staging.data_ptr(), self.staging.numel(), p, n,
-                                             _stream(stream), C.byref(self.plan))
-        _lib.check("pkv_decode_plan_host", st)
-        self.plan.num_blocks = self.num_blocks
-        return self
-
-    def build_host_image(self, token_pos_host) -> int:
-        """The host planner without the upload: the image goes to self.staging (pinned) and its size
-        is returned; the caller copies it to the start of self.workspace, typically as a node of a
-        captured graph that is replayed every step."""
-        import numpy as np
-        pos = np.ascontiguousarray(token_pos_host, dtype=np.int32)
-        n = C.c_size_t(0)
-        st = _lib.lib().pkv_decode_plan_host_image(pos.ctypes.data, self.n_tokens, self.q_heads, self.kv_heads, self.head_dim,
-                                                   self.staging.data_ptr(), self.staging.numel(), self.workspace.numel(),
-                                                   C.byref(self.plan), C.byref(n))
-        _lib.check("pkv_decode_plan_host_image", st)
-        self.plan.num_blocks = self.num_blocks
-        return int(n.value)
-
-    def build_host_shared(self, idx, block_size: int, min_saved_bytes: int = -1, stream=None) -> "DecodePlan":
-        """Shared-prefix-aware plan from the host copies of the step's index arrays (`idx`: a
-        StepIndices as returned by pack_step): sequences whose tables start with the same blocks
-        have that range read once per group of up to four tokens, if that saves at least
-        min_saved_bytes of K/V reads per layer (-1: the library's default; 0: always)."""
-        import numpy as np
-        pos = np.ascontiguousarray(idx.token_pos, dtype=np.int32)
-        seq = np.ascontiguousarray(idx.token_seq, dtype=np.int32)
-        tabs = np.ascontiguousarray(idx.block_tables, dtype=np.int32)
-        off = np.ascontiguousarray(idx.table_offset, dtype=np.int32)
-        p, n = self._ws()
-        st = _lib.lib().pkv_decode_plan_host_shared(pos.ctypes.data, seq.ctypes.data, tabs.ctypes.data, off.ctypes.data,
-                                                    self.n_tokens, off.size, tabs.size, block_size, self.q_heads,
-                                                    self.kv_heads, self.head_dim, min_saved_bytes, self.staging.data_ptr(),
-                                                    self.staging.numel(), p, n, _stream(stream), C.byref(self.plan))
-        _lib.check("pkv_decode_plan_host_shared", st)
-        self.plan.num_blocks = self.num_blocks
-        return self
-
-    @property
-    def n_shared_units(self) -> int:
-        return int(self.plan.reserved) >> 1
-
-    def build_device(self, token_pos, stream=None) -> "DecodePlan":
-        p, n = self._ws()
-        st = _lib.lib().pkv_decode_plan_device(_ptr(token_pos), self.n_tokens, self.q_heads, self.kv_heads,
-                                               self.head_dim, p, n, _stream(stream), C.byref(self.plan))
-        _lib.check("pkv_decode_plan_device", st)
-        self.plan.num_blocks = self.num_blocks
-        return self
-
-    def attention(self, q, k_cache, v_cache, block_tables, table_offset, token_seq, token_pos, out,
-                  block_size: int, scale: float, stream=None) -> None:
-        fn, call = _fn("pkv_decode_attn_planned_", k_cache)
-        p, n = self._ws()
-        st = call(C.byref(self.plan), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
-                  _ptr(table_offset), _ptr(token_seq), _ptr(token_pos), _ptr(out), block_size,
-                  C.c_float(scale), p, n, _stream(stream))
-        _lib.check(fn, st)
-
-    def append_attention(self, q, k, v, slots, k_cache, v_cache, block_tables, table_offset, token_seq, token_pos, out,
-                         block_size: int, scale: float, stream=None) -> None:
-        """launch_store_kv + attention in one chain (decode steps only: one token per sequence)."""
-        fn, call = _fn("pkv_append_decode_attn_planned_", k_cache)
-        p, n = self._ws()
-        st = call(C.byref(self.plan), _ptr(q), _ptr(k), _ptr(v), _ptr(slots), _ptr(k_cache), _ptr(v_cache),
-                  _ptr(block_tables), _ptr(table_offset), _ptr(token_seq), _ptr(token_pos), _ptr(out),
-                  block_size, C.c_float(scale), p, n, _stream(stream))
-        _lib.check(fn, st)
-
-
 def _passed(event, wait: bool) -> bool:
     """Whether the GPU has come past `event`, inside a stream capture too (torch's own query ends one)."""
     return bool(_lib.check("pkv_event_passed", _lib.lib().pkv_event_passed(event.cuda_event, wait)))
@@ -373,6 +277,107 @@ class _Staging:
     def __del__(self, left=_left):
         if getattr(self, "_sent", None) is not None:
             left.append((self._sent, self.bytes))
+
+
+class DecodePlan:
+    """Split-K work list built once per step and shared by every layer's attention call."""
+
+    def __init__(self, n_tokens: int, q_heads: int, kv_heads: int, head_dim: int, workspace=None, device="cuda",
+                 num_blocks: int = 0):
+        """num_blocks: blocks per K/V pool, if known: the kernels' tensor maps then end at the pool
+        (a wrong block id reads zeros); 0 = unknown, as through llm-engine's own launcher signature."""
+        import torch
+        self.n_tokens, self.q_heads, self.kv_heads, self.head_dim = n_tokens, q_heads, kv_heads, head_dim
+        self.num_blocks = num_blocks
+        self.workspace = workspace if workspace is not None else alloc_decode_workspace(
+            n_tokens, q_heads, kv_heads, head_dim, device)
+        self._staging = _Staging(int(_lib.lib().pkv_decode_plan_staging_bytes(n_tokens, kv_heads)))
+        self.staging = self._staging.bytes
+        self.plan = _lib.DecodePlan()
+
+    def _ws(self):
+        return self.workspace.data_ptr(), self.workspace.numel()
+
+    def build_host(self, token_pos_host, stream=None) -> "DecodePlan":
+        """token_pos_host: int32 numpy array or CPU tensor of the packed tokens' positions."""
+        import numpy as np
+        pos = np.ascontiguousarray(token_pos_host, dtype=np.int32)
+        p, n = self._ws()
+        self._staging.writable()
+        st = _lib.lib().pkv_decode_plan_host(pos.ctypes.data, self.n_tokens, self.q_heads, self.kv_heads,
+                                             self.head_dim, self.staging.data_ptr(), self.staging.numel(), p, n,
+                                             _stream(stream), C.byref(self.plan))
+        self._staging.sent(stream, self.workspace.get_device())
+        _lib.check("pkv_decode_plan_host", st)
+        self.plan.num_blocks = self.num_blocks
+        return self
+
+    def build_host_image(self, token_pos_host) -> int:
+        """The host planner without the upload: the image goes to self.staging (pinned) and its size
+        is returned; the caller copies it to the start of self.workspace, typically as a node of a
+        captured graph that is replayed every step."""
+        import numpy as np
+        pos = np.ascontiguousarray(token_pos_host, dtype=np.int32)
+        n = C.c_size_t(0)
+        self._staging.writable()
+        st = _lib.lib().pkv_decode_plan_host_image(pos.ctypes.data, self.n_tokens, self.q_heads, self.kv_heads, self.head_dim,
+                                                   self.staging.data_ptr(), self.staging.numel(), self.workspace.numel(),
+                                                   C.byref(self.plan), C.byref(n))
+        _lib.check("pkv_decode_plan_host_image", st)
+        self.plan.num_blocks = self.num_blocks
+        return int(n.value)
+
+    def build_host_shared(self, idx, block_size: int, min_saved_bytes: int = -1, stream=None) -> "DecodePlan":
+        """Shared-prefix-aware plan from the host copies of the step's index arrays (`idx`: a
+        StepIndices as returned by pack_step): sequences whose tables start with the same blocks
+        have that range read once per group of up to four tokens, if that saves at least
+        min_saved_bytes of K/V reads per layer (-1: the library's default; 0: always)."""
+        import numpy as np
+        pos = np.ascontiguousarray(idx.token_pos, dtype=np.int32)
+        seq = np.ascontiguousarray(idx.token_seq, dtype=np.int32)
+        tabs = np.ascontiguousarray(idx.block_tables, dtype=np.int32)
+        off = np.ascontiguousarray(idx.table_offset, dtype=np.int32)
+        p, n = self._ws()
+        self._staging.writable()
+        st = _lib.lib().pkv_decode_plan_host_shared(pos.ctypes.data, seq.ctypes.data, tabs.ctypes.data, off.ctypes.data,
+                                                    self.n_tokens, off.size, tabs.size, block_size, self.q_heads,
+                                                    self.kv_heads, self.head_dim, min_saved_bytes, self.staging.data_ptr(),
+                                                    self.staging.numel(), p, n, _stream(stream), C.byref(self.plan))
+        self._staging.sent(stream, self.workspace.get_device())
+        _lib.check("pkv_decode_plan_host_shared", st)
+        self.plan.num_blocks = self.num_blocks
+        return self
+
+    @property
+    def n_shared_units(self) -> int:
+        return int(self.plan.reserved) >> 1
+
+    def build_device(self, token_pos, stream=None) -> "DecodePlan":
+        p, n = self._ws()
+        st = _lib.lib().pkv_decode_plan_device(_ptr(token_pos), self.n_tokens, self.q_heads, self.kv_heads,
+                                               self.head_dim, p, n, _stream(stream), C.byref(self.plan))
+        _lib.check("pkv_decode_plan_device", st)
+        self.plan.num_blocks = self.num_blocks
+        return self
+
+    def attention(self, q, k_cache, v_cache, block_tables, table_offset, token_seq, token_pos, out,
+                  block_size: int, scale: float, stream=None) -> None:
+        fn, call = _fn("pkv_decode_attn_planned_", k_cache)
+        p, n = self._ws()
+        st = call(C.byref(self.plan), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
+                  _ptr(table_offset), _ptr(token_seq), _ptr(token_pos), _ptr(out), block_size,
+                  C.c_float(scale), p, n, _stream(stream))
+        _lib.check(fn, st)
+
+    def append_attention(self, q, k, v, slots, k_cache, v_cache, block_tables, table_offset, token_seq, token_pos, out,
+                         block_size: int, scale: float, stream=None) -> None:
+        """launch_store_kv + attention in one chain (decode steps only: one token per sequence)."""
+        fn, call = _fn("pkv_append_decode_attn_planned_", k_cache)
+        p, n = self._ws()
+        st = call(C.byref(self.plan), _ptr(q), _ptr(k), _ptr(v), _ptr(slots), _ptr(k_cache), _ptr(v_cache),
+                  _ptr(block_tables), _ptr(table_offset), _ptr(token_seq), _ptr(token_pos), _ptr(out),
+                  block_size, C.c_float(scale), p, n, _stream(stream))
+        _lib.check(fn, st)
 
 
 class _SegmentPlan:

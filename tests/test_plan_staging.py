@@ -29,6 +29,13 @@ class Uploads:
         self.pending.append((staging, plan._obj.image_bytes, C.string_at(staging, plan._obj.image_bytes)))
         return st
 
+    def pkv_decode_plan_host(self, *a):
+        *sizes, staging, staging_bytes, _, ws_bytes, _, plan = a
+        n = C.c_size_t(0)
+        st = self.real.pkv_decode_plan_host_image(*sizes, staging, staging_bytes, ws_bytes, plan, C.byref(n))
+        self.pending.append((staging, n.value, C.string_at(staging, n.value)))
+        return st
+
     def run(self, up_to=None):
         while self.pending and (up_to is None or len(self.done) < up_to):
             staging, n, planned = self.pending.pop(0)
@@ -69,6 +76,22 @@ def cross(pkv, torch, n):
 def prefix(pkv, torch, n):
     ws = torch.zeros(pkv.lib().pkv_prefix_workspace_bytes(n, 14, 2, 64), dtype=torch.uint8)
     return pkv.PrefixPlan(n, 14, 2, 64, 16, torch.bfloat16, workspace=ws)
+
+
+def test_decode_plan_made_anew_or_dropped_while_its_upload_is_pending(pkv, uploads, monkeypatch):
+    torch = pytest.importorskip("torch")
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
+    ws = torch.zeros(pkv.decode_workspace_bytes(40, 14, 2, 64), dtype=torch.uint8)
+    for step in range(3):
+        plan = pkv.DecodePlan(40, 14, 2, 64, workspace=ws)
+        for again in range(2):
+            plan.build_host([100 + 170 * i + 1000 * step + again for i in range(40)])
+        del plan
+        gc.collect()
+    plan = pkv.DecodePlan(40, 14, 2, 64, workspace=ws).build_host([5000] * 40)
+    plan.build_host_image([70] * 40)
+    uploads.run()
+    assert uploads.done == [True] * 7
 
 
 def test_plan_made_anew_while_its_upload_is_pending(pkv, uploads):

@@ -405,6 +405,7 @@ class _SegmentPlan:
         self._plan_ref = C.byref(self.plan)
         self._device, self._ws = workspace.get_device(), (_ptr(workspace), workspace.numel())
         self._out_elems = n_tokens * q_heads * head_dim
+        self._block_elems = block_size * kv_heads * head_dim
 
     def _geometry(self):
         return self.q_heads, self.kv_heads, self.head_dim, self.block_size, self.dtype.itemsize
@@ -443,6 +444,11 @@ class _SegmentPlan:
         _check(ints, _torch.int32, device, "index arrays")
         if q.numel() < self._out_elems or out.numel() < self._out_elems:
             raise ValueError(f"q and out must have {self.n_tokens} rows of {self.q_heads} heads")
+        pool = k_cache.numel()
+        if v_cache.numel() != pool:
+            raise ValueError("K and V pools differ in size")
+        if self.plan.num_blocks * self._block_elems > pool:
+            raise ValueError(f"the pools are smaller than the plan's {self.plan.num_blocks} blocks")
         fn, call = _fn(op, k_cache)
         handle = _stream_of(stream, device)
         if self._streams is not None and handle not in self._streams:

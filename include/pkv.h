@@ -63,7 +63,8 @@ const char* pkv_last_error(void);
  * launch's output incomplete.  The record of it is a bit -- 1: a TMA producer never saw
  * its ring slot released; 2: a consumer never saw its tile arrive; 4: a prefill
  * pipeline wait; 8: a peer GPU's flag in the head-sharded exchange; 16: a block copy; 32: a wait of
- * the tile kernel (pkv_cross_attn_*, pkv_prefix_attn_*) -- kept in two
+ * the tile kernel (pkv_cross_attn_*, pkv_prefix_attn_*); 64 (no wait): a replayed call of these found
+ * another plan in its workspace than it was captured with, and did nothing -- kept in two
  * places: a device word, and a pinned host word the kernels store to.  The attention
  * entry points (pkv_decode_attn_*, the planned, fused, peer and mixed forms,
  * pkv_prefill_attn_*) look at the host word before they enqueue anything, and so do
@@ -486,9 +487,12 @@ int pkv_prefill_attn_f16(const void* q, const void* k_cache, const void* v_cache
  *
  * A plan belongs to the host lengths it was made from and to the workspace it was uploaded
  * to (256-byte aligned; pkv_cross_workspace_bytes / pkv_prefix_workspace_bytes are enough for
- * any lengths); it serves any number of calls on one stream, captured ones included: a replay
- * repeats the captured step's work list, other lengths want another plan and capture.  Calls
- * that may overlap need a workspace each.  h_staging (at least pkv_segment_staging_bytes, pinned
+ * any lengths); it serves any number of calls on one stream, captured ones included.  Unlike
+ * those of pkv_decode_plan, a captured call serves its own step only: its launches are made for
+ * the counts in the plan.  A replay over an image of other counts does nothing but record bit 64
+ * (pkv_debug_device_flags), other lengths want another plan and capture.  (Calls that took the
+ * cluster form, plan->cluster, follow any image of as many rows in which every row has keys.)
+ * Calls that may overlap need a workspace each.  h_staging (at least pkv_segment_staging_bytes, pinned
  * for a truly asynchronous copy) must stay untouched until the upload has run; the _image forms
  * write it and leave the copy of plan->image_bytes to the start of the workspace to the caller.
  * elem_bytes: 2 for f16 and bf16, 4 for f32.  A caller that knows the pool size sets

@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const int* __
     header->n_parts = n_parts;
     header->kv_heads = lim.kv_heads;
     header->n_shares = rule.n_shares;
-    header->pad = 0;
+    header->stamp = 0;
+    header->cluster_stamp = 0;
   }
   if constexpr (ROUTE) {
     if (tid == 0) {
@@ -628,6 +629,7 @@ void fill_args(DecodeArgs& a, const void* q, const void* kc, const void* vc, con
   a.block_size = block_size; a.bs_log2 = log2_exact(block_size);
   a.scale = scale;
   a.header = nullptr; a.items = nullptr; a.tok_split = nullptr; a.counters = nullptr;
+  a.stamp = 0;
   a.part_ml = nullptr; a.part_acc = nullptr;
   a.direct = 1;
   a.shared_items = nullptr;
@@ -1009,11 +1011,13 @@ int decode_listed(const DecodeList& l, cudaStream_t stream, bool* merged) {
             l.kv_heads, l.head_dim, l.block_size, l.scale);
   a.host_err = l.host_err;
   if (l.pool_rows > 0) a.pool_rows = l.pool_rows;
+  a.header = l.header;
   if (l.cluster >= 2 && a.group <= 8 && tma_path<T>(a)) {
+    a.stamp = l.cluster_stamp;
     const int st = launch_tma_cluster<T>(a, l.cluster, l.cluster_least, stream, merged);
     if (st != PKV_OK || *merged) return st;
   }
-  a.header = l.header;
+  a.stamp = l.stamp;
   a.items = l.items;
   a.part_ml = l.part_ml;
   a.part_acc = l.part_acc;

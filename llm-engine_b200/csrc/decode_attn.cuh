@@ -30,7 +30,8 @@ namespace pkv {
 __device__ unsigned int g_pkv_device_error = 0;
 
 constexpr int kMaxPeers = 8;
-constexpr unsigned kErrPeerWait = 8u;   // bit of the device error word: a peer's flag did not arrive in time
+// Bits of the device error word: a peer's flag did not arrive in time; the workspace holds another plan than the launch was made for.
+constexpr unsigned kErrPeerWait = 8u, kErrOtherPlan = 64u;
 
 struct DecodeArgs {
   const void* q;
@@ -46,6 +47,7 @@ struct DecodeArgs {
   float scale;
   // plan (all null / 0 in direct mode)
   const PlanHeader* header;
+  int stamp;   // != 0: the launch is made for the plan with this stamp (PlanHeader), and does nothing if it finds another
   const WorkItem* items;
   const TokSplit* tok_split;
   int* counters;
@@ -93,6 +95,16 @@ __device__ __forceinline__ void report_give_up(const DecodeArgs& a, unsigned int
     *reinterpret_cast<volatile unsigned int*>(a.host_err) = bit;
     __threadfence_system();
   }
+}
+
+// Whether the plan in the workspace is another than the launch's: a captured call that is replayed over a later step's
+// image.  Recorded once, by the first thread.  The launch then does nothing, but its completion implies the previous one's.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool other_plan(const DecodeArgs& a) {
+  if (a.stamp == 0 || (CLUSTER ? a.header->cluster_stamp : a.header->stamp) == a.stamp) return false;
+  pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) report_give_up(a, kErrOtherPlan);
+  return true;
 }
 
 // Output row of (token, head 0) under the layout above.
@@ -399,7 +411,7 @@ __global__ void __launch_bounds__(kDecodeThreads, MIN_BLOCKS) decode_mma_kernel(
 
   pdl_launch_dependents();
   pdl_wait();  // the pool rows appended by the preceding launch, the plan, the previous merge
-  const int n_items = a.direct ? a.n_tokens : a.header->n_items;
+  const int n_items = a.direct ? a.n_tokens : other_plan(a) ? 0 : a.header->n_items;
   const int total = n_items * a.kv_heads;
 
   for (int work = blockIdx.x; work < total; work += gridDim.x) {
@@ -663,7 +675,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_simt_kernel(const Decod
 
   pdl_launch_dependents();
   pdl_wait();
-  const int n_items = a.direct ? a.n_tokens : a.header->n_items;
+  const int n_items = a.direct ? a.n_tokens : other_plan(a) ? 0 : a.header->n_items;
   const int total = n_items * a.kv_heads;
 
   for (int work = blockIdx.x; work < total; work += gridDim.x) {

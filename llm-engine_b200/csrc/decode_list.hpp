@@ -14,6 +14,7 @@ struct DecodeList {
   int n_tokens, q_heads, kv_heads, head_dim, block_size;
   float scale;
   const PlanHeader* header;
+  int stamp, cluster_stamp;    // what the header must show
   const WorkItem* items;
   int n_items;
   float *part_ml, *part_acc;

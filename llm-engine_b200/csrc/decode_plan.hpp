@@ -44,7 +44,9 @@ struct PlanHeader {
   int n_parts;
   int kv_heads;
   int n_shares;  // 0: units are dealt one by one; otherwise int first_item[n_shares + 1] follows the items
-  int pad;
+  // Of plans whose launches are made for their counts and offsets (segment_plan.hpp), else 0: what names those, and what
+  // the cluster form needs of them.
+  int stamp, cluster_stamp;
 };
 
 struct WorkItem {

@@ -303,6 +303,8 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_BLOCKS)
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(&vmap) : "memory");
   }
   bool waited = !CLUSTER && !FUSED_APPEND && a.wait_last != 0;
+  bool other = false;
+  if constexpr (!INLINE_PLAN && !FUSED_APPEND && TOK == 1) other = other_plan<CLUSTER>(a);
   // Cluster launches: this warp's one unit, from the token's position alone (a step constant).
   int c_token = 0, c_kvh = 0, c_begin = 0, c_len = 0, c_nsplits = 1, c_split = 0;
   uint32_t c_rank = 0, c_size = 1;
@@ -315,10 +317,10 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_BLOCKS)
     const int len = max(__ldg(a.token_pos + c_token), 0) + 1;
     const int nw = WARPS * static_cast<int>(c_size);
     const int range = (((len + nw - 1) / nw + SLAB - 1) / SLAB) * SLAB;   // whole slabs per warp
-    c_nsplits = (len + range - 1) / range;
+    c_nsplits = other ? 1 : (len + range - 1) / range;
     c_split = warp * static_cast<int>(c_size) + static_cast<int>(c_rank);   // neighbouring ranges on different SMs
     c_begin = c_split * range;
-    c_len = min(range, len - c_begin);                     // <= 0: no unit for this warp
+    c_len = other ? 0 : min(range, len - c_begin);         // <= 0: no unit for this warp
     if (c_nsplits > 1) {                                   // the same for every thread of the cluster
       if (threadIdx.x == 0) {
         const int owned = (a.group - static_cast<int>(c_rank) + static_cast<int>(c_size) - 1) / static_cast<int>(c_size);
@@ -346,8 +348,8 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_BLOCKS)
     }
     ip.build(a, smem_raw + (ring0 - smem_u32(smem_raw)) + WARPS * S::kWarpBytes);
   }
-  const int n_shares = INLINE_PLAN ? ip.rule.n_shares : (CLUSTER || TOK > 1 || a.direct) ? 0 : a.header->n_shares;
-  const int n_items = INLINE_PLAN ? ip.n_items : CLUSTER ? 0 : (TOK > 1 ? a.n_shared : (a.direct ? a.n_tokens : a.header->n_items));
+  const int n_shares = INLINE_PLAN ? ip.rule.n_shares : (CLUSTER || TOK > 1 || a.direct || other) ? 0 : a.header->n_shares;
+  const int n_items = INLINE_PLAN ? ip.n_items : CLUSTER || other ? 0 : (TOK > 1 ? a.n_shared : (a.direct ? a.n_tokens : a.header->n_items));
   const int total = CLUSTER ? (c_len > 0 ? 1 : 0) : (n_shares > 0 ? n_shares : n_items) * a.kv_heads;
   const int gw = CLUSTER ? 0 : blockIdx.x * WARPS + warp, GW = CLUSTER ? 1 : gridDim.x * WARPS;
   const int* share_first = CLUSTER || TOK > 1 || INLINE_PLAN || a.direct ? nullptr : reinterpret_cast<const int*>(a.items + n_items);

@@ -63,7 +63,8 @@ int check_error_mirror(const char* fn, unsigned int bits) {
   if (!v) return PKV_OK;
   return fail(PKV_E_CUDA,
               "%s: an earlier launch gave up on a bounded wait (flags 0x%x: 1 TMA producer, 2 tile consumer, 4 prefill "
-              "pipeline, 8 peer GPU, 16 block copy, 32 tile pipeline) and left its output incomplete; this call enqueued nothing, the next one runs normally",
+              "pipeline, 8 peer GPU, 16 block copy, 32 tile pipeline) or found another plan in its workspace (64), and left its output incomplete; this "
+              "call enqueued nothing, the next one runs normally",
               fn, v);
 }
 

@@ -52,7 +52,7 @@
 namespace pkv {
 
 __device__ unsigned int g_pkv_tile_error = 0;
-constexpr unsigned kErrTileWait = 32u;
+constexpr unsigned kErrTileWait = 32u, kErrOtherPlan = 64u;   // kErrOtherPlan: as in decode_attn.cuh
 
 unsigned int* error_mirror(bool create);                 // error_mirror.cu
 int check_error_mirror(const char* fn, unsigned int bits = ~0u);
@@ -87,6 +87,8 @@ struct TileArgs {
   const int *block_tables, *table_offset, *token_seq;
   const int *row_token, *list_first;
   const TileItem* tiles;
+  const PlanHeader* header;          // shows `stamp`, or this launch is not for the plan that the workspace holds
+  int stamp;
   void* out;
   float *part_ml, *part_acc;         // by partial row
   int q_heads, group;
@@ -96,6 +98,14 @@ struct TileArgs {
   float ml_scale;                    // what partial maxima are multiplied with: scale, or scale log2 e
   unsigned int* host_err;
 };
+
+__device__ __forceinline__ void report(unsigned int* host_err, unsigned int bit) {
+  atomicOr(&g_pkv_tile_error, bit);
+  if (host_err) {
+    *reinterpret_cast<volatile unsigned int*>(host_err) = bit;
+    __threadfence_system();
+  }
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -202,7 +212,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   };
 
   const TileItem* tiles = a.tiles + __ldg(a.list_first + blockIdx.x);
-  const int n_items = __ldg(a.list_first + blockIdx.x + 1) - __ldg(a.list_first + blockIdx.x);
+  // (no list is empty: 0 stands for another plan's image)
+  const int n_items = __ldg(&a.header->stamp) == a.stamp ? __ldg(a.list_first + blockIdx.x + 1) - __ldg(a.list_first + blockIdx.x) : 0;
 
   bool dead = false;
   auto WAIT = [&](uint32_t bar, uint32_t parity, uint32_t polls = 1u << 17) {
@@ -593,13 +604,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::fence_before();
     }
   }
-  if (dead) {
-    atomicOr(&g_pkv_tile_error, kErrTileWait);
-    if (a.host_err) {
-      *reinterpret_cast<volatile unsigned int*>(a.host_err) = kErrTileWait;
-      __threadfence_system();
-    }
-  }
+  if (dead) report(a.host_err, kErrTileWait);
+  if (n_items == 0 && blockIdx.x == 0 && threadIdx.x == 0) report(a.host_err, kErrOtherPlan);
   tc::fence_before();
   __syncthreads();
   if (warp == kIssuer) {
@@ -616,19 +622,23 @@ struct MergeArgs {
   int n_rows, q_heads, group, head_dim;
   const float *tile_ml, *tile_acc, *own_ml, *own_acc;
   void* out;
+  const PlanHeader* header;
+  int stamp;
+  unsigned int* host_err;
 };
 template <typename T, bool LOG2, int VEC>
 __global__ void __launch_bounds__(kMergeThreads) segment_merge_kernel(const MergeArgs a) {
   pdl_launch_dependents();
   const int per_head = a.head_dim / VEC, per_row = a.group * per_head;
   const long long i = blockIdx.x * static_cast<long long>(kMergeThreads) + threadIdx.x, row = i / per_row;
-  const bool live = row < a.n_rows;
+  const bool other = __ldg(&a.header->stamp) != a.stamp, live = row < a.n_rows && !other;
   MergeRow m{};
   if (live) {                                            // part of the plan, complete before the kernels that wrote the partials began
     const int4 x = __ldg(reinterpret_cast<const int4*>(a.rows + row)), y = __ldg(reinterpret_cast<const int4*>(a.rows + row) + 1);
     m = MergeRow{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
   }
   pdl_wait();
+  if (other && i == 0) report(a.host_err, kErrOtherPlan);
   if (!live) return;
   const int at = static_cast<int>(i - row * per_row), h = at / per_head, d = (at - h * per_head) * VEC, head = m.kvh * a.group + h;
   const int n = m.n_tile + m.n_own;
@@ -780,8 +790,31 @@ int tiles_asked() {
   return e && (*e == '0' || *e == '1') ? *e - '0' : -1;
 }
 
+// Names what a step's launches are made for: everything in the plan but the caller's num_blocks.  Never 0.
+int stamp_of(const pkv_segment_plan& plan) {
+  pkv_segment_plan p = plan;
+  p.num_blocks = 0;
+  static_assert(sizeof(p) % 8 == 0, "whole words, no padding");
+  unsigned long long word, h = 0x9e3779b97f4a7c15ull;
+  for (size_t i = 0; i < sizeof(p); i += 8) {
+    std::memcpy(&word, reinterpret_cast<const char*>(&p) + i, 8);
+    h = (h ^ word) * 0xd1342543de82ef95ull;
+    h ^= h >> 32;
+  }
+  return static_cast<int>(h) | 1;
+}
+// What the cluster form, which reads the tokens' positions and sequences only, needs: a step of the same sizes.
+int cluster_stamp_of(const pkv_segment_plan& plan) {
+  pkv_segment_plan p{};
+  p.kind = plan.kind;
+  p.n_tokens = plan.n_tokens; p.q_heads = plan.q_heads; p.kv_heads = plan.kv_heads; p.head_dim = plan.head_dim;
+  p.block_size = plan.block_size; p.elem_bytes = plan.elem_bytes;
+  return stamp_of(p);
+}
+
+// every: every row has keys.
 int write_image(const char* fn, Kind kind, const SegmentGeometry& g, const SegmentLists& l, const std::vector<int>& seq, const std::vector<int>& pos,
-                bool cluster, void* h_staging, size_t staging_bytes, size_t workspace_bytes, pkv_segment_plan* plan) {
+                bool every, bool cluster, void* h_staging, size_t staging_bytes, size_t workspace_bytes, pkv_segment_plan* plan) {
   const SegmentOffsets o = segment_offsets(g, SegmentCounts{l.row_token.size(), l.items.size(), l.first.size(), l.list_first.size(), l.tiles.size(),
                                                             l.merge.size(), static_cast<size_t>(l.n_tile_rows), static_cast<size_t>(l.n_parts)});
   if (o.total > workspace_bytes) return fail(PKV_E_WORKSPACE, "%s: workspace of %zu bytes; this step takes %zu", fn, workspace_bytes, o.total);
@@ -824,7 +857,9 @@ int write_image(const char* fn, Kind kind, const SegmentGeometry& g, const Segme
   plan->off_seq = o.seq; plan->off_pos = o.pos; plan->off_rows = o.rows; plan->off_items = o.items;
   plan->off_lists = o.lists; plan->off_tiles = o.tiles; plan->off_merge = o.merge;
   plan->off_tile_ml = o.tile_ml; plan->off_tile_acc = o.tile_acc; plan->off_ml = o.ml; plan->off_acc = o.acc;
-  if (cluster && l.n_parts > 0) plan->cluster = decode_cluster_size(g.n_tokens, l.longest, g.q_heads, g.kv_heads, g.head_dim, &plan->cluster_least);
+  if (every && cluster && l.n_parts > 0) plan->cluster = decode_cluster_size(g.n_tokens, l.longest, g.q_heads, g.kv_heads, g.head_dim, &plan->cluster_least);
+  hd->stamp = stamp_of(*plan);
+  hd->cluster_stamp = every ? cluster_stamp_of(*plan) : 0;
   return PKV_OK;
 }
 
@@ -893,7 +928,7 @@ int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* 
   }
   split(fewest);
   list_segments(segs, own, empty, g, decode_sms(), false, l);
-  return write_image(fn, kCross, g, l, seq, pos, segs.empty() && empty.empty() && listed == g.n_tokens, h_staging, staging_bytes, workspace_bytes, plan);
+  return write_image(fn, kCross, g, l, seq, pos, empty.empty() && listed == g.n_tokens, segs.empty(), h_staging, staging_bytes, workspace_bytes, plan);
 }
 
 int plan_prefix(const char* fn, const int* token_pos, int prefix_len, const SegmentGeometry& g, void* h_staging, size_t staging_bytes,
@@ -940,7 +975,7 @@ int plan_prefix(const char* fn, const int* token_pos, int prefix_len, const Segm
   if (segs.empty()) l.row_token.clear();
   ranges(!segs.empty());
   list_segments(segs, own, empty, g, decode_sms(), true, l);
-  return write_image(fn, kPrefix, g, l, none, pos, segs.empty(), h_staging, staging_bytes, workspace_bytes, plan);
+  return write_image(fn, kPrefix, g, l, none, pos, true, segs.empty(), h_staging, staging_bytes, workspace_bytes, plan);
 }
 
 int upload(const char* fn, pkv_segment_plan* plan, const void* h_staging, void* workspace, pkv_stream stream) {
@@ -977,6 +1012,8 @@ int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const v
   float *ml = reinterpret_cast<float*>(ws + plan->off_ml), *acc = reinterpret_cast<float*>(ws + plan->off_acc);
   float *tile_ml = reinterpret_cast<float*>(ws + plan->off_tile_ml), *tile_acc = reinterpret_cast<float*>(ws + plan->off_tile_acc);
   unsigned int* host_err = error_mirror(true);
+  const PlanHeader* header = reinterpret_cast<const PlanHeader*>(ws);
+  const int stamp = stamp_of(*plan);
   if (plan->n_tiles > 0) {
     if constexpr (sizeof(T) == 2) {
       if (!tensor_map_encoder()) return fail(PKV_E_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", fn);
@@ -985,6 +1022,7 @@ int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const v
       a.row_token = reinterpret_cast<const int*>(ws + plan->off_rows);
       a.list_first = reinterpret_cast<const int*>(ws + plan->off_lists);
       a.tiles = reinterpret_cast<const TileItem*>(ws + plan->off_tiles);
+      a.header = header; a.stamp = stamp;
       a.out = out; a.part_ml = tile_ml; a.part_acc = tile_acc;
       a.q_heads = plan->q_heads; a.group = group;
       a.block_size = plan->block_size; a.bs_log2 = log2_floor(plan->block_size); a.box_log2 = std::min(a.bs_log2, 7);
@@ -1004,7 +1042,8 @@ int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const v
     l.out = out;
     l.n_tokens = plan->n_tokens; l.q_heads = plan->q_heads; l.kv_heads = plan->kv_heads; l.head_dim = D; l.block_size = plan->block_size;
     l.scale = scale;
-    l.header = reinterpret_cast<const PlanHeader*>(ws);
+    l.header = header;
+    l.stamp = stamp; l.cluster_stamp = plan->cluster > 0 ? cluster_stamp_of(*plan) : 0;
     l.items = reinterpret_cast<const WorkItem*>(ws + plan->off_items);
     l.n_items = plan->n_items;
     l.part_ml = ml; l.part_acc = acc;
@@ -1017,7 +1056,7 @@ int segment_attn(Kind kind, const pkv_segment_plan* plan, const void* q, const v
     if (st != PKV_OK || merged) return st;
   }
   if (plan->n_merged > 0) {
-    MergeArgs m{reinterpret_cast<const MergeRow*>(ws + plan->off_merge), plan->n_merged, plan->q_heads, group, D, tile_ml, tile_acc, ml, acc, out};
+    MergeArgs m{reinterpret_cast<const MergeRow*>(ws + plan->off_merge), plan->n_merged, plan->q_heads, group, D, tile_ml, tile_acc, ml, acc, out, header, stamp, host_err};
     // four values in one store where every row of out begins on a multiple of them (rows of other than 16-byte multiples may begin anywhere)
     const int vec = D % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0 ? 4 : 1;
     const long long blocks = (static_cast<long long>(plan->n_merged) * group * (D / vec) + kMergeThreads - 1) / kMergeThreads;

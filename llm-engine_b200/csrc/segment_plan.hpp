@@ -13,6 +13,8 @@
 // Tiles are dealt to blocks here, one list of items for each block of the tile kernel (one per SM): either whole, the
 // longest first to the block with the least to do, or laid end to end and cut into equal shares, whichever ends first.
 //
+// The launches of a step are made for its counts and offsets, so each of them looks at the image's stamp, which names these, first.
+//
 // Image in the workspace (every region 256-byte aligned, offsets in pkv_segment_plan):
 //   PlanHeader | token_seq[n_tokens] | token_pos[n_tokens] | row_token[..] | WorkItem[..] (and the first item of every
 //   share) | int first tile of every list, and the end | TileItem[..] | MergeRow[..]

@@ -168,3 +168,104 @@ def test_plans_around_a_capture(pkv, torch_cuda):
         step.out.copy_(step.mark)
         graph.replay()
         step.check(pkv)
+
+
+def captured(torch, call):
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    return graph
+
+
+def replace_image(plan, n):
+    plan.workspace[:n].copy_(plan.staging[:n])
+
+
+OTHER_PLAN = 64
+
+
+@pytest.mark.parametrize("geom,dtype,tiles", [(TINY, "bf16", "1"), (WIDE, "f16", "1"), (TINY, "bf16", "0"), (WIDE, "f32", ""),
+                                              ((6, 2, 40), "f16", ""), ((20, 1, 64), "bf16", "1"), ((24, 1, 128), "f16", "0")])
+def test_replay_over_another_steps_plan_does_nothing_and_says_so(pkv, torch_cuda, monkeypatch, geom, dtype, tiles):
+    """A captured call is made for the counts of its step: over an image of others it leaves the output alone."""
+    torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
+    monkeypatch.setenv("PKV_DECODE_CLUSTER", "0")
+    n, shared = 70, 512
+    step = Step(torch, dtype, geom, [1] * n, [shared + 10 + 29 * i for i in range(n)], 16, seed=70, shared=shared)
+    step.token_seq = torch.arange(n, device="cuda", dtype=torch.int32)
+    plan = prefix_plan(pkv, step).build_host([k - 1 for k in step.kv_len], shared)
+    graph = captured(torch, lambda: attend_prefix(plan, step))
+    step.out.copy_(step.mark)
+    graph.replay()
+    step.check(pkv)
+    first = pkv._lib.SegmentPlan.from_buffer_copy(plan.plan)
+    shorter = [shared + (k - shared) // 3 for k in step.kv_len]
+    image = plan.build_host_image([k - 1 for k in shorter], shared)
+    assert first.n_items != plan.plan.n_items
+    replace_image(plan, image)
+    step.out.copy_(step.mark)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(step.out, step.mark)
+    assert pkv.debug_device_flags() == OTHER_PLAN
+    graph.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(pkv.PkvError, match="0x40"):                  # told by the next call, which runs nothing
+        attend_prefix(plan, step)
+    attend_prefix(plan, step)                                        # the present plan, called for itself
+    assert pkv.debug_device_flags() == OTHER_PLAN                    # (the device's own record of the replay before)
+    step.check(pkv, limits=shorter)
+    # the captured step's image again: the replay is whole again
+    image = plan.build_host_image([k - 1 for k in step.kv_len], shared)
+    replace_image(plan, image)
+    step.out.copy_(step.mark)
+    graph.replay()
+    step.check(pkv)
+
+
+def test_replay_over_an_image_of_the_same_layout(pkv, torch_cuda, monkeypatch):
+    torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
+    step = Step(torch, "bf16", TINY, [40, 40], [383, 1000], 16, seed=71)
+    plan = cross(pkv, step)
+    graph = captured(torch, lambda: attend(plan, step))
+    replace_image(plan, plan.build_host_image([40, 40], [300, 910]))
+    step.out.copy_(step.mark)
+    graph.replay()
+    step.check(pkv, limits=[300, 910])
+
+
+@pytest.mark.parametrize("geom,dtype", [(QWEN, "bf16"), (QWEN, "f32"), ((8, 2, 128), "f16")])
+def test_replays_of_the_cluster_form(pkv, torch_cuda, geom, dtype):
+    """Small steps read their positions only: captured once, they follow the images of later steps as long as every row has keys."""
+    torch = torch_cuda
+    n, shared, most = 3, 64, 700
+    step = Step(torch, dtype, geom, [1] * n, [shared + most] * n, 16, seed=73, shared=shared)
+    step.token_seq = torch.arange(n, device="cuda", dtype=torch.int32)
+    plan = prefix_plan(pkv, step).build_host([shared + 399, shared + 410, shared + 415], shared)
+    assert plan.plan.cluster > 0
+    before = pkv.lib().pkv_debug_cluster_launches()
+    graph = captured(torch, lambda: attend_prefix(plan, step))
+    assert pkv.lib().pkv_debug_cluster_launches() == before + 2
+    for grown in (0, 1, 60, 200, 284):
+        pos = [shared + 399 + grown, shared + 410 + grown, shared + 415 + grown]
+        replace_image(plan, plan.build_host_image(pos, shared))
+        step.out.copy_(step.mark)
+        graph.replay()
+        step.check(pkv, limits=[p + 1 for p in pos])
+
+    step = Step(torch, dtype, geom, [1] * n, [600, 500, 640], 16, seed=74)
+    plan = cross(pkv, step)
+    assert plan.plan.cluster > 0
+    graph = captured(torch, lambda: attend(plan, step))
+    replace_image(plan, plan.build_host_image([1] * n, [600, 0, 640]))       # a row without keys
+    step.out.copy_(step.mark)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(step.out, step.mark) and pkv.debug_device_flags() == OTHER_PLAN
+    replace_image(plan, plan.build_host_image([1] * n, [333, 20, 640]))
+    graph.replay()
+    step.check(pkv, limits=[333, 20, 640])

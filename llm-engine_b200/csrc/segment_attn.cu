@@ -479,6 +479,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
           sm_max[done & 1][g][half][r_in] = mx;
           meet();
+          // Where P lies over S, one warp's stores go over scores that the other has loaded: its loads (wait_ld, fence_before) come first.
+          if constexpr (S::kLead == 1) tc::fence_after();
           mx = fmaxf(mx, sm_max[done & 1][g][half ^ 1][r_in]);
           // O is free of the group's product before this one where that is awaited here, or where the next scores, which have
           // arrived, were issued behind it; so is P's place.

@@ -269,3 +269,46 @@ def test_replays_of_the_cluster_form(pkv, torch_cuda, geom, dtype):
     replace_image(plan, plan.build_host_image([1] * n, [333, 20, 640]))
     graph.replay()
     step.check(pkv, limits=[333, 20, 640])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("geom", [(256, 1, 64), (256, 1, 128), (200, 1, 64), (129, 1, 128), (128, 1, 64), (130, 2, 64), (256, 2, 128)])
+def test_many_query_heads_to_a_kv_head(pkv, torch_cuda, monkeypatch, dtype, geom):
+    """Up to a whole tile of one token's heads; pairs of kv heads with a full group each."""
+    torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
+    step = Step(torch, dtype, geom, [1, 3, 2], [700, 129, 1], 16, seed=80)
+    plan = cross(pkv, step)
+    assert plan.plan.n_tiles > 0 and plan.plan.n_items == 0
+    attend(plan, step)
+    step.check(pkv)
+    step = prefix_step(torch, geom, 3, 256, 40, seed=81)
+    plan = prefix_plan(pkv, step).build_host([k - 1 for k in step.kv_len], 256)
+    assert plan.plan.n_tiles > 0
+    attend_prefix(plan, step)
+    step.check(pkv)
+
+
+def test_streams_by_handle(pkv, torch_cuda):
+    """Plans made and used on a stream named by its handle, the default stream's among them."""
+    torch = torch_cuda
+    side = torch.cuda.Stream()
+    for handle in (side.cuda_stream, 0, side):
+        step = prefix_step(torch, TINY, 20, 128, 50, seed=82)
+        source = Step(torch, "bf16", TINY, [2] * 10, [77 * i for i in range(10)], 16, seed=83)
+        plan = prefix_plan(pkv, step)
+        other = pkv.CrossPlan(source.n, 10, *TINY, 16, torch.bfloat16)
+        decode = pkv.DecodePlan(step.n, *TINY)
+        pos = torch.tensor([k - 1 for k in step.kv_len], dtype=torch.int32, device="cuda")
+        out = step.mark.clone()
+        torch.cuda.synchronize()
+        for _ in range(2):
+            plan.build_host([k - 1 for k in step.kv_len], 128, stream=handle)
+            other.build_host(source.q_len, source.kv_len, stream=handle)
+            decode.build_host([k - 1 for k in step.kv_len], stream=handle)
+            attend_prefix(plan, step, stream=handle)
+            other.attention(source.q, source.kc, source.vc, source.block_tables, source.table_offset, source.out, source.scale, stream=handle)
+            decode.attention(step.q, step.kc, step.vc, step.block_tables, step.table_offset, step.token_seq, pos, out, 16, step.scale, stream=handle)
+        step.check(pkv)
+        source.check(pkv)
+        step.check(pkv, out=out)

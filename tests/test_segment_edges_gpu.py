@@ -312,3 +312,16 @@ def test_streams_by_handle(pkv, torch_cuda):
         step.check(pkv)
         source.check(pkv)
         step.check(pkv, out=out)
+
+
+@pytest.mark.parametrize("geom", [(1, 1, 64), (1, 1, 128), (3, 3, 64), (5, 5, 128), (2, 1, 64)])
+def test_few_heads(pkv, torch_cuda, monkeypatch, geom):
+    """A kv head without a partner; a tile of 128 or 256 tokens."""
+    torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", "1")
+    step = Step(torch, "bf16", geom, [257, 1, 128, 300], [1000, 129, 64, 2000], 16, seed=84)
+    attend(cross(pkv, step), step)
+    step.check(pkv)
+    step = prefix_step(torch, geom, 300, 1024, 30, seed=85)
+    attend_prefix(prefix_plan(pkv, step).build_host([k - 1 for k in step.kv_len], 1024), step)
+    step.check(pkv)

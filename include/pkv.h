@@ -140,7 +140,8 @@ int pkv_rope_append_f32(void* q, const void* k, const void* v, const int* positi
  *   k_cache[slots[t]][h][:] <- rope(y of k[t][h], positions[t])
  *   v_cache[slots[t]][:]    <- v[t][:]
  * with the rotation and the tables of pkv_rope_append_*.  fp32 arithmetic, one rounding
- * to the element type at the end.  Weights are [head_dim], of the element type.
+ * to the element type at the end (a head whose squares pass the range of fp32, values beyond 1e18 or so, comes out
+ * as zero).  Weights are [head_dim], of the element type.
  * q, k and v rows are q_stride, k_stride and v_stride ELEMENTS apart, so they may be
  * column ranges of one projection's output; q_out is [n_tokens][q_heads*head_dim], and
  * may be q itself if q's rows are contiguous (no other overlap is allowed).
@@ -467,8 +468,10 @@ int pkv_prefill_attn_f16(const void* q, const void* k_cache, const void* v_cache
  *
  * pkv_prefix_*: pkv_decode_attn_* for tokens whose sequences all begin with the same
  * prefix_len positions in the same blocks (as KVCacheManager::allocate_prompt shares them,
- * src/kv_cache/block_allocator.cpp:28-78).  The prefix is worked through once for all tokens
- * together, through the table of one of them, each token's other keys as ever.  The index
+ * src/kv_cache/block_allocator.cpp:28-78).  Where the tensor-core kernel takes the geometry and the
+ * planner reckons that it pays, the prefix is worked through once for all tokens together, through
+ * the table of one of them, and each token's other keys as ever; elsewhere every token reads all of
+ * its keys, as in pkv_decode_attn_*.  The index
  * arrays are those of pkv_decode_attn_*, with the whole tables; that they agree on the
  * prefix is the caller's word.  A token whose position lies inside the prefix sees the keys up
  * to its own position only.  (pkv_decode_plan_host_shared finds common prefixes by itself and

@@ -11,8 +11,8 @@
 // 16 bytes.  A v head is a head without the arithmetic.  Steps that fill the GPU give a lane the same piece of two heads of
 // one token, which share the token's cos / sin: 8,191 tokens of 32/8 heads of 128, bf16 (206 MB), 48 us with one head a
 // lane, 43 with two, 71 with four (94 registers).  Steps whose rows do not fit L2 read and write them as data that is
-// not used again: 36.5 us, 5.6 TB/s; 1,024 tokens lose a tenth that way (6.2 and 6.9), and the launch behind them finds
-// its q, K and V in L2.  Sending for the rows before the position is known: 36.2 -> 38.2 us.
+// not used again: 36.5 us, 5.6 TB/s.  (The same rows again and again, kept and streamed: 2,048 tokens, 50 MB, 9.6 us both; 4,096,
+// 101 MB, 21.4 and 18.2.  Below the border the launch behind finds its q, K and V in L2.)  Sending for the rows before the position is known: 36.2 -> 38.2 us.
 #include "common.cuh"
 #include "launch_util.hpp"
 #include "status.hpp"
@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormAr
   }
 }
 
-// Any even head_dim, any alignment and strides: a warp a head, a rotation pair a lane at a time.
+// Any even head_dim, any alignment and strides: a warp a head, a rotation pair a lane at a time.  An element a load, rows read
+// twice: 8,191 tokens of 32/8 heads of 96, bf16, 182 us (a copy of the rows 24), 256 tokens 5.8.
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_pairs_kernel(const NormArgs<T> a) {
   pdl_launch_dependents();

@@ -31,7 +31,7 @@
 // Measured on B200: a key tile of both groups takes about 3,500 cycles at head_dim 128 (products 2,048, exponentials 2,048, the rest a
 // group's chain of load, maximum, exponentials, store that one other group does not cover) and 3,200 at 64 (products 1,024; the issuing
 // warp's waits); an item's start and end 5,000.  4 sequences of 1,000 - 2,048 tokens and 4,000 - 6,500 keys, 32/8 heads of 128 dims: 593 us,
-// 1,155 TFLOP/s, in a burst (650 under the power cap).  24 of 3 - 448 tokens and 100 - 1,500 keys, 16/16 heads of 64: 50 us.
+// 1,155 TFLOP/s, in a burst (688, 995, over seconds, under the power cap).  24 of 3 - 448 tokens and 100 - 1,500 keys, 16/16 heads of 64: 50 us.
 //
 // Blocks are persistent, one on an SM, each with a list of items of its own.  Every wait is bounded: one that runs
 // out sets bit 32 of the error word and the block winds down.
@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         };
         // Products of one thread run in order: where P lies over S, the group's next scores overwrite it behind these.
         auto values = [&](int g, uint32_t v_addr, bool first, bool final) {
-          // (a look first: 242 us against 247 for full tiles at 64 dims, 660 against 647 for the largest case at 128)
+          // (a look first: 242 us against 247 for full tiles at 64 dims; at 128, the largest case over seconds, 691 against 688, and
+          // 695 where the softmax threads look first too)
           if constexpr (D == 64) WAIT(BAR(P_FULL + g), (done >> g) & 1);
           else BLOCK(BAR(P_FULL + g), (done >> g) & 1);
           tc::fence_after();
@@ -878,7 +879,7 @@ int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* 
   if (st != PKV_OK) return st;
   std::vector<int> seq(g.n_tokens, -1), pos(g.n_tokens, -1), empty, start(n_seqs);
   long long next = 0;
-  int listed = 0, most = 0;
+  int listed = 0;
   for (int s = 0; s < n_seqs; ++s) {
     const long long at = q_start ? q_start[s] : next;
     if (kv_len[s] > kMostKeys) return fail(PKV_E_UNSUPPORTED, "%s: sequence %d has %d keys; at most 2^30", fn, s, kv_len[s]);
@@ -887,7 +888,6 @@ int plan_cross(const char* fn, const int* q_start, const int* q_len, const int* 
     next = at + q_len[s];
     start[s] = static_cast<int>(at);
     listed += q_len[s];
-    if (kv_len[s] > 0) most = std::max(most, q_len[s]);
     for (int t = start[s]; t < next; ++t) {
       if (seq[t] >= 0) return fail(PKV_E_ARG, "%s: row %d belongs to sequences %d and %d", fn, t, seq[t], s);
       seq[t] = s;

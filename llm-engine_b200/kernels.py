@@ -501,8 +501,9 @@ class CrossPlan(_SegmentPlan):
 
 
 class PrefixPlan(_SegmentPlan):
-    """Decode attention of tokens whose sequences all begin with the same blocks: the prefix is worked through once
-    for all of them."""
+    """Decode attention of tokens whose sequences all begin with the same blocks.  16-bit K/V at head_dim 64 or 128 in blocks of a power
+    of two of at least 16 slots: the prefix is worked through once for all of them, where that is reckoned to pay; else
+    as launch_attention_decode.  A captured call serves the step it was captured in."""
 
     def __init__(self, n_tokens: int, q_heads: int, kv_heads: int, head_dim: int, block_size: int, dtype, num_blocks: int = 0, workspace=None,
                  device="cuda"):

@@ -380,6 +380,18 @@ class DecodePlan:
         _lib.check(fn, st)
 
 
+def _int32(a):
+    """`a` as a contiguous int32 array; what would come out as other numbers (2^32 + 5 as 5, 1.5 as 1) is refused."""
+    import numpy as np
+    given = np.asarray(a)
+    if given.dtype.kind in "iubf":
+        with np.errstate(invalid="ignore"):
+            out = np.ascontiguousarray(given, dtype=np.int32)
+        if given.dtype == np.int32 or np.array_equal(out, given):
+            return out
+    raise ValueError("lengths and positions must be whole numbers of 32 bits")
+
+
 class _SegmentPlan:
     """Work list of attention in which many rows see the same keys, built once per step on the host and used by
     every layer's call (include/pkv.h, pkv_segment_plan).  Its calls share one workspace: those that may
@@ -469,8 +481,7 @@ class CrossPlan(_SegmentPlan):
         self.n_seqs = n_seqs
 
     def _lengths(self, q_len, kv_len, q_start):
-        import numpy as np
-        arrays = [None if a is None else np.ascontiguousarray(a, dtype=np.int32) for a in (q_start, q_len, kv_len)]
+        arrays = [None if a is None else _int32(a) for a in (q_start, q_len, kv_len)]
         for a in arrays:
             if a is not None and a.shape != (self.n_seqs,):
                 raise ValueError(f"the plan is for {self.n_seqs} sequences")
@@ -510,8 +521,7 @@ class PrefixPlan(_SegmentPlan):
         super().__init__("pkv_prefix_workspace_bytes", n_tokens, q_heads, kv_heads, head_dim, block_size, dtype, num_blocks, workspace, device)
 
     def _positions(self, token_pos):
-        import numpy as np
-        pos = np.ascontiguousarray(token_pos, dtype=np.int32)
+        pos = _int32(token_pos)
         if pos.shape != (self.n_tokens,):
             raise ValueError(f"the plan is for {self.n_tokens} tokens")
         return pos

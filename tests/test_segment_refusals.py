@@ -18,6 +18,25 @@ def host(pkv, monkeypatch):
     return torch, called
 
 
+def test_lengths_that_do_not_fit_are_refused(pkv, host):
+    import numpy as np
+    torch, _ = host
+    ws = torch.zeros(1 << 22, dtype=torch.uint8)
+    cross = pkv.CrossPlan(3, 3, 4, 2, 64, 16, torch.bfloat16, workspace=ws)
+    prefix = pkv.PrefixPlan(3, 4, 2, 64, 16, torch.bfloat16, workspace=ws)
+    good = cross.build_host_image([1] * 3, [5, 6, 7])
+    for same in (np.array([5, 6, 7]), np.array([5, 6, 7], np.uint8), torch.tensor([5, 6, 7]), (5, 6, 7), np.arange(5, 8, dtype=np.uint64), np.array([5.0, 6.0, 7.0])):
+        assert cross.build_host_image([1] * 3, same) == good
+    every_second = np.array([5, 0, 6, 0, 7], np.int32)[::2]
+    assert cross.build_host_image([1] * 3, every_second) == good and prefix.build_host_image(every_second, 0) > 0
+    for bad in ([5, 6, 2 ** 32 + 7], np.array([5, 6, -2 ** 32]), np.array([5, 6, 2 ** 31]), np.array([2 ** 32 - 1] * 3, np.uint32), [5, 6, 7.5],
+                np.array([5.0, 6.0, float("nan")]), ["5", "6", "7"]):
+        for call in (lambda: cross.build_host_image([1] * 3, bad), lambda: cross.build_host_image(bad, [5, 6, 7]),
+                     lambda: cross.build_host_image([1] * 3, [5, 6, 7], q_start=bad), lambda: prefix.build_host_image(bad, 0)):
+            with pytest.raises(ValueError):
+                call()
+
+
 @pytest.mark.parametrize("kind", ["cross", "prefix"])
 def test_pools_and_blocks_belong_together(pkv, host, kind):
     torch, called = host

@@ -325,3 +325,54 @@ def test_few_heads(pkv, torch_cuda, monkeypatch, geom):
     step = prefix_step(torch, geom, 300, 1024, 30, seed=85)
     attend_prefix(prefix_plan(pkv, step).build_host([k - 1 for k in step.kv_len], 1024), step)
     step.check(pkv)
+
+
+@pytest.mark.parametrize("geom,n,shared", [(TINY, 60, 640), (WIDE, 70, 2048), (QWEN, 3, 64)])
+@pytest.mark.parametrize("tiles", ["", "1", "0"])
+def test_layers_back_to_back_over_the_same_buffers(pkv, torch_cuda, monkeypatch, geom, n, shared, tiles):
+    """Every layer writes q, and its tokens' rows of the pools, where the layer before had them, with launches of this library alone
+    between: each sees what its own norm pass left, launched eagerly or replayed, as when the layers run one by one."""
+    torch = torch_cuda
+    monkeypatch.setenv("PKV_SEGMENT_TILES", tiles)
+    qh, kvh, hd = geom
+    layers = 12
+    step = prefix_step(torch, geom, n, shared, 90, seed=90)
+    plan = prefix_plan(pkv, step).build_host([k - 1 for k in step.kv_len], shared)
+    source = Step(torch, "bf16", geom, [1 + i % 3 for i in range(n)], [40 + 13 * i for i in range(n)], 16, seed=91)
+    encoder = cross(pkv, source)
+    g = torch.Generator(device="cuda").manual_seed(92)
+    rows = torch.randn((layers, n, (qh + 2 * kvh) * hd), generator=g, device="cuda").to(step.q.dtype)
+    parts = [r.split([qh * hd, kvh * hd, kvh * hd], dim=1) for r in rows]
+    w = torch.ones(hd, device="cuda", dtype=step.q.dtype)
+    pos = torch.tensor([k - 1 for k in step.kv_len], dtype=torch.int32, device="cuda")
+    slots = torch.stack([s[-1] for s in step.slots]).int()
+    angle = torch.rand((max(step.kv_len), hd // 2), generator=g, device="cuda") * 6.28
+    cos, sin = angle.cos().contiguous(), angle.sin().contiguous()
+    outs, encs = ([torch.empty_like(x.mark) for _ in range(layers)] for x in (step, source))
+
+    def layer(i):
+        q, k, v = parts[i]
+        pkv.launch_qk_norm_rope_store_kv(q, k, v, w, w, 1e-6, pos, cos, sin, slots, step.q, step.kc, step.vc, n, qh, kvh, hd)
+        plan.attention(step.q, step.kc, step.vc, step.block_tables, step.table_offset, step.token_seq, outs[i], step.scale)
+        encoder.attention(source.q, source.kc, source.vc, source.block_tables, source.table_offset, encs[i], source.scale)
+
+    want = []
+    for i in range(layers):
+        layer(i)
+        torch.cuda.synchronize()
+        step.out.copy_(outs[i])
+        step.check(pkv)
+        want.append((outs[i].clone(), encs[i].clone()))
+
+    def run():
+        for i in range(layers):
+            layer(i)
+
+    graph = captured(torch, run)
+    for go in (run, graph.replay) * 4:
+        for t in outs + encs:
+            t.fill_(float("nan"))
+        go()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, x) and torch.equal(b, y) for a, b, (x, y) in zip(outs, encs, want))
+    assert pkv.debug_device_flags() == 0
